@@ -198,6 +198,8 @@ enum {
   OCT_B200_DETAIL_TP_NCCL = -7022,           /* communicator or peer-memory setup failed */
   OCT_B200_DETAIL_TP_NOT_FOUND = -7023,      /* unknown tensor-parallel SGEMM id */
   OCT_B200_DETAIL_TP_EXEC = -7024,           /* a kernel, copy or collective of the call failed */
+  OCT_B200_DETAIL_KV4_BAD_INDEX = -7030,     /* a page number, length or row range on the device was out of range */
+  OCT_B200_DETAIL_KV4_WORKSPACE = -7031,     /* workspace missing or smaller than the call needs */
 };
 
 /* ---- reductions (reactor_api.h:375-581) ---- */
@@ -1527,6 +1529,147 @@ PROM_REACTOR_API int oct_b200_attention_device(void* handle, const float* d_q, c
                                                float* d_out, uint32_t items, uint32_t seq, uint32_t heads,
                                                uint32_t head_dim, float scale, void* stream, int* out_detail_code);
 
+/* ---- token-by-token serving: head norm + rotation, a cache in 4 bits, attention over it ----
+   No counterparts in the reference's C ABI: its RoPE, head RMSNorm and raw scores
+   (reactor_api.h:2694-2712) take host buffers of a whole sequence.  Every call
+   below enqueues on `stream` (NULL = the CUDA default stream) and returns; it
+   allocates nothing, keeps nothing between calls and may be captured into a
+   CUDA graph.  Pointers are device pointers of the handle's GPU unless stated
+   otherwise, 16-byte aligned where they point at elements; strides count
+   elements and make every row start on 16 bytes; the channels of a row are
+   adjacent.  Errors: OCT_B200_DETAIL_INVALID_ARGUMENT, _UNALIGNED,
+   _UNSUPPORTED_SHAPE, _KV4_WORKSPACE, and PROM_DETAIL_CAPABILITY_MISMATCH on a
+   handle without a device.  Nothing is enqueued by a call that fails. */
+enum { OCT_B200_F32 = 0u, OCT_B200_BF16 = 1u, OCT_B200_F16 = 2u };
+
+/* RMSNorm of every query and key head, then the rotation to its position, in
+   one pass.  Per head row x of head_dim channels:
+     y = x / sqrt(mean(x^2) + eps) * weight     (y = x when normalize is 0; no weight when NULL)
+     pair j of rotary_dim / 2 turns by positions[token][axis of j] * frequencies[j]:
+       (a, b) -> (a cos - b sin, b cos + a sin)
+     half-split pairs are channels (j, j + rotary_dim/2), interleaved ones
+     (2j, 2j + 1); the first axis_pairs[0] pairs belong to axis 0, the next
+     axis_pairs[1] to axis 1, and so on; channels from rotary_dim on keep y.
+   Statistics and rotation are fp32, angles binary64; outputs are rounded once.
+   An output may be its own input (same pointer and strides) and overlap no
+   other part of one.  q or k may be absent (0 heads). */
+typedef struct OctB200QkNormRopeRequest {
+  uint32_t struct_size;
+  uint32_t dtype;      /* OCT_B200_F32 / _BF16 / _F16, of q, k and their outputs */
+  uint64_t tokens;
+  uint32_t q_heads, k_heads;
+  uint32_t head_dim;   /* a multiple of 16, <= 512 */
+  uint32_t rotary_dim; /* a multiple of 16, <= head_dim */
+  uint32_t interleaved, normalize;
+  float eps;           /* > 0 */
+  uint32_t axes;       /* 1..4 */
+  uint32_t axis_pairs[4]; /* sum over the axes: rotary_dim / 2 */
+  const void *q, *k;   /* [tokens][heads][head_dim] by their strides */
+  void *q_out, *k_out;
+  uint64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  uint64_t q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
+  const float *q_weight, *k_weight; /* [head_dim] or NULL */
+  const int32_t* positions;         /* [tokens][axes], rows position_stride apart; 4-byte aligned */
+  uint64_t position_stride;
+  const double* frequencies;        /* [rotary_dim / 2], radians per position; 8-byte aligned */
+} OctB200QkNormRopeRequest;
+PROM_REACTOR_API int oct_b200_qk_norm_rope_device(void* handle, const OctB200QkNormRopeRequest* request,
+                                                  void* stream, int* out_detail_code);
+
+/* The cache: `pages` pages of page_size tokens for kv_heads key heads.  Rows are
+   quantised in groups of 32 channels to codes 0..15 with a scale and a zero:
+     x clamped to +-65504;  z = greatest float16 <= min x;  s = least float16 with z + 15 s >= max x;
+     code = (x - z) / s rounded to nearest, ties to even (0 when s = 0);  value = z + s * code.
+   A NaN makes the 32 values of its group NaN; float16 outputs are clamped to +-65504.  Layout of `data`
+   ([pages][kv_heads][page_size / 16] tiles of oct_b200_kv4_tile_bytes(head_dim) bytes):
+     key codes [16][head_dim / 2] | key (s, z) float16 pairs [16][head_dim / 32] | the same of the values;
+   in a row of codes, channels 32 j + 4 g + 0..3 are halfword g * (head_dim / 32) + j, channel + 0 lowest. */
+typedef struct OctB200Kv4Cache {
+  uint32_t struct_size;
+  uint32_t page_size; /* a multiple of 16, <= 65536 */
+  uint32_t kv_heads;
+  uint32_t head_dim;  /* 64, 128 or 256 */
+  uint32_t pages;
+  uint32_t reserved;  /* 0 */
+  void* data;
+} OctB200Kv4Cache;
+/* Bytes of a 16-token tile of one key head; of the whole cache: pages * kv_heads * (page_size / 16) of them.
+   0 for a head_dim that is not supported. */
+PROM_REACTOR_API uint64_t oct_b200_kv4_tile_bytes(uint32_t head_dim);
+
+/* The sequences of a call.  Sequence b brings rows cu_tokens[b] .. cu_tokens[b + 1] - 1
+   of the call's tensors (row b alone when cu_tokens is NULL); they are its last
+   tokens, at positions kv_lens[b] - their count onward.  Position p lies in page
+   page_table[b][p / page_size].  Arrays on the device are checked there against
+   the bounds below: a sequence whose length or rows do not fit, and a row or
+   16-token tile whose page is not one of the cache's, is skipped (rows of it are
+   not written, keys of it not seen) and reported by oct_b200_sync_status as
+   OCT_B200_DETAIL_KV4_BAD_INDEX.  Rows behind the last sequence are left as they
+   were.  Two sequences of one call must not write the same position of a page. */
+typedef struct OctB200Kv4Batch {
+  uint32_t struct_size;
+  uint32_t batch;              /* sequences, <= 65535 */
+  const int32_t* page_table;   /* [batch][page_table_width], rows page_table_stride apart */
+  uint64_t page_table_stride;
+  uint32_t page_table_width;
+  uint32_t max_tokens;         /* most rows of one sequence */
+  uint32_t max_kv_len;         /* longest sequence; <= page_table_width * page_size */
+  uint32_t reserved;           /* 0 */
+  const int32_t* kv_lens;      /* [batch] tokens held, the call's own rows among them */
+  const int32_t* cu_tokens;    /* [batch + 1] or NULL */
+} OctB200Kv4Batch;
+
+/* Key and value rows of a call: [tokens][kv_heads][head_dim] by their strides. */
+typedef struct OctB200Kv4Rows {
+  uint32_t struct_size;
+  uint32_t dtype;
+  uint64_t tokens;
+  void *k, *v; /* read by the store, written by the load */
+  uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} OctB200Kv4Rows;
+/* Quantises the rows into the cache / reads the same positions back. */
+PROM_REACTOR_API int oct_b200_kv4_store_device(void* handle, const OctB200Kv4Cache* cache,
+                                               const OctB200Kv4Batch* batch, const OctB200Kv4Rows* rows,
+                                               void* stream, int* out_detail_code);
+PROM_REACTOR_API int oct_b200_kv4_load_device(void* handle, const OctB200Kv4Cache* cache,
+                                              const OctB200Kv4Batch* batch, const OctB200Kv4Rows* rows,
+                                              void* stream, int* out_detail_code);
+
+/* Attention of the rows' queries over the cached keys and values of their
+   sequence: out = softmax(scale q k^T) v, query head h with key head
+   h / (q_heads / kv_heads).  With causal, the query at position p sees keys <= p
+   and, with a window, keys > p - window; without, every key of its sequence.  A
+   query that sees nothing gets zeros and lse = -inf.  lse (may be NULL) is the
+   natural logarithm of the softmax's sum, [tokens][q_heads].  The workspace
+   (oct_b200_kv4_attention_workspace_bytes of the same sizes; NULL when that is
+   0) is used between this call's kernels only: calls that may run at the same
+   time, graphs too, need one each.  Meant for the few tokens of a decode or
+   verification step; more work the same, 8 to 32 rows of (token, query head) per
+   pass over the keys. */
+typedef struct OctB200Kv4AttentionRequest {
+  uint32_t struct_size;
+  uint32_t dtype;    /* of q and out */
+  uint32_t q_heads;  /* a multiple of kv_heads */
+  uint32_t causal;
+  uint32_t window;   /* 0: none; needs causal */
+  float scale;       /* finite */
+  uint64_t tokens;
+  const void* q;     /* [tokens][q_heads][head_dim] by its strides */
+  void* out;
+  uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  float* lse;
+  void* workspace;
+  uint64_t workspace_bytes;
+} OctB200Kv4AttentionRequest;
+/* Host arithmetic on sizes alone: no handle, no device. */
+PROM_REACTOR_API int oct_b200_kv4_attention_workspace_bytes(const OctB200Kv4Cache* cache, const OctB200Kv4Batch* batch,
+                                                            const OctB200Kv4AttentionRequest* request,
+                                                            uint64_t* out_bytes, int* out_detail_code);
+PROM_REACTOR_API int oct_b200_kv4_attention_device(void* handle, const OctB200Kv4Cache* cache,
+                                                   const OctB200Kv4Batch* batch,
+                                                   const OctB200Kv4AttentionRequest* request, void* stream,
+                                                   int* out_detail_code);
+
 /* Test-only, no reference counterpart: runs the tensor-parallel peer-wait
    kernel against a flag that nothing sets, with a wall-clock budget of
    budget_ns (1 ms .. 1 s).  The wait must give up, record its error bit and
@@ -1536,8 +1679,9 @@ PROM_REACTOR_API int oct_b200_selftest_wait_timeout(void* handle, uint64_t budge
 
 /* Waits for `stream` (NULL: the CUDA default stream), then reads and
    clears the device status words the kernels write: returns PROM_ERROR with
-   OCT_B200_DETAIL_DEVICE_TIMEOUT if a bounded in-kernel wait gave up, or
-   PROM_REDUCTION_DETAIL_NONFINITE_INPUT if a reduction saw NaN/Inf. */
+   OCT_B200_DETAIL_DEVICE_TIMEOUT if a bounded in-kernel wait gave up,
+   OCT_B200_DETAIL_KV4_BAD_INDEX if a cache call skipped what its indices named,
+   or PROM_REDUCTION_DETAIL_NONFINITE_INPUT if a reduction saw NaN/Inf. */
 PROM_REACTOR_API int oct_b200_sync_status(void* handle, void* stream, int* out_detail_code);
 
 /* No counterpart in the reference.  C = A * B on device pointers (row-major,

@@ -1,0 +1,758 @@
+// kv4_attention.cu -- attention of a few query tokens per sequence over the
+// 4-bit paged cache (the single-token form of the attention that the blocks
+// run over whole sequences; the reference has neither a cache nor this step).
+//
+// For a query row and the keys p it sees (p <= its own position, and within
+// the window when there is one):
+//   score_p = scale * sum_j (s_pj (q . code)_pj + z_pj sum(q)_j),   j over groups of 32 channels
+//   out     = sum_p w_p (z_pj + s_pj code_p) / sum_p w_p,           w_p = exp(score_p - max)
+// so the codes enter the matrix products as integers and the scales, zeros and
+// softmax stay in fp32.
+//
+// Codes as operands.  A code masked out of its word into the low bits of a
+// float16 IS the number code * 2^-24 (a subnormal, exact in the tensor cores),
+// and one nibble further up code * 2^-20.  So four ANDs and one shift turn
+// eight codes into matrix operands, with no conversion and no unpacking; the
+// powers of two are undone on the other operand (q / 16 for the upper nibbles)
+// and at the end.  q is scaled per row by a power of two that puts its largest
+// value near 2^10, so that as float16 (one part for 16-bit inputs, two for fp32)
+// it keeps its digits.
+//
+// Tokens are the rows of both products (m16n8k16: 16 tokens, 8 query rows), so
+// one warp works through 16 keys at a time for 8 query rows -- the query heads
+// that share a key head -- and the scores' fragment becomes the second
+// product's operand with one 8 x 8 transposition per 8 tokens.
+//
+// Bound: HBM at a decode batch, reading each cached key once; the tensor pipe
+// has nothing to do beside it, which is why this runs on warp-level matrix
+// instructions whose operands come from registers instead of through tcgen05
+// and tensor memory.  Each warp streams its own tiles (16 tokens, keys and
+// values side by side, one bulk copy) through a private ring in shared memory:
+// no barrier between warps until the end.
+//
+// Keys are split over blocks when the (sequence, key head) pairs do not fill
+// the GPU; the partial results are joined in a second kernel, in split order.
+#include <type_traits>
+
+#include "kernels.h"
+#include "ptx.cuh"
+#include "serving.cuh"
+
+namespace oct {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// The running maximum is renewed only when a score exceeds it by this much (in
+// powers of two): weights stay below 2^8, and most tiles skip the exchange.
+constexpr float kSlack = 8.f;
+constexpr float kCodeLow = 16777216.f, kCodeHigh = 1048576.f;  // 2^24, 2^20
+
+template <int D>
+struct Geometry {
+  static constexpr int kGroups = D / 32;
+  static constexpr int kRowBytes = D / 2;
+  static constexpr int kKeyParams = 16 * kRowBytes;
+  static constexpr int kValues = kKeyParams + 16 * kGroups * 4;
+  static constexpr int kValueParams = kValues + 16 * kRowBytes;
+  static constexpr int kBytes = 2 * kValues;
+  // ring of tiles per warp: about 10 to 20 KB, and room for the warp's result at the end
+  static constexpr int kStages = D == 64 ? 8 : 4;
+};
+
+// Query rows of one block in groups of 8, by what the accumulators leave of the registers.
+template <int D> constexpr int kMaxRowGroups = D == 64 ? 4 : (D == 128 ? 2 : 1);
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+// a power of two with the exponent of x shifted to `target`; 1 for zero and non-finite x
+__device__ __forceinline__ float pow2_toward(float x, int target) {
+  const int e = static_cast<int>((__float_as_uint(x) >> 23) & 255u);
+  if (e == 0 || e == 255) return 1.f;
+  const int f = target + 127 - (e - 127);
+  return __uint_as_float(static_cast<uint32_t>(f < 1 ? 1 : (f > 254 ? 254 : f)) << 23);
+}
+
+template <int N>
+__device__ __forceinline__ void lds(uint32_t (&w)[N], const uint8_t* p) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 16 * i);
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  }
+}
+
+struct KernelArgs {
+  Kv4View view;
+  const void* q;
+  void* out;
+  uint64_t q_token, q_head, out_token, out_head;
+  float* lse;
+  float scale_log2;
+  uint32_t heads, share;  // query heads, query heads of one key head
+  uint32_t causal, window;
+  uint32_t row_tiles, span, splits;
+  float* part_o;   // [splits][tokens * heads][D]
+  float2* part_ml; // [splits][tokens * heads]
+  unsigned int* err;
+};
+
+// The keys that the rows of one row tile see: row r of a sequence is query
+// token r / share, whose own position is last.
+struct Rows {
+  uint32_t first, count;  // rows of the tile inside the sequence
+  int32_t lo_min, lo_max, hi_min, hi_max;
+  int32_t t_begin, t_end;  // 16-key tiles
+};
+__device__ __forceinline__ int32_t row_hi(const KernelArgs& a, const Kv4Seq& s, uint32_t row) {
+  return a.causal ? static_cast<int32_t>(s.len) - static_cast<int32_t>(s.n) + static_cast<int32_t>(row / a.share)
+                  : static_cast<int32_t>(s.len) - 1;
+}
+__device__ __forceinline__ int32_t row_lo(const KernelArgs& a, int32_t hi) {
+  const int64_t lo = static_cast<int64_t>(hi) - a.window + 1;
+  return a.window == 0 || lo < 0 ? 0 : static_cast<int32_t>(lo);
+}
+__device__ __forceinline__ bool row_range(const KernelArgs& a, const Kv4Seq& s, uint32_t tile, uint32_t rows_per_tile,
+                                          Rows* r) {
+  const uint32_t rows = s.n * a.share;
+  r->first = tile * rows_per_tile;
+  if (r->first >= rows) return false;
+  r->count = min(rows_per_tile, rows - r->first);
+  r->hi_min = row_hi(a, s, r->first);
+  r->hi_max = row_hi(a, s, r->first + r->count - 1);
+  r->lo_min = row_lo(a, r->hi_min);
+  r->lo_max = row_lo(a, r->hi_max);
+  r->t_begin = r->lo_min / static_cast<int32_t>(kKv4Tile);
+  r->t_end = r->hi_max < 0 ? r->t_begin : r->hi_max / static_cast<int32_t>(kKv4Tile) + 1;
+  return true;
+}
+
+template <typename T, int D, int NT, int QP, int PP>
+__global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const KernelArgs a) {
+  using G = Geometry<D>;
+  constexpr int NG = G::kGroups;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kWarps][G::kStages];
+  __shared__ uint32_t loaded[kWarps][G::kStages];
+  __shared__ float2 warp_ml[kWarps][8 * NT];
+
+  griddep_launch_dependents();
+  const uint32_t split = blockIdx.x, head = blockIdx.y / a.row_tiles, b = blockIdx.z;
+  Kv4Seq seq;
+  if (!kv4_seq(a.view, b, &seq)) return;
+  Rows rows;
+  if (!row_range(a, seq, blockIdx.y % a.row_tiles, 8 * NT, &rows)) return;
+  const int32_t t0 = rows.t_begin + static_cast<int32_t>(split * a.span);
+  const int32_t t1 = min(rows.t_end, t0 + static_cast<int32_t>(a.span));
+  if (t0 >= t1 && split > 0) return;  // the join looks at no split behind the last key
+
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, i4 = lane % 4;
+  const int32_t tiles = t0 + static_cast<int32_t>(warp) < t1 ? (t1 - t0 - static_cast<int32_t>(warp) + kWarps - 1) / kWarps : 0;
+  uint8_t* ring = smem + warp * (G::kStages * G::kBytes);
+  if (lane == 0) {
+    for (int st = 0; st < G::kStages; ++st) mbar_init(&bars[warp][st], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+
+  // Page numbers of this warp's next 32 tiles, one per lane.
+  const int32_t* table = a.view.table + b * a.view.table_stride;
+  uint32_t pages = 0;
+  auto fetch_pages = [&](int32_t k0) {
+    const int32_t k = k0 + static_cast<int32_t>(lane);
+    const int32_t t = t0 + static_cast<int32_t>(warp) + k * kWarps;
+    pages = k < tiles ? static_cast<uint32_t>(table[static_cast<uint32_t>(t) / a.view.page_tiles]) : 0u;
+  };
+  auto issue = [&](int32_t k) {  // tile k of this warp into its stage (whole warp)
+    if (k % 32 == 0) fetch_pages(k);
+    const uint32_t page = __shfl_sync(0xffffffffu, pages, k % 32);
+    const int32_t t = t0 + static_cast<int32_t>(warp) + k * kWarps;
+    const int st = k % G::kStages;
+    if (lane == 0) {
+      const bool ok = page < a.view.pages;
+      loaded[warp][st] = ok;
+      if (ok) {
+        mbar_arrive_expect_tx(&bars[warp][st], G::kBytes);
+        bulk_load(ring + st * G::kBytes,
+                  kv4_tile(a.view, page, head, static_cast<uint32_t>(t) % a.view.page_tiles, G::kBytes), G::kBytes,
+                  &bars[warp][st]);
+      } else {
+        atomicOr(a.view.bad, 1u);
+        mbar_arrive(&bars[warp][st]);
+      }
+    }
+  };
+  for (int32_t k = 0; k < min(tiles, G::kStages - 1); ++k) issue(k);
+
+  // Query fragments: column g of group nt is row rows.first + 8 nt + g.
+  uint32_t qf[NT][NG][2][2][QP];
+  float kf[NT][2], qs[NT][NG][2];  // for this lane's score columns 2 i4, 2 i4 + 1
+  int32_t hi[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const uint32_t col = 8 * nt + g;
+    float v[NG][8];
+    float amax = 0.f;
+    if (col < rows.count) {
+      const uint32_t row = rows.first + col;
+      const T* p = static_cast<const T*>(a.q) + (seq.row0 + row / a.share) * a.q_token +
+                   (head * a.share + row % a.share) * a.q_head + 8 * i4;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) load8(p + 32 * j, v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+    }
+    float sums[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s += v[j][e];
+        amax = fmaxf(amax, fabsf(v[j][e]));
+      }
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      sums[j] = s * a.scale_log2;
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const float nq = pow2_toward(amax, 10);
+    const float factor = kCodeLow / nq * a.scale_log2;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int from = (2 * i4 + c) * 4;
+      kf[nt][c] = __shfl_sync(0xffffffffu, factor, from);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) qs[nt][j][c] = __shfl_sync(0xffffffffu, sums[j], from);
+      const uint32_t cc = 8 * nt + 2 * i4 + c;
+      hi[nt][c] = cc < rows.count ? row_hi(a, seq, rows.first + cc) : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int m2 = 0; m2 < 2; ++m2)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float f = r == 0 ? nq : nq * 0.0625f;  // the upper nibble's code is 16 times as large
+          const float x = v[j][2 * m2 + r] * f, y = v[j][4 + 2 * m2 + r] * f;
+          qf[nt][j][m2][r][0] = pack_half2(x, y);
+          if constexpr (QP == 2) {
+            const float2 h = unpack_half2(qf[nt][j][m2][r][0]);
+            qf[nt][j][m2][r][1] = pack_half2(x - h.x, y - h.y);
+          }
+        }
+  }
+
+  float o[NT][NG][2][4];  // out^T: channels 32 j + 4 g + 2 m2 (+ 1, 16 times as large), columns 2 i4, 2 i4 + 1
+  float zsum[NT][NG][2], l[NT][2], m[NT][2], trigger[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      l[nt][c] = 0.f;
+      m[nt][c] = 0.f;
+      trigger[nt][c] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        zsum[nt][j][c] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][j][c][e] = 0.f;
+      }
+    }
+  float pm = 0.f, pm_limit = -1.f;  // weights enter as w * s * pm; s <= pm_limit keeps that in float16
+
+  // Token of score row g (and, 8 further, of row g + 8): an order in which a
+  // quarter warp's key loads touch every bank once and the value loads twice.
+  const int32_t tok_g = (g & 1) ? 4 + static_cast<int32_t>((g >> 1) ^ 1u) : static_cast<int32_t>(g >> 1);
+  const int32_t tok_v[2] = {static_cast<int32_t>(i4), 4 + static_cast<int32_t>(i4 ^ 1u)};  // rows 2 i4, 2 i4 + 1
+
+  auto tile_step = [&](const uint8_t* st, int32_t key0, auto masked_tag) {
+    constexpr bool kMasked = decltype(masked_tag)::value;
+    const int32_t pos[2] = {key0 + tok_g, key0 + tok_g + 8};
+    bool keep[2] = {true, true};  // tokens that some row sees: what lies outside may be any bits
+    if constexpr (kMasked) {
+      keep[0] = pos[0] >= rows.lo_min && pos[0] <= rows.hi_max;
+      keep[1] = pos[1] >= rows.lo_min && pos[1] <= rows.hi_max;
+    }
+    // ---- scores
+    float raw[NT][4], zz[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw[nt][e] = zz[nt][e] = 0.f;
+    {
+      uint32_t w0[NG], w1[NG], p0[NG], p1[NG];
+      lds(w0, st + tok_g * G::kRowBytes + i4 * 4 * NG);
+      lds(w1, st + (tok_g + 8) * G::kRowBytes + i4 * 4 * NG);
+      lds(p0, st + G::kKeyParams + tok_g * 4 * NG);
+      lds(p1, st + G::kKeyParams + (tok_g + 8) * 4 * NG);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+        uint32_t x0 = __byte_perm(w0[j / 2], w0[j / 2 + NG / 2], sel);
+        uint32_t x1 = __byte_perm(w1[j / 2], w1[j / 2 + NG / 2], sel);
+        float acc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
+#pragma unroll
+        for (int m2 = 0; m2 < 2; ++m2) {
+          const uint32_t a0 = x0 & 0x000f000fu, a2 = x0 & 0x00f000f0u;
+          const uint32_t a1 = x1 & 0x000f000fu, a3 = x1 & 0x00f000f0u;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int qp = 0; qp < QP; ++qp)
+              mma_f16(acc[nt], a0, a1, a2, a3, qf[nt][j][m2][0][qp], qf[nt][j][m2][1][qp]);
+          x0 >>= 8;
+          x1 >>= 8;
+        }
+        const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);  // (s, z)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            raw[nt][c] = fmaf(f0.x, acc[nt][c], raw[nt][c]);
+            raw[nt][2 + c] = fmaf(f1.x, acc[nt][2 + c], raw[nt][2 + c]);
+            zz[nt][c] = fmaf(f0.y, qs[nt][j][c], zz[nt][c]);
+            zz[nt][2 + c] = fmaf(f1.y, qs[nt][j][c], zz[nt][2 + c]);
+          }
+      }
+    }
+    bool vis[NT][4];
+    bool renew = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float s = fmaf(raw[nt][2 * r + c], kf[nt][c], zz[nt][2 * r + c]);
+          vis[nt][2 * r + c] = true;
+          if constexpr (kMasked) {
+            vis[nt][2 * r + c] = pos[r] <= hi[nt][c] && pos[r] >= row_lo(a, hi[nt][c]);
+            if (!vis[nt][2 * r + c]) s = -INFINITY;
+          }
+          raw[nt][2 * r + c] = s;
+        }
+        renew |= fmaxf(raw[nt][c], raw[nt][2 + c]) > trigger[nt][c];
+      }
+    if (__any_sync(0xffffffffu, renew)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float top = fmaxf(raw[nt][c], raw[nt][2 + c]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          if (!(top > -INFINITY)) continue;  // this column still sees nothing, or nothing but NaN
+          const bool first = trigger[nt][c] == -INFINITY;
+          const float next = first ? top : fmaxf(m[nt][c], top);
+          const float alpha = first ? 0.f : exp2_approx(m[nt][c] - next);
+          m[nt][c] = next;
+          trigger[nt][c] = next + kSlack;
+          l[nt][c] *= alpha;
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            zsum[nt][j][c] *= alpha;
+#pragma unroll
+            for (int m2 = 0; m2 < 2; ++m2) {
+              o[nt][j][m2][c] *= alpha;
+              o[nt][j][m2][2 + c] *= alpha;
+            }
+          }
+        }
+    }
+    // ---- weights
+    float w[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        w[nt][c] = exp2_approx(raw[nt][c] - m[nt][c]);
+        w[nt][2 + c] = exp2_approx(raw[nt][2 + c] - m[nt][c]);
+        l[nt][c] += w[nt][c] + w[nt][2 + c];
+      }
+    // ---- values
+    uint32_t vw[4][NG / 2], p0[NG], p1[NG];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lds(vw[r], st + G::kValues + (tok_v[r & 1] + 8 * (r >> 1)) * G::kRowBytes + g * 2 * NG);
+    lds(p0, st + G::kValueParams + tok_g * 4 * NG);
+    lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
+    if constexpr (kMasked) {
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        if (!keep[0]) p0[j] = 0u;
+        if (!keep[1]) p1[j] = 0u;
+      }
+    }
+    float smax = 0.f;
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+      smax = fmaxf(smax, fmaxf(fabsf(unpack_half2(p0[j]).x), fabsf(unpack_half2(p1[j]).x)));
+    if (__any_sync(0xffffffffu, smax > pm_limit)) {
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
+      // a largest scale of zero sets no measure for those to come
+      const float next = pow2_toward(smax, 5);
+      const float ratio = pm_limit < 0.f ? 0.f : next / pm;
+      pm = next;
+      pm_limit = smax > 0.f ? 128.f / next : 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+          for (int m2 = 0; m2 < 2; ++m2)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nt][j][m2][e] *= ratio;
+    }
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+      uint32_t x01 = __byte_perm(vw[0][j / 2], vw[1][j / 2], sel);
+      uint32_t x23 = __byte_perm(vw[2][j / 2], vw[3][j / 2], sel);
+      const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
+      uint32_t bf[NT][2][PP];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float u[4], zw[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = e < 2 ? f0 : f1;
+          u[e] = w[nt][e] * (f.x * pm);
+          zw[e] = w[nt][e] * f.y;
+          if constexpr (kMasked) {
+            if (!vis[nt][e]) u[e] = zw[e] = 0.f;
+          }
+        }
+        zsum[nt][j][0] += zw[0] + zw[2];
+        zsum[nt][j][1] += zw[1] + zw[3];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t h = pack_half2(u[2 * r], u[2 * r + 1]);
+          bf[nt][r][0] = transpose8x8(h);
+          if constexpr (PP == 2) {
+            const float2 f = unpack_half2(h);
+            bf[nt][r][1] = transpose8x8(pack_half2(u[2 * r] - f.x, u[2 * r + 1] - f.y));
+          }
+        }
+      }
+#pragma unroll
+      for (int m2 = 0; m2 < 2; ++m2) {
+        const uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
+        const uint32_t a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int pp = 0; pp < PP; ++pp) mma_f16(o[nt][j][m2], a0, a1, a2, a3, bf[nt][0][pp], bf[nt][1][pp]);
+        x01 >>= 8;
+        x23 >>= 8;
+      }
+    }
+  };
+
+  auto arrived = [&](int32_t k) {
+    return __all_sync(0xffffffffu, mbar_wait(&bars[warp][k % G::kStages],
+                                             static_cast<uint32_t>(k / G::kStages) & 1u, a.err, kErrWaitFull));
+  };
+  for (int32_t k = 0; k < tiles; ++k) {
+    if (k + G::kStages - 1 < tiles) issue(k + G::kStages - 1);
+    const int st = k % G::kStages;
+    if (!arrived(k)) {  // gave up (reported in *err): the copies in flight still land in this ring
+      for (int32_t d = k + 1; d < min(tiles, k + G::kStages); ++d) arrived(d);
+      break;
+    }
+    if (loaded[warp][st]) {
+      const int32_t key0 = (t0 + static_cast<int32_t>(warp) + k * kWarps) * static_cast<int32_t>(kKv4Tile);
+      const uint8_t* p = ring + st * G::kBytes;
+      if (key0 >= rows.lo_max && key0 + static_cast<int32_t>(kKv4Tile) - 1 <= rows.hi_min)
+        tile_step(p, key0, std::false_type{});
+      else
+        tile_step(p, key0, std::true_type{});
+    }
+    __syncwarp();  // every lane has read the stage before it is filled again
+  }
+
+  // ---- this warp's result, then the block's
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) zsum[nt][j][c] += __shfl_xor_sync(0xffffffffu, zsum[nt][j][c], d);
+      }
+    }
+  float* mine = reinterpret_cast<float*>(ring);  // [8 NT][D]
+  const float low = pm_limit < 0.f ? 0.f : kCodeLow / pm, high = pm_limit < 0.f ? 0.f : kCodeHigh / pm;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int col = 8 * nt + 2 * static_cast<int>(i4) + c;
+      // a column that saw no key; one whose scores are all NaN has l = NaN and is none
+      const bool none = trigger[nt][c] == -INFINITY && l[nt][c] == 0.f;
+      if (g == 0) warp_ml[warp][col] = make_float2(none ? -INFINITY : m[nt][c], l[nt][c]);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        float2* to = reinterpret_cast<float2*>(mine + col * D + 32 * j + 4 * g);
+#pragma unroll
+        for (int m2 = 0; m2 < 2; ++m2)
+          to[m2] = make_float2(fmaf(o[nt][j][m2][c], low, zsum[nt][j][c]), fmaf(o[nt][j][m2][2 + c], high, zsum[nt][j][c]));
+      }
+    }
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(smem);
+  constexpr int kWarpFloats = G::kStages * G::kBytes / 4;
+  for (uint32_t e = threadIdx.x; e < rows.count * (D / 4); e += kThreads) {
+    const uint32_t col = e / (D / 4), c4 = e % (D / 4);
+    float top = -INFINITY;
+#pragma unroll
+    for (int wi = 0; wi < kWarps; ++wi) top = fmaxf(top, warp_ml[wi][col].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float total = 0.f;
+#pragma unroll
+    for (int wi = 0; wi < kWarps; ++wi) {
+      const float2 ml = warp_ml[wi][col];
+      if (ml.x == -INFINITY) continue;
+      const float f = exp2_approx(ml.x - base);
+      const float4 x = *reinterpret_cast<const float4*>(all + wi * kWarpFloats + col * D + 4 * c4);
+      total = fmaf(f, ml.y, total);
+      sum.x = fmaf(f, x.x, sum.x);
+      sum.y = fmaf(f, x.y, sum.y);
+      sum.z = fmaf(f, x.z, sum.z);
+      sum.w = fmaf(f, x.w, sum.w);
+    }
+    const uint32_t row = rows.first + col;
+    const uint64_t token = seq.row0 + row / a.share;
+    const uint32_t qh = head * a.share + row % a.share;
+    if (a.splits == 1) {
+      const float inv = top == -INFINITY ? 0.f : 1.0f / total;
+      store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c4,
+             make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+      if (c4 == 0 && a.lse != nullptr)
+        a.lse[token * a.heads + qh] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
+    } else {
+      const uint64_t at = (split * a.view.tokens + token) * a.heads + qh;
+      *reinterpret_cast<float4*>(a.part_o + at * D + 4 * c4) = sum;
+      if (c4 == 0) a.part_ml[at] = make_float2(top, total);
+    }
+  }
+}
+
+// Joins the splits of every row: four warps take the splits in turn.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) kv4_join_kernel(const KernelArgs a, uint32_t rows_per_tile) {
+  __shared__ float4 part[kWarps][D / 4];
+  __shared__ float part_l[kWarps];
+  griddep_wait();
+  Kv4Seq seq;
+  if (!kv4_seq(a.view, blockIdx.y, &seq)) return;
+  const uint32_t r = blockIdx.x;  // token * heads + head
+  if (r >= seq.n * a.heads) return;
+  const uint32_t t = r / a.heads, qh = r % a.heads;
+  // the splits that have keys: those of the row tile this row was computed in
+  const uint32_t row = t * a.share + qh % a.share;
+  Rows rows;
+  row_range(a, seq, row / rows_per_tile, rows_per_tile, &rows);
+  const uint32_t tiles = static_cast<uint32_t>(rows.t_end - rows.t_begin);
+  const uint32_t splits = max(1u, min(a.splits, (tiles + a.span - 1) / a.span));
+  const uint64_t token = seq.row0 + t, stride = a.view.tokens * a.heads, at = token * a.heads + qh;
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  float top = -INFINITY;
+  for (uint32_t s = lane; s < splits; s += 32) top = fmaxf(top, a.part_ml[s * stride + at].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const float base = top == -INFINITY ? 0.f : top;
+  constexpr int kVec = (D / 4 + 31) / 32;
+  float4 sum[kVec];
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (uint32_t s = warp; s < splits; s += kWarps) {
+    const float2 ml = a.part_ml[s * stride + at];
+    if (ml.x == -INFINITY) continue;
+    const float f = exp2_approx(ml.x - base);
+    total = fmaf(f, ml.y, total);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const uint32_t c = lane + 32 * i;
+      if (c >= D / 4) continue;
+      const float4 x = *reinterpret_cast<const float4*>(a.part_o + (s * stride + at) * D + 4 * c);
+      sum[i].x = fmaf(f, x.x, sum[i].x);
+      sum[i].y = fmaf(f, x.y, sum[i].y);
+      sum[i].z = fmaf(f, x.z, sum[i].z);
+      sum[i].w = fmaf(f, x.w, sum[i].w);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kVec; ++i)
+    if (lane + 32 * i < D / 4) part[warp][lane + 32 * i] = sum[i];
+  if (lane == 0) part_l[warp] = total;
+  __syncthreads();
+  total = part_l[0] + part_l[1] + part_l[2] + part_l[3];
+  for (uint32_t c = threadIdx.x; c < D / 4; c += kThreads) {
+    float4 v = part[0][c];
+#pragma unroll
+    for (int wi = 1; wi < kWarps; ++wi) {
+      const float4 x = part[wi][c];
+      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+    }
+    const float inv = top == -INFINITY ? 0.f : 1.0f / total;
+    store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c,
+           make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+  }
+  if (threadIdx.x == 0 && a.lse != nullptr)
+    a.lse[at] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
+}
+
+template <typename T, int D, int NT>
+cudaError_t launch(const KernelArgs& a, uint32_t kv_heads, cudaStream_t stream) {
+  using G = Geometry<D>;
+  constexpr int QP = sizeof(T) == 4 ? 2 : 1;
+  constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
+  constexpr size_t kSmem = static_cast<size_t>(kWarps) * G::kStages * G::kBytes;
+  static_assert(G::kStages * G::kBytes >= 8 * NT * D * 4, "the ring holds the warp's result at the end");
+  const auto kernel = kv4_attention_kernel<T, D, NT, QP, PP>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
+  if (e != cudaSuccess) return e;
+  const dim3 grid(a.splits, kv_heads * a.row_tiles, a.view.batch);
+  kernel<<<grid, kThreads, kSmem, stream>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || a.splits == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.view.max_tokens * a.heads, a.view.batch);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D>, a, static_cast<uint32_t>(8 * NT));
+}
+
+template <typename T, int D>
+cudaError_t dispatch(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream) {
+  switch (plan.row_tile) {
+    case 8: return launch<T, D, 1>(a, a.view.kv_heads, stream);
+    case 16:
+      if constexpr (kMaxRowGroups<D> >= 2) return launch<T, D, 2>(a, a.view.kv_heads, stream);
+      return cudaErrorInvalidValue;
+    case 32:
+      if constexpr (kMaxRowGroups<D> >= 4) return launch<T, D, 4>(a, a.view.kv_heads, stream);
+      return cudaErrorInvalidValue;
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+template <typename T>
+cudaError_t dispatch_dim(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream) {
+  switch (a.view.dim) {
+    case 64: return dispatch<T, 64>(a, plan, stream);
+    case 128: return dispatch<T, 128>(a, plan, stream);
+    case 256: return dispatch<T, 256>(a, plan, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+bool kv4_attention_supported(uint32_t dim) { return dim == 64 || dim == 128 || dim == 256; }
+
+Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint32_t batch, uint32_t max_tokens,
+                           uint32_t max_kv_len, uint64_t tokens, uint32_t window) {
+  Kv4Plan p;
+  const uint64_t rows = static_cast<uint64_t>(max_tokens) * (heads / kv_heads);
+  const uint32_t most = dim == 64 ? 32 : (dim == 128 ? 16 : 8);
+  p.row_tile = 8;
+  while (p.row_tile < most && p.row_tile < rows) p.row_tile *= 2;
+  p.row_tiles = static_cast<uint32_t>((rows + p.row_tile - 1) / p.row_tile);
+  uint64_t keys = max_kv_len;
+  // a row tile spans at most row_tile tokens; its window's first key may start mid-tile
+  if (window != 0 && keys > static_cast<uint64_t>(window) + p.row_tile) keys = static_cast<uint64_t>(window) + p.row_tile + 15;
+  const uint64_t tiles = (keys + kKv4Tile - 1) / kKv4Tile + (window != 0 ? 1 : 0);
+  const uint64_t items = static_cast<uint64_t>(batch) * kv_heads * p.row_tiles;
+  // Two blocks per SM and two waves of them; a block takes at least two tiles per warp.
+  const uint64_t want = 148ull * 4;
+  uint64_t splits = items >= want ? 1 : (want + items - 1) / (items == 0 ? 1 : items);
+  uint64_t span = splits == 0 ? tiles : (tiles + splits - 1) / splits;
+  span = (span + kWarps - 1) / kWarps * kWarps;
+  if (span < 2 * kWarps) span = 2 * kWarps;
+  p.span = static_cast<uint32_t>(span);
+  p.splits = static_cast<uint32_t>(tiles == 0 ? 1 : (tiles + span - 1) / span);
+  if (p.splits > 1) p.workspace = (p.splits * tokens * heads) * (static_cast<uint64_t>(dim) * 4 + 8);
+  return p;
+}
+
+cudaError_t kv4_attention(const Kv4AttnArgs& in, const Kv4Plan& plan, cudaStream_t stream) {
+  if (in.view.batch == 0 || in.view.tokens == 0 || in.view.max_tokens == 0) return cudaSuccess;
+  KernelArgs a{};
+  a.view = in.view;
+  a.q = in.q;
+  a.out = in.out;
+  a.q_token = in.q_token;
+  a.q_head = in.q_head;
+  a.out_token = in.out_token;
+  a.out_head = in.out_head;
+  a.lse = in.lse;
+  a.scale_log2 = in.scale * kLog2e;
+  a.heads = in.heads;
+  a.share = in.heads / in.view.kv_heads;
+  a.causal = in.causal ? 1 : 0;
+  a.window = in.window;
+  a.row_tiles = plan.row_tiles;
+  a.span = plan.span;
+  a.splits = plan.splits;
+  a.part_o = static_cast<float*>(in.workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<uint64_t>(plan.splits) * in.view.tokens * in.heads * in.view.dim);
+  a.err = in.err;
+  switch (in.type) {
+    case kF32: return dispatch_dim<float>(a, plan, stream);
+    case kBf16: return dispatch_dim<__nv_bfloat16>(a, plan, stream);
+    default: return dispatch_dim<__half>(a, plan, stream);
+  }
+}
+
+}  // namespace oct

@@ -113,7 +113,7 @@ struct Runtime {
   DevBuf scratch;               // split-TF32 operand buffers
   DevBuf da, db, dc;            // staging for host-pointer SGEMM
   DevBuf rin, rout, rw, rinv;   // staging for reductions / RMSNorm
-  DevBuf words;                 // [0] kernel error bits (u32), [8] first non-finite index (u64)
+  DevBuf words;                 // [0] kernel error bits (u32), [8] first non-finite index (u64), [16] cache index (u32)
   AsyncTask tasks[kAsyncSlots];
   int next_task_id = 1;
   AsyncStats async_stats;
@@ -158,6 +158,11 @@ struct Runtime {
   unsigned int* err_word() { return static_cast<unsigned int*>(words.aligned()); }
   unsigned long long* nonfinite_word() {
     return reinterpret_cast<unsigned long long*>(static_cast<char*>(words.aligned()) + 8);
+  }
+  // Set by the cache kernels when an index on the device is out of range.  A word of
+  // its own: the host entries read and clear the one above around their own kernels.
+  unsigned int* cache_index_word() {
+    return reinterpret_cast<unsigned int*>(static_cast<char*>(words.aligned()) + 16);
   }
 };
 

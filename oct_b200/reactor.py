@@ -591,6 +591,55 @@ class OctB200TpSgemmConfig(C.Structure):
     ]
 
 
+class OctB200QkNormRopeRequest(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_uint32), ("tokens", C.c_uint64), ("q_heads", C.c_uint32),
+        ("k_heads", C.c_uint32), ("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32), ("interleaved", C.c_uint32),
+        ("normalize", C.c_uint32), ("eps", C.c_float), ("axes", C.c_uint32), ("axis_pairs", C.c_uint32 * 4),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+        ("q_token_stride", C.c_uint64), ("q_head_stride", C.c_uint64), ("k_token_stride", C.c_uint64),
+        ("k_head_stride", C.c_uint64), ("q_out_token_stride", C.c_uint64), ("q_out_head_stride", C.c_uint64),
+        ("k_out_token_stride", C.c_uint64), ("k_out_head_stride", C.c_uint64), ("q_weight", C.c_void_p),
+        ("k_weight", C.c_void_p), ("positions", C.c_void_p), ("position_stride", C.c_uint64),
+        ("frequencies", C.c_void_p),
+    ]
+
+
+class OctB200Kv4Cache(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("page_size", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+        ("pages", C.c_uint32), ("reserved", C.c_uint32), ("data", C.c_void_p),
+    ]
+
+
+class OctB200Kv4Batch(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("batch", C.c_uint32), ("page_table", C.c_void_p),
+        ("page_table_stride", C.c_uint64), ("page_table_width", C.c_uint32), ("max_tokens", C.c_uint32),
+        ("max_kv_len", C.c_uint32), ("reserved", C.c_uint32), ("kv_lens", C.c_void_p), ("cu_tokens", C.c_void_p),
+    ]
+
+
+class OctB200Kv4Rows(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_uint32), ("tokens", C.c_uint64), ("k", C.c_void_p),
+        ("v", C.c_void_p), ("k_token_stride", C.c_uint64), ("k_head_stride", C.c_uint64),
+        ("v_token_stride", C.c_uint64), ("v_head_stride", C.c_uint64),
+    ]
+
+
+class OctB200Kv4AttentionRequest(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_uint32), ("q_heads", C.c_uint32), ("causal", C.c_uint32),
+        ("window", C.c_uint32), ("scale", C.c_float), ("tokens", C.c_uint64), ("q", C.c_void_p),
+        ("out", C.c_void_p), ("q_token_stride", C.c_uint64), ("q_head_stride", C.c_uint64),
+        ("out_token_stride", C.c_uint64), ("out_head_stride", C.c_uint64), ("lse", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+DETAIL_KV4_BAD_INDEX, DETAIL_KV4_WORKSPACE = -7030, -7031
 TP_COLLECTIVE_AUTO, TP_COLLECTIVE_PEER, TP_COLLECTIVE_NCCL = 0, 1, 2
 DETAIL_TP_INVALID, DETAIL_TP_ALLOC, DETAIL_TP_NCCL, DETAIL_TP_NOT_FOUND, DETAIL_TP_EXEC = (
     -7020, -7021, -7022, -7023, -7024)
@@ -697,6 +746,18 @@ SIGNATURES = {
     "oct_b200_rmsnorm_device": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, C.c_float, _vp, _i32p]),
     "oct_b200_attention_device": (
         C.c_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, C.c_float, _vp, _i32p]),
+    "oct_b200_qk_norm_rope_device": (C.c_int, [_vp, C.POINTER(OctB200QkNormRopeRequest), _vp, _i32p]),
+    "oct_b200_kv4_tile_bytes": (_u64, [_u32]),
+    "oct_b200_kv4_store_device": (
+        C.c_int, [_vp, C.POINTER(OctB200Kv4Cache), C.POINTER(OctB200Kv4Batch), C.POINTER(OctB200Kv4Rows), _vp, _i32p]),
+    "oct_b200_kv4_load_device": (
+        C.c_int, [_vp, C.POINTER(OctB200Kv4Cache), C.POINTER(OctB200Kv4Batch), C.POINTER(OctB200Kv4Rows), _vp, _i32p]),
+    "oct_b200_kv4_attention_workspace_bytes": (
+        C.c_int, [C.POINTER(OctB200Kv4Cache), C.POINTER(OctB200Kv4Batch), C.POINTER(OctB200Kv4AttentionRequest),
+                  C.POINTER(C.c_uint64), _i32p]),
+    "oct_b200_kv4_attention_device": (
+        C.c_int, [_vp, C.POINTER(OctB200Kv4Cache), C.POINTER(OctB200Kv4Batch), C.POINTER(OctB200Kv4AttentionRequest),
+                  _vp, _i32p]),
     "oct_b200_selftest_wait_timeout": (C.c_int, [_vp, _u64, _i32p]),
     "oct_b200_sync_status": (C.c_int, [_vp, _vp, _i32p]),
     "oct_b200_sgemm_device_noalloc": (
@@ -1166,6 +1227,101 @@ class Runtime:
         if rc != PROM_OK:
             raise RuntimeError(f"device attention rc={rc} detail={detail.value}")
 
+    # -- token-by-token serving (torch tensors on the handle's GPU)
+    def qk_norm_rope_device(self, q, k, q_out, k_out, positions, frequencies, *, axis_pairs=None,
+                            interleaved: bool = False, normalize: bool = True, q_weight=None, k_weight=None,
+                            eps: float = 1e-6, stream=None) -> None:
+        """RMSNorm of every head of q and k, then the rotation to its position, in one pass.
+
+        q, k, q_out, k_out: [tokens][heads][head_dim] of one type (fp32, bf16, fp16), any strides with
+        adjacent channels; an output may be its input; k and k_out may be None.  positions: int32
+        [tokens][axes] (or [tokens]); frequencies: fp64 [rotary_dim / 2], radians per position, whose
+        pairs go to the axes in order, axis_pairs[i] each (default: one axis).  Weights: fp32 [head_dim]
+        or None."""
+        pairs = frequencies.numel()
+        if positions.dim() == 1:
+            positions = positions.unsqueeze(1)
+        axis_pairs = (pairs,) if axis_pairs is None else tuple(axis_pairs)
+        if len(axis_pairs) > 4 or positions.dim() != 2 or positions.shape[1] != len(axis_pairs):
+            raise ValueError("positions must be [tokens][axes] with as many axes (1..4) as axis_pairs")
+        tokens, heads, dim = q.shape
+        dtype = _dtype_id(q)
+        r = OctB200QkNormRopeRequest(_SIZEOF_ROPE, dtype, tokens, heads, 0, dim, 2 * pairs, interleaved, normalize,
+                                     eps, len(axis_pairs), (C.c_uint32 * 4)(*axis_pairs))
+        r.q, r.q_token_stride, r.q_head_stride = _rows(q, "q", dtype, tokens, heads, dim)
+        r.q_out, r.q_out_token_stride, r.q_out_head_stride = _rows(q_out, "q_out", dtype, tokens, heads, dim)
+        if k is not None:
+            r.k_heads = kh = k.shape[1]
+            r.k, r.k_token_stride, r.k_head_stride = _rows(k, "k", dtype, tokens, kh, dim)
+            r.k_out, r.k_out_token_stride, r.k_out_head_stride = _rows(k_out, "k_out", dtype, tokens, kh, dim)
+        r.positions = _vector(positions, "positions", "torch.int32", tokens * len(axis_pairs))
+        if positions.stride(1) != 1 and len(axis_pairs) > 1:
+            raise ValueError("positions: the axes of a token must be adjacent")
+        r.position_stride = positions.stride(0)
+        r.frequencies = _vector(frequencies, "frequencies", "torch.float64", pairs, contiguous=True)
+        r.q_weight = _vector(q_weight, "q_weight", "torch.float32", dim, contiguous=True)
+        r.k_weight = _vector(k_weight, "k_weight", "torch.float32", dim, contiguous=True)
+        detail = C.c_int()
+        rc = self.lib.oct_b200_qk_norm_rope_device(self.handle, r, _stream_ptr(stream), detail)
+        if rc != PROM_OK:
+            raise RuntimeError(f"device qk norm rope rc={rc} detail={detail.value}")
+
+    def _kv4_rows(self, fn, cache: "Kv4Cache", batch: "Kv4Batch", k, v, stream) -> None:
+        tokens, dtype = k.shape[0], _dtype_id(k)
+        r = OctB200Kv4Rows(_SIZEOF_ROWS, dtype, tokens)
+        r.k, r.k_token_stride, r.k_head_stride = _rows(k, "k", dtype, tokens, cache.kv_heads, cache.head_dim)
+        r.v, r.v_token_stride, r.v_head_stride = _rows(v, "v", dtype, tokens, cache.kv_heads, cache.head_dim)
+        detail = C.c_int()
+        rc = fn(self.handle, cache.desc, batch.desc, r, _stream_ptr(stream), detail)
+        if rc != PROM_OK:
+            raise RuntimeError(f"device kv4 rows rc={rc} detail={detail.value}")
+
+    def kv4_store_device(self, cache: "Kv4Cache", batch: "Kv4Batch", k, v, stream=None) -> None:
+        """Quantises rows k, v [tokens][kv_heads][head_dim] (fp32, bf16, fp16) into the cache, as the last
+        tokens of the batch's sequences."""
+        self._kv4_rows(self.lib.oct_b200_kv4_store_device, cache, batch, k, v, stream)
+
+    def kv4_load_device(self, cache: "Kv4Cache", batch: "Kv4Batch", k, v, stream=None) -> None:
+        """Reads the rows that the same batch would store back into k, v."""
+        self._kv4_rows(self.lib.oct_b200_kv4_load_device, cache, batch, k, v, stream)
+
+    def _kv4_request(self, cache: "Kv4Cache", q, causal, window, scale) -> OctB200Kv4AttentionRequest:
+        tokens, heads, _ = q.shape
+        if scale is None:
+            scale = cache.default_scale
+        return OctB200Kv4AttentionRequest(_SIZEOF_ATTENTION, _dtype_id(q), heads, causal, window, scale, tokens)
+
+    def kv4_attention_workspace_bytes(self, cache: "Kv4Cache", batch: "Kv4Batch", q, *, causal: bool = True,
+                                      window: int = 0) -> int:
+        """Workspace of kv4_attention_device for these sizes (0: none).  Host arithmetic only."""
+        size, detail = C.c_uint64(), C.c_int()
+        rc = self.lib.oct_b200_kv4_attention_workspace_bytes(cache.desc, batch.desc,
+                                                             self._kv4_request(cache, q, causal, window, None), size,
+                                                             detail)
+        if rc != PROM_OK:
+            raise RuntimeError(f"kv4 attention workspace rc={rc} detail={detail.value}")
+        return size.value
+
+    def kv4_attention_device(self, cache: "Kv4Cache", batch: "Kv4Batch", q, out, *, scale: Optional[float] = None,
+                             causal: bool = True, window: int = 0, lse=None, workspace=None, stream=None) -> None:
+        """Attention of the batch's rows q [tokens][q_heads][head_dim] (fp32, bf16, fp16) over the cache.
+
+        out: as q; lse: fp32 [tokens][q_heads] or None; workspace: a uint8 tensor of
+        kv4_attention_workspace_bytes of the same sizes, one per call that may run at the same time.
+        scale defaults to 1 / sqrt(head_dim)."""
+        r = self._kv4_request(cache, q, causal, window, scale)
+        tokens, heads, dtype = r.tokens, r.q_heads, r.dtype
+        r.q, r.q_token_stride, r.q_head_stride = _rows(q, "q", dtype, tokens, heads, cache.head_dim)
+        r.out, r.out_token_stride, r.out_head_stride = _rows(out, "out", dtype, tokens, heads, cache.head_dim)
+        if lse is not None:
+            r.lse = _vector(lse, "lse", "torch.float32", tokens * heads, contiguous=True)
+        if workspace is not None:
+            r.workspace, r.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        detail = C.c_int()
+        rc = self.lib.oct_b200_kv4_attention_device(self.handle, cache.desc, batch.desc, r, _stream_ptr(stream), detail)
+        if rc != PROM_OK:
+            raise RuntimeError(f"device kv4 attention rc={rc} detail={detail.value}")
+
     def selftest_wait_timeout(self, budget_ns: int) -> CallStatus:
         """Test-only: a bounded in-kernel wait on a flag nothing sets must report a timeout."""
         detail = C.c_int()
@@ -1209,6 +1365,96 @@ def nccl_unique_id(lib) -> bytes:
     if lib.oct_b200_nccl_unique_id(C.cast(buf, C.c_void_p)) != PROM_OK:
         raise RuntimeError("ncclGetUniqueId failed (libnccl.so.2 not loadable?)")
     return bytes(buf)
+
+
+_DTYPES = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_F16}
+_DTYPE_IDS: dict = {}  # torch.dtype -> id, filled as types are met (torch is not imported here)
+_SIZEOF_ROPE, _SIZEOF_ROWS, _SIZEOF_ATTENTION = (
+    C.sizeof(OctB200QkNormRopeRequest), C.sizeof(OctB200Kv4Rows), C.sizeof(OctB200Kv4AttentionRequest))
+
+
+def _dtype_id(x) -> int:
+    got = _DTYPE_IDS.get(x.dtype)
+    if got is None:
+        got = _DTYPES.get(str(x.dtype))
+        if got is None:
+            raise TypeError(f"element type {x.dtype} is not one of float32, bfloat16, float16")
+        _DTYPE_IDS[x.dtype] = got
+    return got
+
+
+def _rows(x, name: str, dtype: int, tokens: int, heads: int, dim: int) -> tuple:
+    """(address, token stride, head stride) of a [tokens][heads][dim] tensor with adjacent channels."""
+    if x.shape != (tokens, heads, dim):
+        raise ValueError(f"{name} must be [{tokens}][{heads}][{dim}], got {tuple(x.shape)}")
+    if _dtype_id(x) != dtype or not x.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor of the call's element type")
+    token, head, channel = x.stride()
+    if channel != 1:
+        raise ValueError(f"{name}: the channels of a row must be adjacent")
+    return x.data_ptr(), token, head
+
+
+def _vector(x, name: str, dtype: str, count: int, contiguous: bool = False) -> int:
+    if x is None:
+        return 0
+    if str(x.dtype) != dtype or not x.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor of {dtype}")
+    if x.numel() != count or (contiguous and not x.is_contiguous()):
+        raise ValueError(f"{name} must hold {count} values" + (", contiguous" if contiguous else ""))
+    return x.data_ptr()
+
+
+def kv4_tile_bytes(head_dim: int) -> int:
+    """Bytes of the cache for 16 tokens of one key head; a cache has pages * kv_heads * (page_size / 16) of them."""
+    return 2 * 16 * (head_dim // 2 + head_dim // 32 * 4)
+
+
+class Kv4Cache:
+    """The 4-bit paged cache over caller-owned memory.
+
+    data: a contiguous uint8 CUDA tensor of whole pages, kv_heads * (page_size / 16) *
+    kv4_tile_bytes(head_dim) bytes each.  It needs no initialisation."""
+
+    def __init__(self, data, *, page_size: int, kv_heads: int, head_dim: int):
+        page = kv_heads * (page_size // 16) * kv4_tile_bytes(head_dim)
+        if str(data.dtype) != "torch.uint8" or not data.is_cuda or not data.is_contiguous():
+            raise TypeError("data must be a contiguous uint8 CUDA tensor")
+        if page_size <= 0 or page_size % 16 != 0 or page <= 0 or data.numel() % page != 0:
+            raise ValueError(f"data must hold whole pages of {page} bytes, of a page_size that is a multiple of 16")
+        self.data, self.page_size, self.kv_heads, self.head_dim = data, page_size, kv_heads, head_dim
+        self.pages = data.numel() // page
+        self.default_scale = float(np.float32(1.0) / np.sqrt(np.float32(head_dim)))
+        self.desc = OctB200Kv4Cache(C.sizeof(OctB200Kv4Cache), page_size, kv_heads, head_dim, self.pages, 0,
+                                    data.data_ptr())
+
+
+class Kv4Batch:
+    """The sequences of a cache call; keeps its tensors, whose contents may change between calls.
+
+    page_table: int32 [batch][pages per sequence]; kv_lens: int32 [batch], tokens held including those
+    of the call; cu_tokens: int32 [batch + 1] first rows, or None for one row per sequence; max_tokens
+    and max_kv_len bound a sequence's rows and length (default of the latter: what the table holds)."""
+
+    def __init__(self, page_table, kv_lens, cu_tokens=None, *, max_tokens: int = 1,
+                 max_kv_len: Optional[int] = None, page_size: Optional[int] = None):
+        batch = kv_lens.numel()
+        for name, x in (("page_table", page_table), ("kv_lens", kv_lens), ("cu_tokens", cu_tokens)):
+            if x is not None and (str(x.dtype) != "torch.int32" or not x.is_cuda):
+                raise TypeError(f"{name} must be an int32 CUDA tensor")
+        if page_table.dim() != 2 or page_table.shape[0] != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError("page_table must be [batch][pages], the pages of a sequence adjacent")
+        if not kv_lens.is_contiguous() or (cu_tokens is not None and (
+                cu_tokens.numel() != batch + 1 or not cu_tokens.is_contiguous())):
+            raise ValueError("kv_lens must hold batch and cu_tokens batch + 1 adjacent values")
+        if max_kv_len is None:
+            if page_size is None:
+                raise ValueError("give max_kv_len, or page_size for what the page table holds")
+            max_kv_len = page_table.shape[1] * page_size
+        self.page_table, self.kv_lens, self.cu_tokens = page_table, kv_lens, cu_tokens
+        self.desc = OctB200Kv4Batch(C.sizeof(OctB200Kv4Batch), batch, page_table.data_ptr(), page_table.stride(0),
+                                    page_table.shape[1], max_tokens, max_kv_len, 0, kv_lens.data_ptr(),
+                                    cu_tokens.data_ptr() if cu_tokens is not None else None)
 
 
 class Block:

@@ -63,6 +63,8 @@ struct Geometry {
 };
 
 // Query rows of one block in groups of 8, by what the accumulators leave of the registers.
+// Blocks per SM the compiler leaves registers for: latencies here are hidden by warps.
+template <int D, int NT> constexpr int kBlocksPerSm = D * NT <= 64 ? 5 : (D * NT <= 128 ? 4 : 2);
 template <int D> constexpr int kMaxRowGroups = D == 64 ? 4 : (D == 128 ? 2 : 1);
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -72,6 +74,15 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Value codes less 8, for fp32 results: code - 8 from the low nibble, 16 times that from
+// the high one.  The tensor cores truncate as they accumulate; unsigned codes let that grow with the
+// sum of the weights while the zeros cancel most of the sum itself (1.6e-5 of the result over 512 keys).
+constexpr uint32_t kMiddleLow = 0x64086408u, kMiddleHigh = 0x64806480u;  // 1024 + 8, 1024 + 128
+__device__ __forceinline__ uint32_t centred(uint32_t codes, uint32_t middle) {
+  const uint32_t x = codes | 0x64006400u;  // 1024 + code
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&middle));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -80,6 +91,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -159,9 +175,10 @@ __device__ __forceinline__ bool row_range(const KernelArgs& a, const Kv4Seq& s, 
 }
 
 template <typename T, int D, int NT, int QP, int PP>
-__global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const KernelArgs a) {
+__global__ void __launch_bounds__(kThreads, QP == 1 ? kBlocksPerSm<D, NT> : (D * NT <= 128 ? 3 : 2)) kv4_attention_kernel(const KernelArgs a) {
   using G = Geometry<D>;
   constexpr int NG = G::kGroups;
+  constexpr bool kCentred = std::is_same<T, float>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kWarps][G::kStages];
   __shared__ uint32_t loaded[kWarps][G::kStages];
@@ -186,29 +203,30 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const KernelArg
   }
   __syncwarp();
 
-  // Page numbers of this warp's next 32 tiles, one per lane.
+  // Where this warp's next 32 tiles lie, one per lane (null: no page of the cache).
   const int32_t* table = a.view.table + b * a.view.table_stride;
-  uint32_t pages = 0;
-  auto fetch_pages = [&](int32_t k0) {
+  const uint8_t* source = nullptr;
+  auto locate = [&](int32_t k0) {
     const int32_t k = k0 + static_cast<int32_t>(lane);
-    const int32_t t = t0 + static_cast<int32_t>(warp) + k * kWarps;
-    pages = k < tiles ? static_cast<uint32_t>(table[static_cast<uint32_t>(t) / a.view.page_tiles]) : 0u;
+    source = nullptr;
+    if (k >= tiles) return;
+    const uint32_t t = static_cast<uint32_t>(t0 + static_cast<int32_t>(warp) + k * kWarps);
+    const uint32_t in_table = t / a.view.page_tiles;
+    const uint32_t page = static_cast<uint32_t>(table[in_table]);
+    if (page < a.view.pages)
+      source = kv4_tile(a.view, page, head, t - in_table * a.view.page_tiles, G::kBytes);
+    else
+      atomicOr(a.view.bad, 1u);
   };
   auto issue = [&](int32_t k) {  // tile k of this warp into its stage (whole warp)
-    if (k % 32 == 0) fetch_pages(k);
-    const uint32_t page = __shfl_sync(0xffffffffu, pages, k % 32);
-    const int32_t t = t0 + static_cast<int32_t>(warp) + k * kWarps;
+    if (k % 32 == 0) locate(k);
     const int st = k % G::kStages;
-    if (lane == 0) {
-      const bool ok = page < a.view.pages;
-      loaded[warp][st] = ok;
-      if (ok) {
+    if (lane == static_cast<uint32_t>(k % 32)) {
+      loaded[warp][st] = source != nullptr;
+      if (source != nullptr) {
         mbar_arrive_expect_tx(&bars[warp][st], G::kBytes);
-        bulk_load(ring + st * G::kBytes,
-                  kv4_tile(a.view, page, head, static_cast<uint32_t>(t) % a.view.page_tiles, G::kBytes), G::kBytes,
-                  &bars[warp][st]);
+        bulk_load(ring + st * G::kBytes, source, G::kBytes, &bars[warp][st]);
       } else {
-        atomicOr(a.view.bad, 1u);
         mbar_arrive(&bars[warp][st]);
       }
     }
@@ -411,6 +429,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const KernelArg
         l[nt][c] += w[nt][c] + w[nt][2 + c];
       }
     // ---- values
+    float wp[NT][4];
     uint32_t vw[4][NG / 2], p0[NG], p1[NG];
 #pragma unroll
     for (int r = 0; r < 4; ++r) lds(vw[r], st + G::kValues + (tok_v[r & 1] + 8 * (r >> 1)) * G::kRowBytes + g * 2 * NG);
@@ -426,7 +445,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const KernelArg
     float smax = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j)
-      smax = fmaxf(smax, fmaxf(fabsf(unpack_half2(p0[j]).x), fabsf(unpack_half2(p1[j]).x)));
+      smax = max3(smax, unpack_half2(p0[j]).x, unpack_half2(p1[j]).x);
     if (__any_sync(0xffffffffu, smax > pm_limit)) {
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
@@ -445,11 +464,19 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const KernelArg
             for (int e = 0; e < 4; ++e) o[nt][j][m2][e] *= ratio;
     }
 #pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wp[nt][e] = w[nt][e] * pm;
+#pragma unroll
     for (int j = 0; j < NG; ++j) {
       const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
       uint32_t x01 = __byte_perm(vw[0][j / 2], vw[1][j / 2], sel);
       uint32_t x23 = __byte_perm(vw[2][j / 2], vw[3][j / 2], sel);
-      const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
+      float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
+      if constexpr (kCentred) {
+        f0.y = fmaf(8.f, f0.x, f0.y);
+        f1.y = fmaf(8.f, f1.x, f1.y);
+      }
       uint32_t bf[NT][2][PP];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -457,7 +484,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const KernelArg
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 f = e < 2 ? f0 : f1;
-          u[e] = w[nt][e] * (f.x * pm);
+          u[e] = wp[nt][e] * f.x;
           zw[e] = w[nt][e] * f.y;
           if constexpr (kMasked) {
             if (!vis[nt][e]) u[e] = zw[e] = 0.f;
@@ -477,8 +504,12 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const KernelArg
       }
 #pragma unroll
       for (int m2 = 0; m2 < 2; ++m2) {
-        const uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
-        const uint32_t a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
+        uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
+        uint32_t a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
+        if constexpr (kCentred) {
+          a0 = centred(a0, kMiddleLow), a1 = centred(a1, kMiddleHigh);
+          a2 = centred(a2, kMiddleLow), a3 = centred(a3, kMiddleHigh);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -524,7 +555,8 @@ __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const KernelArg
       }
     }
   float* mine = reinterpret_cast<float*>(ring);  // [8 NT][D]
-  const float low = pm_limit < 0.f ? 0.f : kCodeLow / pm, high = pm_limit < 0.f ? 0.f : kCodeHigh / pm;
+  const float unit = pm_limit < 0.f ? 0.f : 1.f / pm;
+  const float low = kCentred ? unit : unit * kCodeLow, high = kCentred ? unit * 0.0625f : unit * kCodeHigh;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

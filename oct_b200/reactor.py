@@ -1238,41 +1238,43 @@ class Runtime:
         [tokens][axes] (or [tokens]); frequencies: fp64 [rotary_dim / 2], radians per position, whose
         pairs go to the axes in order, axis_pairs[i] each (default: one axis).  Weights: fp32 [head_dim]
         or None."""
-        pairs = frequencies.numel()
-        if positions.dim() == 1:
-            positions = positions.unsqueeze(1)
-        axis_pairs = (pairs,) if axis_pairs is None else tuple(axis_pairs)
-        if len(axis_pairs) > 4 or positions.dim() != 2 or positions.shape[1] != len(axis_pairs):
-            raise ValueError("positions must be [tokens][axes] with as many axes (1..4) as axis_pairs")
-        tokens, heads, dim = q.shape
-        dtype = _dtype_id(q)
-        r = OctB200QkNormRopeRequest(_SIZEOF_ROPE, dtype, tokens, heads, 0, dim, 2 * pairs, interleaved, normalize,
-                                     eps, len(axis_pairs), (C.c_uint32 * 4)(*axis_pairs))
-        r.q, r.q_token_stride, r.q_head_stride = _rows(q, "q", dtype, tokens, heads, dim)
-        r.q_out, r.q_out_token_stride, r.q_out_head_stride = _rows(q_out, "q_out", dtype, tokens, heads, dim)
+        dtype, shape, pairs = _element_type(q), q.shape, frequencies.numel()
+        if axis_pairs is None:
+            axis_pairs = (pairs,)
+        axes = len(axis_pairs)
+        tokens, heads, dim = shape
+        if positions.dtype is not _TORCH_TYPES["i32"] or not positions.is_cuda:
+            raise TypeError("positions must be an int32 CUDA tensor")
+        if (not 1 <= axes <= 4 or positions.shape != ((tokens, axes) if positions.dim() == 2 else (tokens * axes,))
+                or (axes > 1 and (positions.dim() != 2 or positions.stride(1) != 1))):
+            raise ValueError("positions must be [tokens][axes], a token's axes adjacent, with as many axes (1..4) "
+                             "as axis_pairs")
+        k_heads, k_rows, ko_rows = 0, _NO_ROWS, _NO_ROWS
         if k is not None:
-            r.k_heads = kh = k.shape[1]
-            r.k, r.k_token_stride, r.k_head_stride = _rows(k, "k", dtype, tokens, kh, dim)
-            r.k_out, r.k_out_token_stride, r.k_out_head_stride = _rows(k_out, "k_out", dtype, tokens, kh, dim)
-        r.positions = _vector(positions, "positions", "torch.int32", tokens * len(axis_pairs))
-        if positions.stride(1) != 1 and len(axis_pairs) > 1:
-            raise ValueError("positions: the axes of a token must be adjacent")
-        r.position_stride = positions.stride(0)
-        r.frequencies = _vector(frequencies, "frequencies", "torch.float64", pairs, contiguous=True)
-        r.q_weight = _vector(q_weight, "q_weight", "torch.float32", dim, contiguous=True)
-        r.k_weight = _vector(k_weight, "k_weight", "torch.float32", dim, contiguous=True)
+            k_heads = k.shape[1]
+            k_shape = (tokens, k_heads, dim)
+            k_rows, ko_rows = _rows(k, "k", q.dtype, k_shape), _rows(k_out, "k_out", q.dtype, k_shape)
+        q_rows, qo_rows = _rows(q, "q", q.dtype, shape), _rows(q_out, "q_out", q.dtype, shape)
         detail = C.c_int()
-        rc = self.lib.oct_b200_qk_norm_rope_device(self.handle, r, _stream_ptr(stream), detail)
+        rc = self.lib.oct_b200_qk_norm_rope_device(self.handle, OctB200QkNormRopeRequest(
+            _SIZEOF_ROPE, dtype, tokens, heads, k_heads, dim, 2 * pairs, interleaved, normalize, eps, axes,
+            tuple(axis_pairs), q_rows[0], k_rows[0], qo_rows[0], ko_rows[0], q_rows[1], q_rows[2], k_rows[1], k_rows[2],
+            qo_rows[1], qo_rows[2], ko_rows[1], ko_rows[2], _vector(q_weight, "q_weight", "f32", dim),
+            _vector(k_weight, "k_weight", "f32", dim), positions.data_ptr(), positions.stride(0),
+            _vector(frequencies, "frequencies", "f64", pairs)), _stream_ptr(stream), detail)
         if rc != PROM_OK:
             raise RuntimeError(f"device qk norm rope rc={rc} detail={detail.value}")
 
     def _kv4_rows(self, fn, cache: "Kv4Cache", batch: "Kv4Batch", k, v, stream) -> None:
-        tokens, dtype = k.shape[0], _dtype_id(k)
-        r = OctB200Kv4Rows(_SIZEOF_ROWS, dtype, tokens)
-        r.k, r.k_token_stride, r.k_head_stride = _rows(k, "k", dtype, tokens, cache.kv_heads, cache.head_dim)
-        r.v, r.v_token_stride, r.v_head_stride = _rows(v, "v", dtype, tokens, cache.kv_heads, cache.head_dim)
+        tokens = k.shape[0]
+        shape = (tokens, cache.kv_heads, cache.head_dim)
+        dtype = _element_type(k)
+        k_ptr, k_token, k_head = _rows(k, "k", k.dtype, shape)
+        v_ptr, v_token, v_head = _rows(v, "v", k.dtype, shape)
         detail = C.c_int()
-        rc = fn(self.handle, cache.desc, batch.desc, r, _stream_ptr(stream), detail)
+        rc = fn(self.handle, cache.desc, batch.desc,
+                OctB200Kv4Rows(_SIZEOF_ROWS, dtype, tokens, k_ptr, v_ptr, k_token, k_head, v_token, v_head),
+                _stream_ptr(stream), detail)
         if rc != PROM_OK:
             raise RuntimeError(f"device kv4 rows rc={rc} detail={detail.value}")
 
@@ -1285,19 +1287,13 @@ class Runtime:
         """Reads the rows that the same batch would store back into k, v."""
         self._kv4_rows(self.lib.oct_b200_kv4_load_device, cache, batch, k, v, stream)
 
-    def _kv4_request(self, cache: "Kv4Cache", q, causal, window, scale) -> OctB200Kv4AttentionRequest:
-        tokens, heads, _ = q.shape
-        if scale is None:
-            scale = cache.default_scale
-        return OctB200Kv4AttentionRequest(_SIZEOF_ATTENTION, _dtype_id(q), heads, causal, window, scale, tokens)
-
     def kv4_attention_workspace_bytes(self, cache: "Kv4Cache", batch: "Kv4Batch", q, *, causal: bool = True,
                                       window: int = 0) -> int:
         """Workspace of kv4_attention_device for these sizes (0: none).  Host arithmetic only."""
         size, detail = C.c_uint64(), C.c_int()
-        rc = self.lib.oct_b200_kv4_attention_workspace_bytes(cache.desc, batch.desc,
-                                                             self._kv4_request(cache, q, causal, window, None), size,
-                                                             detail)
+        rc = self.lib.oct_b200_kv4_attention_workspace_bytes(
+            cache.desc, batch.desc, OctB200Kv4AttentionRequest(_SIZEOF_ATTENTION, _element_type(q), q.shape[1], causal,
+                                                               window, cache.default_scale, q.shape[0]), size, detail)
         if rc != PROM_OK:
             raise RuntimeError(f"kv4 attention workspace rc={rc} detail={detail.value}")
         return size.value
@@ -1309,16 +1305,21 @@ class Runtime:
         out: as q; lse: fp32 [tokens][q_heads] or None; workspace: a uint8 tensor of
         kv4_attention_workspace_bytes of the same sizes, one per call that may run at the same time.
         scale defaults to 1 / sqrt(head_dim)."""
-        r = self._kv4_request(cache, q, causal, window, scale)
-        tokens, heads, dtype = r.tokens, r.q_heads, r.dtype
-        r.q, r.q_token_stride, r.q_head_stride = _rows(q, "q", dtype, tokens, heads, cache.head_dim)
-        r.out, r.out_token_stride, r.out_head_stride = _rows(out, "out", dtype, tokens, heads, cache.head_dim)
-        if lse is not None:
-            r.lse = _vector(lse, "lse", "torch.float32", tokens * heads, contiguous=True)
+        tokens, heads, _ = q.shape
+        shape, dtype = (tokens, heads, cache.head_dim), _element_type(q)
+        q_ptr, q_token, q_head = _rows(q, "q", q.dtype, shape)
+        out_ptr, out_token, out_head = _rows(out, "out", q.dtype, shape)
+        ws_ptr = ws_bytes = 0
         if workspace is not None:
-            r.workspace, r.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+            ws_bytes = workspace.numel()
+            ws_ptr = _vector(workspace, "workspace", "u8", ws_bytes)
         detail = C.c_int()
-        rc = self.lib.oct_b200_kv4_attention_device(self.handle, cache.desc, batch.desc, r, _stream_ptr(stream), detail)
+        rc = self.lib.oct_b200_kv4_attention_device(
+            self.handle, cache.desc, batch.desc,
+            OctB200Kv4AttentionRequest(_SIZEOF_ATTENTION, dtype, heads, causal, window,
+                                       cache.default_scale if scale is None else scale, tokens, q_ptr, out_ptr, q_token,
+                                       q_head, out_token, out_head, _vector(lse, "lse", "f32", tokens * heads), ws_ptr,
+                                       ws_bytes), _stream_ptr(stream), detail)
         if rc != PROM_OK:
             raise RuntimeError(f"device kv4 attention rc={rc} detail={detail.value}")
 
@@ -1367,41 +1368,48 @@ def nccl_unique_id(lib) -> bytes:
     return bytes(buf)
 
 
-_DTYPES = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_F16}
-_DTYPE_IDS: dict = {}  # torch.dtype -> id, filled as types are met (torch is not imported here)
 _SIZEOF_ROPE, _SIZEOF_ROWS, _SIZEOF_ATTENTION = (
     C.sizeof(OctB200QkNormRopeRequest), C.sizeof(OctB200Kv4Rows), C.sizeof(OctB200Kv4AttentionRequest))
+_NO_ROWS = (0, 0, 0)
+_TORCH_TYPES: dict = {}  # the torch dtypes of the serving calls, once such a call has been made
 
 
-def _dtype_id(x) -> int:
-    got = _DTYPE_IDS.get(x.dtype)
+def _torch_types() -> dict:
+    """torch.dtype -> element type id; torch is not imported before a call takes its tensors."""
+    if not _TORCH_TYPES:
+        import torch
+        _TORCH_TYPES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16})
+        _TORCH_TYPES.update({"i32": torch.int32, "f64": torch.float64, "f32": torch.float32, "u8": torch.uint8})
+    return _TORCH_TYPES
+
+
+def _element_type(x) -> int:
+    got = _torch_types().get(x.dtype)
     if got is None:
-        got = _DTYPES.get(str(x.dtype))
-        if got is None:
-            raise TypeError(f"element type {x.dtype} is not one of float32, bfloat16, float16")
-        _DTYPE_IDS[x.dtype] = got
+        raise TypeError(f"element type {x.dtype} is not one of float32, bfloat16, float16")
     return got
 
 
-def _rows(x, name: str, dtype: int, tokens: int, heads: int, dim: int) -> tuple:
+def _rows(x, name: str, like, shape: tuple) -> tuple:
     """(address, token stride, head stride) of a [tokens][heads][dim] tensor with adjacent channels."""
-    if x.shape != (tokens, heads, dim):
-        raise ValueError(f"{name} must be [{tokens}][{heads}][{dim}], got {tuple(x.shape)}")
-    if _dtype_id(x) != dtype or not x.is_cuda:
+    if x.dtype is not like or not x.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor of the call's element type")
+    if x.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(x.shape)}")
     token, head, channel = x.stride()
     if channel != 1:
         raise ValueError(f"{name}: the channels of a row must be adjacent")
     return x.data_ptr(), token, head
 
 
-def _vector(x, name: str, dtype: str, count: int, contiguous: bool = False) -> int:
+def _vector(x, name: str, kind: str, count: int) -> int:
+    """Address of `count` adjacent values, or 0 for None."""
     if x is None:
         return 0
-    if str(x.dtype) != dtype or not x.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor of {dtype}")
-    if x.numel() != count or (contiguous and not x.is_contiguous()):
-        raise ValueError(f"{name} must hold {count} values" + (", contiguous" if contiguous else ""))
+    if x.dtype is not _TORCH_TYPES[kind] or not x.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor of {_TORCH_TYPES[kind]}")
+    if x.numel() != count or not x.is_contiguous():
+        raise ValueError(f"{name} must hold {count} adjacent values")
     return x.data_ptr()
 
 
@@ -1418,7 +1426,7 @@ class Kv4Cache:
 
     def __init__(self, data, *, page_size: int, kv_heads: int, head_dim: int):
         page = kv_heads * (page_size // 16) * kv4_tile_bytes(head_dim)
-        if str(data.dtype) != "torch.uint8" or not data.is_cuda or not data.is_contiguous():
+        if data.dtype is not _torch_types()["u8"] or not data.is_cuda or not data.is_contiguous():
             raise TypeError("data must be a contiguous uint8 CUDA tensor")
         if page_size <= 0 or page_size % 16 != 0 or page <= 0 or data.numel() % page != 0:
             raise ValueError(f"data must hold whole pages of {page} bytes, of a page_size that is a multiple of 16")
@@ -1440,7 +1448,7 @@ class Kv4Batch:
                  max_kv_len: Optional[int] = None, page_size: Optional[int] = None):
         batch = kv_lens.numel()
         for name, x in (("page_table", page_table), ("kv_lens", kv_lens), ("cu_tokens", cu_tokens)):
-            if x is not None and (str(x.dtype) != "torch.int32" or not x.is_cuda):
+            if x is not None and (x.dtype is not _torch_types()["i32"] or not x.is_cuda):
                 raise TypeError(f"{name} must be an int32 CUDA tensor")
         if page_table.dim() != 2 or page_table.shape[0] != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
             raise ValueError("page_table must be [batch][pages], the pages of a sequence adjacent")

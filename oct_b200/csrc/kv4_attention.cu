@@ -30,8 +30,9 @@
 // values side by side, one bulk copy) through a private ring in shared memory:
 // no barrier between warps until the end.
 //
-// Keys are split over blocks when the (sequence, key head) pairs do not fill
-// the GPU; the partial results are joined in a second kernel, in split order.
+// Blocks take equal runs of the call's tiles, whatever the sequences' lengths:
+// each adds up the lengths on the device and finds its own run.  An item that
+// a run's end cuts leaves partial results, which a second kernel joins in order.
 #include <type_traits>
 
 #include "kernels.h"
@@ -63,8 +64,11 @@ struct Geometry {
 };
 
 // Query rows of one block in groups of 8, by what the accumulators leave of the registers.
-// Blocks per SM the compiler leaves registers for: latencies here are hidden by warps.
-template <int D, int NT> constexpr int kBlocksPerSm = D * NT <= 64 ? 5 : (D * NT <= 128 ? 4 : 2);
+// Blocks per SM that the compiler leaves registers for, and that a launch fills: latencies here are
+// hidden by warps, accumulators and query fragments grow with the channels and the row groups.
+constexpr int blocks_per_sm(int dim, int row_groups, int query_parts) {
+  return row_groups == 1 && dim <= 128 ? (query_parts == 1 || dim == 64 ? 4 : 3) : (dim * row_groups <= 128 ? 3 : 2);
+}
 template <int D> constexpr int kMaxRowGroups = D == 64 ? 4 : (D == 128 ? 2 : 1);
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -138,9 +142,10 @@ struct KernelArgs {
   float scale_log2;
   uint32_t heads, share;  // query heads, query heads of one key head
   uint32_t causal, window;
-  uint32_t row_tiles, span, splits;
-  float* part_o;   // [splits][tokens * heads][D]
-  float2* part_ml; // [splits][tokens * heads]
+  uint32_t row_tiles;
+  float* part_o;    // [blocks][2][rows of a tile][D]
+  float2* part_ml;  // [blocks][2][rows of a tile]
+  uint4* part_of;   // [blocks]: what the block's unfinished last item is, for the join
   unsigned int* err;
 };
 
@@ -174,528 +179,702 @@ __device__ __forceinline__ bool row_range(const KernelArgs& a, const Kv4Seq& s, 
   return true;
 }
 
+// An item is one (sequence, row tile, key head); its units are runs of kWarps
+// tiles, at least one so that a row without keys is written too.  Items stand
+// in that order, and every block takes an equal run of all the call's units.
+__device__ __forceinline__ uint32_t item_units(const Rows& r) {
+  return static_cast<uint32_t>(max(1, (r.t_end - r.t_begin + kWarps - 1) / kWarps));
+}
+__device__ __forceinline__ bool item_rows(const KernelArgs& a, uint32_t pair, uint32_t rows_per_tile, Kv4Seq* s,
+                                          Rows* r) {
+  const uint32_t b = pair / a.row_tiles;
+  return kv4_seq(a.view, b, s) && row_range(a, *s, pair - b * a.row_tiles, rows_per_tile, r);
+}
+struct Share {
+  unsigned long long begin, end, per;  // this block's units; units of every block
+  uint32_t pair, head, offset;         // where its first unit lies
+};
+// Called by the whole block.
+__device__ __forceinline__ bool find_share(const KernelArgs& a, uint32_t rows_per_tile, Share* out) {
+  __shared__ unsigned long long warp_sums[kWarps];
+  __shared__ uint32_t found[3];
+  const uint32_t pairs = a.view.batch * a.row_tiles, chunk = (pairs + kThreads - 1) / kThreads;
+  const uint32_t p0 = min(pairs, threadIdx.x * chunk), p1 = min(pairs, p0 + chunk);
+  unsigned long long mine = 0;
+  Kv4Seq s;
+  Rows r;
+  for (uint32_t p = p0; p < p1; ++p)
+    if (item_rows(a, p, rows_per_tile, &s, &r)) mine += item_units(r);
+  mine *= a.view.kv_heads;
+  unsigned long long upto = mine;
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= static_cast<uint32_t>(d)) upto += v;
+  }
+  if (lane == 31) warp_sums[warp] = upto;
+  __syncthreads();
+  unsigned long long total = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kWarps; ++w) {
+    if (w < warp) upto += warp_sums[w];
+    total += warp_sums[w];
+  }
+  out->per = (total + gridDim.x - 1) / gridDim.x;
+  out->begin = blockIdx.x * out->per;
+  out->end = min(total, out->begin + out->per);
+  if (out->begin >= total) return false;
+  unsigned long long at = upto - mine;
+  if (out->begin >= at && out->begin < upto)
+    for (uint32_t p = p0; p < p1; ++p)
+      if (item_rows(a, p, rows_per_tile, &s, &r)) {
+        const uint32_t units = item_units(r);
+        const unsigned long long all = static_cast<unsigned long long>(units) * a.view.kv_heads;
+        if (out->begin < at + all) {
+          const uint32_t rest = static_cast<uint32_t>(out->begin - at);
+          found[0] = p;
+          found[1] = rest / units;
+          found[2] = rest % units;
+          break;
+        }
+        at += all;
+      }
+  __syncthreads();
+  out->pair = found[0];
+  out->head = found[1];
+  out->offset = found[2];
+  return true;
+}
+
+// float16 bits, zero for infinities and NaN
+__device__ __forceinline__ uint32_t finite_half(uint32_t bits) { return (bits & 0x7c00u) == 0x7c00u ? 0u : bits; }
+
 template <typename T, int D, int NT, int QP, int PP>
-__global__ void __launch_bounds__(kThreads, QP == 1 ? kBlocksPerSm<D, NT> : (D * NT <= 128 ? 3 : 2)) kv4_attention_kernel(const KernelArgs a) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attention_kernel(const KernelArgs a) {
   using G = Geometry<D>;
   constexpr int NG = G::kGroups;
+  constexpr int kRows = 8 * NT;
   constexpr bool kCentred = std::is_same<T, float>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kWarps][G::kStages];
   __shared__ uint32_t loaded[kWarps][G::kStages];
-  __shared__ float2 warp_ml[kWarps][8 * NT];
+  __shared__ float2 warp_ml[kWarps][kRows];
 
   griddep_launch_dependents();
-  const uint32_t split = blockIdx.x, head = blockIdx.y / a.row_tiles, b = blockIdx.z;
-  Kv4Seq seq;
-  if (!kv4_seq(a.view, b, &seq)) return;
-  Rows rows;
-  if (!row_range(a, seq, blockIdx.y % a.row_tiles, 8 * NT, &rows)) return;
-  const int32_t t0 = rows.t_begin + static_cast<int32_t>(split * a.span);
-  const int32_t t1 = min(rows.t_end, t0 + static_cast<int32_t>(a.span));
-  if (t0 >= t1 && split > 0) return;  // the join looks at no split behind the last key
+  Share share;
+  const bool any = find_share(a, kRows, &share);
+  if (threadIdx.x == 0 && a.part_of != nullptr) a.part_of[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+  if (!any) return;
 
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, i4 = lane % 4;
-  const int32_t tiles = t0 + static_cast<int32_t>(warp) < t1 ? (t1 - t0 - static_cast<int32_t>(warp) + kWarps - 1) / kWarps : 0;
   uint8_t* ring = smem + warp * (G::kStages * G::kBytes);
   if (lane == 0) {
     for (int st = 0; st < G::kStages; ++st) mbar_init(&bars[warp][st], 1);
     fence_mbar_init();
   }
   __syncwarp();
-
-  // Where this warp's next 32 tiles lie, one per lane (null: no page of the cache).
-  const int32_t* table = a.view.table + b * a.view.table_stride;
-  const uint8_t* source = nullptr;
-  auto locate = [&](int32_t k0) {
-    const int32_t k = k0 + static_cast<int32_t>(lane);
-    source = nullptr;
-    if (k >= tiles) return;
-    const uint32_t t = static_cast<uint32_t>(t0 + static_cast<int32_t>(warp) + k * kWarps);
-    const uint32_t in_table = t / a.view.page_tiles;
-    const uint32_t page = static_cast<uint32_t>(table[in_table]);
-    if (page < a.view.pages)
-      source = kv4_tile(a.view, page, head, t - in_table * a.view.page_tiles, G::kBytes);
-    else
-      atomicOr(a.view.bad, 1u);
-  };
-  auto issue = [&](int32_t k) {  // tile k of this warp into its stage (whole warp)
-    if (k % 32 == 0) locate(k);
-    const int st = k % G::kStages;
-    if (lane == static_cast<uint32_t>(k % 32)) {
-      loaded[warp][st] = source != nullptr;
-      if (source != nullptr) {
-        mbar_arrive_expect_tx(&bars[warp][st], G::kBytes);
-        bulk_load(ring + st * G::kBytes, source, G::kBytes, &bars[warp][st]);
-      } else {
-        mbar_arrive(&bars[warp][st]);
-      }
-    }
-  };
-  for (int32_t k = 0; k < min(tiles, G::kStages - 1); ++k) issue(k);
-
-  // Query fragments: column g of group nt is row rows.first + 8 nt + g.
-  uint32_t qf[NT][NG][2][2][QP];
-  float kf[NT][2], qs[NT][NG][2];  // for this lane's score columns 2 i4, 2 i4 + 1
-  int32_t hi[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const uint32_t col = 8 * nt + g;
-    float v[NG][8];
-    float amax = 0.f;
-    if (col < rows.count) {
-      const uint32_t row = rows.first + col;
-      const T* p = static_cast<const T*>(a.q) + (seq.row0 + row / a.share) * a.q_token +
-                   (head * a.share + row % a.share) * a.q_head + 8 * i4;
-#pragma unroll
-      for (int j = 0; j < NG; ++j) load8(p + 32 * j, v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < NG; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-    }
-    float sums[NG];
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        s += v[j][e];
-        amax = fmaxf(amax, fabsf(v[j][e]));
-      }
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      sums[j] = s * a.scale_log2;
-    }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const float nq = pow2_toward(amax, 10);
-    const float factor = kCodeLow / nq * a.scale_log2;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int from = (2 * i4 + c) * 4;
-      kf[nt][c] = __shfl_sync(0xffffffffu, factor, from);
-#pragma unroll
-      for (int j = 0; j < NG; ++j) qs[nt][j][c] = __shfl_sync(0xffffffffu, sums[j], from);
-      const uint32_t cc = 8 * nt + 2 * i4 + c;
-      hi[nt][c] = cc < rows.count ? row_hi(a, seq, rows.first + cc) : -1;
-    }
-#pragma unroll
-    for (int j = 0; j < NG; ++j)
-#pragma unroll
-      for (int m2 = 0; m2 < 2; ++m2)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float f = r == 0 ? nq : nq * 0.0625f;  // the upper nibble's code is 16 times as large
-          const float x = v[j][2 * m2 + r] * f, y = v[j][4 + 2 * m2 + r] * f;
-          qf[nt][j][m2][r][0] = pack_half2(x, y);
-          if constexpr (QP == 2) {
-            const float2 h = unpack_half2(qf[nt][j][m2][r][0]);
-            qf[nt][j][m2][r][1] = pack_half2(x - h.x, y - h.y);
-          }
-        }
-  }
-
-  float o[NT][NG][2][4];  // out^T: channels 32 j + 4 g + 2 m2 (+ 1, 16 times as large), columns 2 i4, 2 i4 + 1
-  float zsum[NT][NG][2], l[NT][2], m[NT][2], trigger[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      l[nt][c] = 0.f;
-      m[nt][c] = 0.f;
-      trigger[nt][c] = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        zsum[nt][j][c] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[nt][j][c][e] = 0.f;
-      }
-    }
-  float pm = 0.f, pm_limit = -1.f;  // weights enter as w * s * pm; s <= pm_limit keeps that in float16
+  uint32_t used = 0;   // tiles this warp has had in its ring before the current item
+  bool failed = false;  // a wait gave up (reported in *err)
 
   // Token of score row g (and, 8 further, of row g + 8): an order in which a
   // quarter warp's key loads touch every bank once and the value loads twice.
   const int32_t tok_g = (g & 1) ? 4 + static_cast<int32_t>((g >> 1) ^ 1u) : static_cast<int32_t>(g >> 1);
   const int32_t tok_v[2] = {static_cast<int32_t>(i4), 4 + static_cast<int32_t>(i4 ^ 1u)};  // rows 2 i4, 2 i4 + 1
 
-  auto tile_step = [&](const uint8_t* st, int32_t key0, auto masked_tag) {
-    constexpr bool kMasked = decltype(masked_tag)::value;
-    const int32_t pos[2] = {key0 + tok_g, key0 + tok_g + 8};
-    bool keep[2] = {true, true};  // tokens that some row sees: what lies outside may be any bits
-    if constexpr (kMasked) {
-      keep[0] = pos[0] >= rows.lo_min && pos[0] <= rows.hi_max;
-      keep[1] = pos[1] >= rows.lo_min && pos[1] <= rows.hi_max;
+  unsigned long long unit = share.begin;
+  uint32_t pair = share.pair, head = share.head, offset = share.offset;
+  while (unit < share.end) {
+    Kv4Seq seq;
+    Rows rows;
+    if (pair >= a.view.batch * a.row_tiles) break;  // lengths that changed under the call
+    if (!item_rows(a, pair, kRows, &seq, &rows)) {  // a sequence or row tile without rows has no units
+      ++pair;
+      continue;
     }
-    // ---- scores
-    float raw[NT][4], zz[NT][4];
+    const uint32_t units = item_units(rows);
+    const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(units - offset), share.end - unit));
+    const int32_t t0 = rows.t_begin + static_cast<int32_t>(offset * kWarps);
+    const int32_t t1 = min(rows.t_end, t0 + static_cast<int32_t>(take * kWarps));
+    const int32_t first_tile = t0 + static_cast<int32_t>(warp);
+    const int32_t tiles = !failed && first_tile < t1 ? (t1 - first_tile + kWarps - 1) / kWarps : 0;
+
+    // Where this warp's next 32 tiles lie, one per lane (null: no page of the cache).
+    const int32_t* table = a.view.table + pair / a.row_tiles * a.view.table_stride;
+    const uint8_t* source = nullptr;
+    auto locate = [&](int32_t k0) {
+      const int32_t k = k0 + static_cast<int32_t>(lane);
+      source = nullptr;
+      if (k >= tiles) return;
+      const uint32_t t = static_cast<uint32_t>(first_tile + k * kWarps);
+      const uint32_t in_table = t / a.view.page_tiles;
+      const uint32_t page = static_cast<uint32_t>(table[in_table]);
+      if (page < a.view.pages)
+        source = kv4_tile(a.view, page, head, t - in_table * a.view.page_tiles, G::kBytes);
+      else
+        atomicOr(a.view.bad, 1u);
+    };
+    auto issue = [&](int32_t k) {  // tile k of this warp into its stage (whole warp)
+      if (k % 32 == 0) locate(k);
+      const uint32_t st = (used + k) % G::kStages;
+      if (lane == static_cast<uint32_t>(k % 32)) {
+        loaded[warp][st] = source != nullptr;
+        if (source != nullptr) {
+          mbar_arrive_expect_tx(&bars[warp][st], G::kBytes);
+          bulk_load(ring + st * G::kBytes, source, G::kBytes, &bars[warp][st]);
+        } else {
+          mbar_arrive(&bars[warp][st]);
+        }
+      }
+    };
+    for (int32_t k = 0; k < min(tiles, G::kStages - 1); ++k) issue(k);
+
+    // Query fragments: column g of group nt is row rows.first + 8 nt + g.
+    uint32_t qf[NT][NG][2][2][QP];
+    uint32_t qz[NT][2];   // the sums of q over the groups, in two parts: the zeros' operand
+    float kf[NT][2], zf[NT][2];  // factors of this lane's score columns 2 i4, 2 i4 + 1
+    int32_t hi[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint32_t col = 8 * nt + g;
+      float v[NG][8];
+      float amax = 0.f;
+      if (col < rows.count) {
+        const uint32_t row = rows.first + col;
+        const T* p = static_cast<const T*>(a.q) + (seq.row0 + row / a.share) * a.q_token +
+                     (head * a.share + row % a.share) * a.q_head + 8 * i4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) raw[nt][e] = zz[nt][e] = 0.f;
-    {
-      uint32_t w0[NG], w1[NG], p0[NG], p1[NG];
-      lds(w0, st + tok_g * G::kRowBytes + i4 * 4 * NG);
-      lds(w1, st + (tok_g + 8) * G::kRowBytes + i4 * 4 * NG);
-      lds(p0, st + G::kKeyParams + tok_g * 4 * NG);
-      lds(p1, st + G::kKeyParams + (tok_g + 8) * 4 * NG);
+        for (int j = 0; j < NG; ++j) load8(p + 32 * j, v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+      }
+      float sums[NG];
+      float smax = 0.f;
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-        uint32_t x0 = __byte_perm(w0[j / 2], w0[j / 2 + NG / 2], sel);
-        uint32_t x1 = __byte_perm(w1[j / 2], w1[j / 2 + NG / 2], sel);
-        float acc[NT][4];
+        float s = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 8; ++e) {
+          s += v[j][e];
+          amax = fmaxf(amax, fabsf(v[j][e]));
+        }
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        sums[j] = s;
+        smax = fmaxf(smax, fabsf(s));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const float nq = pow2_toward(amax, 10), nz = pow2_toward(smax, 10);
+      // zeros: slot k of 16 is group k % NG; the first NG slots hold the high part, the next the low one
+      uint32_t zh = 0, zl = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
+      for (int j = 0; j < NG; j += 2) {
+        const float x = sums[j] * nz, y = sums[j + 1] * nz;
+        const uint32_t h = pack_half2(x, y);
+        const float2 f = unpack_half2(h);
+        const uint32_t lo = pack_half2(x - f.x, y - f.y);
+        if (static_cast<int>(i4) % (NG / 2) == j / 2) zh = h, zl = lo;
+      }
+      if constexpr (NG == 8) {
+        qz[nt][0] = zh, qz[nt][1] = zl;  // slots 0..7 and 8..15
+      } else {
+        qz[nt][0] = static_cast<int>(i4) < NG / 2 ? zh : (static_cast<int>(i4) < NG ? zl : 0u);
+        qz[nt][1] = 0u;
+      }
+      const float kfac = kCodeLow / nq * a.scale_log2, zfac = a.scale_log2 / nz;
 #pragma unroll
-        for (int m2 = 0; m2 < 2; ++m2) {
-          const uint32_t a0 = x0 & 0x000f000fu, a2 = x0 & 0x00f000f0u;
-          const uint32_t a1 = x1 & 0x000f000fu, a3 = x1 & 0x00f000f0u;
+      for (int c = 0; c < 2; ++c) {
+        const int from = (2 * i4 + c) * 4;
+        kf[nt][c] = __shfl_sync(0xffffffffu, kfac, from);
+        zf[nt][c] = __shfl_sync(0xffffffffu, zfac, from);
+        const uint32_t cc = 8 * nt + 2 * i4 + c;
+        hi[nt][c] = cc < rows.count ? row_hi(a, seq, rows.first + cc) : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int m2 = 0; m2 < 2; ++m2)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float f = r == 0 ? nq : nq * 0.0625f;  // the upper nibble's code is 16 times as large
+            const float x = v[j][2 * m2 + r] * f, y = v[j][4 + 2 * m2 + r] * f;
+            qf[nt][j][m2][r][0] = pack_half2(x, y);
+            if constexpr (QP == 2) {
+              const float2 h = unpack_half2(qf[nt][j][m2][r][0]);
+              qf[nt][j][m2][r][1] = pack_half2(x - h.x, y - h.y);
+            }
+          }
+    }
+
+    float o[NT][NG][2][4];  // out^T: channels 32 j + 4 g + 2 m2 (+ 1, 16 times as large), columns 2 i4, 2 i4 + 1
+    float oz[NT][4];        // the zeros' share, by group: row g is group g (16-bit results)
+    float zsum[NT][NG][2];  // the same of the zeros + 8 s, of this lane's tokens (fp32 results)
+    float l[NT][2], m[NT][2], trigger[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        l[nt][c] = 0.f;
+        m[nt][c] = 0.f;
+        trigger[nt][c] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          zsum[nt][j][c] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][j][c][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) oz[nt][e] = 0.f;
+    }
+    float pm = 0.f, pm_limit = -1.f;  // weights enter as w * s * pm; s <= pm_limit keeps that in float16
+
+    auto tile_step = [&](const uint8_t* st, int32_t key0, auto masked_tag) {
+      constexpr bool kMasked = decltype(masked_tag)::value;
+      const int32_t pos[2] = {key0 + tok_g, key0 + tok_g + 8};
+      bool keep[2] = {true, true};  // tokens that some row sees: what lies outside may be any bits
+      if constexpr (kMasked) {
+        keep[0] = pos[0] >= rows.lo_min && pos[0] <= rows.hi_max;
+        keep[1] = pos[1] >= rows.lo_min && pos[1] <= rows.hi_max;
+      }
+      // ---- scores
+      float raw[NT][4], zz[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[nt][e] = zz[nt][e] = 0.f;
+      {
+        uint32_t w0[NG], w1[NG], p0[NG], p1[NG];
+        lds(w0, st + tok_g * G::kRowBytes + i4 * 4 * NG);
+        lds(w1, st + (tok_g + 8) * G::kRowBytes + i4 * 4 * NG);
+        lds(p0, st + G::kKeyParams + tok_g * 4 * NG);
+        lds(p1, st + G::kKeyParams + (tok_g + 8) * 4 * NG);
+        {
+          uint32_t z0[2], z1[2];  // (s, z) of groups 2 i4 and 2 i4 + 1, modulo the groups
+          lds(z0, st + G::kKeyParams + tok_g * 4 * NG + 8 * (i4 % (NG / 2)));
+          lds(z1, st + G::kKeyParams + (tok_g + 8) * 4 * NG + 8 * (i4 % (NG / 2)));
+          const uint32_t a0 = __byte_perm(z0[0], z0[1], 0x7632u), a1 = __byte_perm(z1[0], z1[1], 0x7632u);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(zz[nt], a0, a1, a0, a1, qz[nt][0], qz[nt][1]);
+        }
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+          uint32_t x0 = __byte_perm(w0[j / 2], w0[j / 2 + NG / 2], sel);
+          uint32_t x1 = __byte_perm(w1[j / 2], w1[j / 2 + NG / 2], sel);
+          float acc[NT][4];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int qp = 0; qp < QP; ++qp)
-              mma_f16(acc[nt], a0, a1, a2, a3, qf[nt][j][m2][0][qp], qf[nt][j][m2][1][qp]);
-          x0 >>= 8;
-          x1 >>= 8;
-        }
-        const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);  // (s, z)
+            for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int m2 = 0; m2 < 2; ++m2) {
+            const uint32_t a0 = x0 & 0x000f000fu, a2 = x0 & 0x00f000f0u;
+            const uint32_t a1 = x1 & 0x000f000fu, a3 = x1 & 0x00f000f0u;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            raw[nt][c] = fmaf(f0.x, acc[nt][c], raw[nt][c]);
-            raw[nt][2 + c] = fmaf(f1.x, acc[nt][2 + c], raw[nt][2 + c]);
-            zz[nt][c] = fmaf(f0.y, qs[nt][j][c], zz[nt][c]);
-            zz[nt][2 + c] = fmaf(f1.y, qs[nt][j][c], zz[nt][2 + c]);
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int qp = 0; qp < QP; ++qp)
+                mma_f16(acc[nt], a0, a1, a2, a3, qf[nt][j][m2][0][qp], qf[nt][j][m2][1][qp]);
+            x0 >>= 8;
+            x1 >>= 8;
           }
-      }
-    }
-    bool vis[NT][4];
-    bool renew = false;
+          const float s0 = unpack_half2(p0[j]).x, s1 = unpack_half2(p1[j]).x;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float s = fmaf(raw[nt][2 * r + c], kf[nt][c], zz[nt][2 * r + c]);
-          vis[nt][2 * r + c] = true;
-          if constexpr (kMasked) {
-            vis[nt][2 * r + c] = pos[r] <= hi[nt][c] && pos[r] >= row_lo(a, hi[nt][c]);
-            if (!vis[nt][2 * r + c]) s = -INFINITY;
-          }
-          raw[nt][2 * r + c] = s;
+            for (int c = 0; c < 2; ++c) {
+              raw[nt][c] = fmaf(s0, acc[nt][c], raw[nt][c]);
+              raw[nt][2 + c] = fmaf(s1, acc[nt][2 + c], raw[nt][2 + c]);
+            }
         }
-        renew |= fmaxf(raw[nt][c], raw[nt][2 + c]) > trigger[nt][c];
       }
-    if (__any_sync(0xffffffffu, renew)) {
+      bool vis[NT][4];
+      bool renew = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float top = fmaxf(raw[nt][c], raw[nt][2 + c]);
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          if (!(top > -INFINITY)) continue;  // this column still sees nothing, or nothing but NaN
-          const bool first = trigger[nt][c] == -INFINITY;
-          const float next = first ? top : fmaxf(m[nt][c], top);
-          const float alpha = first ? 0.f : exp2_approx(m[nt][c] - next);
-          m[nt][c] = next;
-          trigger[nt][c] = next + kSlack;
-          l[nt][c] *= alpha;
 #pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            zsum[nt][j][c] *= alpha;
+          for (int r = 0; r < 2; ++r) {
+            float s = fmaf(raw[nt][2 * r + c], kf[nt][c], zz[nt][2 * r + c] * zf[nt][c]);
+            vis[nt][2 * r + c] = true;
+            if constexpr (kMasked) {
+              vis[nt][2 * r + c] = pos[r] <= hi[nt][c] && pos[r] >= row_lo(a, hi[nt][c]);
+              if (!vis[nt][2 * r + c]) s = -INFINITY;
+            }
+            raw[nt][2 * r + c] = s;
+          }
+          renew |= fmaxf(raw[nt][c], raw[nt][2 + c]) > trigger[nt][c];
+        }
+      if (__any_sync(0xffffffffu, renew)) {
 #pragma unroll
-            for (int m2 = 0; m2 < 2; ++m2) {
-              o[nt][j][m2][c] *= alpha;
-              o[nt][j][m2][2 + c] *= alpha;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float top = fmaxf(raw[nt][c], raw[nt][2 + c]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            if (!(top > -INFINITY)) continue;  // this column still sees nothing, or nothing but NaN
+            const bool first = trigger[nt][c] == -INFINITY;
+            const float next = first ? top : fmaxf(m[nt][c], top);
+            const float alpha = first ? 0.f : exp2_approx(m[nt][c] - next);
+            m[nt][c] = next;
+            trigger[nt][c] = next + kSlack;
+            l[nt][c] *= alpha;
+            oz[nt][c] *= alpha;
+            oz[nt][2 + c] *= alpha;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+              zsum[nt][j][c] *= alpha;
+#pragma unroll
+              for (int m2 = 0; m2 < 2; ++m2) {
+                o[nt][j][m2][c] *= alpha;
+                o[nt][j][m2][2 + c] *= alpha;
+              }
+            }
+          }
+      }
+      // ---- weights
+      float w[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          w[nt][c] = exp2_approx(raw[nt][c] - m[nt][c]);
+          w[nt][2 + c] = exp2_approx(raw[nt][2 + c] - m[nt][c]);
+          l[nt][c] += w[nt][c] + w[nt][2 + c];
+        }
+      // ---- values
+      uint32_t vw[4][NG / 2], p0[NG], p1[NG];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) lds(vw[r], st + G::kValues + (tok_v[r & 1] + 8 * (r >> 1)) * G::kRowBytes + g * 2 * NG);
+      lds(p0, st + G::kValueParams + tok_g * 4 * NG);
+      lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
+      if constexpr (kMasked) {
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          if (!keep[0]) p0[j] = 0u;
+          if (!keep[1]) p1[j] = 0u;
+        }
+      }
+      // The zeros: rows of the operand are groups, its columns the tile's tokens.  fp32 results sum them
+      // beside the weights below instead, rounded to nearest.
+      if constexpr (!kCentred) {
+        uint32_t z[4] = {0u, 0u, 0u, 0u};
+        if (static_cast<int>(g) < NG) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int32_t token = tok_v[r & 1] + 8 * (r >> 1);
+            z[r] = *reinterpret_cast<const uint16_t*>(st + G::kValueParams + token * 4 * NG + 4 * g + 2);
+            if constexpr (kMasked) {
+              // a zero that is no number is seen through its codes' weights, by the rows that see it
+              z[r] = key0 + token >= rows.lo_min && key0 + token <= rows.hi_max ? finite_half(z[r]) : 0u;
             }
           }
         }
+        const uint32_t a0 = z[0] | (z[1] << 16), a2 = z[2] | (z[3] << 16);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint32_t h0 = pack_half2(w[nt][0], w[nt][1]), h1 = pack_half2(w[nt][2], w[nt][3]);
+          mma_f16(oz[nt], a0, 0u, a2, 0u, transpose8x8(h0), transpose8x8(h1));
+          if constexpr (PP == 2) {
+            const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
+            mma_f16(oz[nt], a0, 0u, a2, 0u, transpose8x8(pack_half2(w[nt][0] - f0.x, w[nt][1] - f0.y)),
+                    transpose8x8(pack_half2(w[nt][2] - f1.x, w[nt][3] - f1.y)));
+          }
+        }
+      }
+      if constexpr (kCentred) {
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
+          const float z0 = fmaf(8.f, f0.x, f0.y), z1 = fmaf(8.f, f1.x, f1.y);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              zsum[nt][j][c] = vis[nt][c] ? fmaf(w[nt][c], z0, zsum[nt][j][c]) : zsum[nt][j][c];
+              zsum[nt][j][c] = vis[nt][2 + c] ? fmaf(w[nt][2 + c], z1, zsum[nt][j][c]) : zsum[nt][j][c];
+            }
+        }
+      }
+      float smax = 0.f;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) smax = max3(smax, unpack_half2(p0[j]).x, unpack_half2(p1[j]).x);
+      if (__any_sync(0xffffffffu, smax > pm_limit)) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
+        // a largest scale of zero sets no measure for those to come
+        const float next = pow2_toward(smax, 5);
+        const float ratio = pm_limit < 0.f ? 0.f : next / pm;
+        pm = next;
+        pm_limit = smax > 0.f ? 128.f / next : 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int m2 = 0; m2 < 2; ++m2)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][j][m2][e] *= ratio;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[nt][e] *= pm;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+        uint32_t x01 = __byte_perm(vw[0][j / 2], vw[1][j / 2], sel);
+        uint32_t x23 = __byte_perm(vw[2][j / 2], vw[3][j / 2], sel);
+        const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
+        uint32_t bf[NT][2][PP];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = e < 2 ? f0 : f1;
+            u[e] = w[nt][e] * f.x;
+            if constexpr (kMasked) {
+              if (!vis[nt][e]) u[e] = 0.f;
+              else if (!kCentred && !(fabsf(f.y) < INFINITY)) u[e] = NAN;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t h = pack_half2(u[2 * r], u[2 * r + 1]);
+            bf[nt][r][0] = transpose8x8(h);
+            if constexpr (PP == 2) {
+              const float2 f = unpack_half2(h);
+              bf[nt][r][1] = transpose8x8(pack_half2(u[2 * r] - f.x, u[2 * r + 1] - f.y));
+            }
+          }
+        }
+#pragma unroll
+        for (int m2 = 0; m2 < 2; ++m2) {
+          uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
+          uint32_t a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
+          if constexpr (kCentred) {
+            a0 = centred(a0, kMiddleLow), a1 = centred(a1, kMiddleHigh);
+            a2 = centred(a2, kMiddleLow), a3 = centred(a3, kMiddleHigh);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int pp = 0; pp < PP; ++pp) mma_f16(o[nt][j][m2], a0, a1, a2, a3, bf[nt][0][pp], bf[nt][1][pp]);
+          x01 >>= 8;
+          x23 >>= 8;
+        }
+      }
+    };
+
+    auto arrived = [&](int32_t k) {
+      const uint32_t at = used + static_cast<uint32_t>(k);
+      return __all_sync(0xffffffffu, mbar_wait(&bars[warp][at % G::kStages], (at / G::kStages) & 1u, a.err, kErrWaitFull));
+    };
+    for (int32_t k = 0; k < tiles; ++k) {
+      if (k + G::kStages - 1 < tiles) issue(k + G::kStages - 1);
+      if (!arrived(k)) {  // the copies in flight still land in this ring
+        for (int32_t d = k + 1; d < min(tiles, k + G::kStages); ++d) arrived(d);
+        failed = true;
+        break;
+      }
+      const uint32_t st = (used + k) % G::kStages;
+      if (loaded[warp][st]) {
+        const int32_t key0 = (first_tile + k * kWarps) * static_cast<int32_t>(kKv4Tile);
+        const uint8_t* p = ring + st * G::kBytes;
+        if (key0 >= rows.lo_max && key0 + static_cast<int32_t>(kKv4Tile) - 1 <= rows.hi_min)
+          tile_step(p, key0, std::false_type{});
+        else
+          tile_step(p, key0, std::true_type{});
+      }
+      __syncwarp();  // every lane has read the stage before it is filled again
     }
-    // ---- weights
-    float w[NT][4];
+    used += static_cast<uint32_t>(tiles);
+
+    // ---- this warp's result, then the block's
+    float* mine = reinterpret_cast<float*>(ring);  // [8 NT][D]
+    const float unit_f = pm_limit < 0.f ? 0.f : 1.f / pm;
+    const float low = kCentred ? unit_f : unit_f * kCodeLow, high = kCentred ? unit_f * 0.0625f : unit_f * kCodeHigh;
+    __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        w[nt][c] = exp2_approx(raw[nt][c] - m[nt][c]);
-        w[nt][2 + c] = exp2_approx(raw[nt][2 + c] - m[nt][c]);
-        l[nt][c] += w[nt][c] + w[nt][2 + c];
-      }
-    // ---- values
-    float wp[NT][4];
-    uint32_t vw[4][NG / 2], p0[NG], p1[NG];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) lds(vw[r], st + G::kValues + (tok_v[r & 1] + 8 * (r >> 1)) * G::kRowBytes + g * 2 * NG);
-    lds(p0, st + G::kValueParams + tok_g * 4 * NG);
-    lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
-    if constexpr (kMasked) {
+        for (int d = 4; d < 32; d <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
+        const int col = 8 * nt + 2 * static_cast<int>(i4) + c;
+        // a column that saw no key; one whose scores are all NaN has l = NaN and is none
+        const bool none = trigger[nt][c] == -INFINITY && l[nt][c] == 0.f;
+        if (g == 0) warp_ml[warp][col] = make_float2(none ? -INFINITY : m[nt][c], l[nt][c]);
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        if (!keep[0]) p0[j] = 0u;
-        if (!keep[1]) p1[j] = 0u;
-      }
-    }
-    float smax = 0.f;
+        for (int j = 0; j < NG; ++j) {
+          float z;
+          if constexpr (kCentred) {
+            z = zsum[nt][j][c];
 #pragma unroll
-    for (int j = 0; j < NG; ++j)
-      smax = max3(smax, unpack_half2(p0[j]).x, unpack_half2(p1[j]).x);
-    if (__any_sync(0xffffffffu, smax > pm_limit)) {
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
-      // a largest scale of zero sets no measure for those to come
-      const float next = pow2_toward(smax, 5);
-      const float ratio = pm_limit < 0.f ? 0.f : next / pm;
-      pm = next;
-      pm_limit = smax > 0.f ? 128.f / next : 0.f;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < NG; ++j)
+            for (int d = 4; d < 32; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+          } else {
+            z = __shfl_sync(0xffffffffu, oz[nt][c], 4 * j + i4);
+          }
+          float2* to = reinterpret_cast<float2*>(mine + col * D + 32 * j + 4 * g);
 #pragma unroll
           for (int m2 = 0; m2 < 2; ++m2)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[nt][j][m2][e] *= ratio;
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) wp[nt][e] = w[nt][e] * pm;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-      uint32_t x01 = __byte_perm(vw[0][j / 2], vw[1][j / 2], sel);
-      uint32_t x23 = __byte_perm(vw[2][j / 2], vw[3][j / 2], sel);
-      float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
-      if constexpr (kCentred) {
-        f0.y = fmaf(8.f, f0.x, f0.y);
-        f1.y = fmaf(8.f, f1.x, f1.y);
-      }
-      uint32_t bf[NT][2][PP];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float u[4], zw[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = e < 2 ? f0 : f1;
-          u[e] = wp[nt][e] * f.x;
-          zw[e] = w[nt][e] * f.y;
-          if constexpr (kMasked) {
-            if (!vis[nt][e]) u[e] = zw[e] = 0.f;
-          }
-        }
-        zsum[nt][j][0] += zw[0] + zw[2];
-        zsum[nt][j][1] += zw[1] + zw[3];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint32_t h = pack_half2(u[2 * r], u[2 * r + 1]);
-          bf[nt][r][0] = transpose8x8(h);
-          if constexpr (PP == 2) {
-            const float2 f = unpack_half2(h);
-            bf[nt][r][1] = transpose8x8(pack_half2(u[2 * r] - f.x, u[2 * r + 1] - f.y));
-          }
+            to[m2] = make_float2(fmaf(o[nt][j][m2][c], low, z), fmaf(o[nt][j][m2][2 + c], high, z));
         }
       }
+    __syncthreads();
+    const bool whole = take == units;
+    const uint32_t slot = blockIdx.x * 2 + (offset == 0 ? 1u : 0u);
+    const float* all = reinterpret_cast<const float*>(smem);
+    constexpr int kWarpFloats = G::kStages * G::kBytes / 4;
+    for (uint32_t e = threadIdx.x; e < rows.count * (D / 4); e += kThreads) {
+      const uint32_t col = e / (D / 4), c4 = e % (D / 4);
+      float top = -INFINITY;
 #pragma unroll
-      for (int m2 = 0; m2 < 2; ++m2) {
-        uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
-        uint32_t a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
-        if constexpr (kCentred) {
-          a0 = centred(a0, kMiddleLow), a1 = centred(a1, kMiddleHigh);
-          a2 = centred(a2, kMiddleLow), a3 = centred(a3, kMiddleHigh);
-        }
+      for (int wi = 0; wi < kWarps; ++wi) top = fmaxf(top, warp_ml[wi][col].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float total = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int pp = 0; pp < PP; ++pp) mma_f16(o[nt][j][m2], a0, a1, a2, a3, bf[nt][0][pp], bf[nt][1][pp]);
-        x01 >>= 8;
-        x23 >>= 8;
+      for (int wi = 0; wi < kWarps; ++wi) {
+        const float2 ml = warp_ml[wi][col];
+        if (ml.x == -INFINITY) continue;
+        const float f = exp2_approx(ml.x - base);
+        const float4 x = *reinterpret_cast<const float4*>(all + wi * kWarpFloats + col * D + 4 * c4);
+        total = fmaf(f, ml.y, total);
+        sum.x = fmaf(f, x.x, sum.x);
+        sum.y = fmaf(f, x.y, sum.y);
+        sum.z = fmaf(f, x.z, sum.z);
+        sum.w = fmaf(f, x.w, sum.w);
+      }
+      if (whole) {
+        const uint32_t row = rows.first + col;
+        const uint64_t token = seq.row0 + row / a.share;
+        const uint32_t qh = head * a.share + row % a.share;
+        const float inv = top == -INFINITY ? 0.f : 1.0f / total;
+        store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c4,
+               make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+        if (c4 == 0 && a.lse != nullptr)
+          a.lse[token * a.heads + qh] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
+      } else {
+        const uint64_t at = static_cast<uint64_t>(slot) * kRows + col;
+        *reinterpret_cast<float4*>(a.part_o + at * D + 4 * c4) = sum;
+        if (c4 == 0) a.part_ml[at] = make_float2(top, total);
       }
     }
-  };
-
-  auto arrived = [&](int32_t k) {
-    return __all_sync(0xffffffffu, mbar_wait(&bars[warp][k % G::kStages],
-                                             static_cast<uint32_t>(k / G::kStages) & 1u, a.err, kErrWaitFull));
-  };
-  for (int32_t k = 0; k < tiles; ++k) {
-    if (k + G::kStages - 1 < tiles) issue(k + G::kStages - 1);
-    const int st = k % G::kStages;
-    if (!arrived(k)) {  // gave up (reported in *err): the copies in flight still land in this ring
-      for (int32_t d = k + 1; d < min(tiles, k + G::kStages); ++d) arrived(d);
-      break;
+    if (!whole && offset == 0 && threadIdx.x == 0) {
+      const uint32_t last = static_cast<uint32_t>((unit + units - 1) / share.per);
+      a.part_of[blockIdx.x] = make_uint4(1u, pair, head, min(last, gridDim.x - 1));
     }
-    if (loaded[warp][st]) {
-      const int32_t key0 = (t0 + static_cast<int32_t>(warp) + k * kWarps) * static_cast<int32_t>(kKv4Tile);
-      const uint8_t* p = ring + st * G::kBytes;
-      if (key0 >= rows.lo_max && key0 + static_cast<int32_t>(kKv4Tile) - 1 <= rows.hi_min)
-        tile_step(p, key0, std::false_type{});
-      else
-        tile_step(p, key0, std::true_type{});
-    }
-    __syncwarp();  // every lane has read the stage before it is filled again
+    unit += take;
+    offset = 0;
+    if (++head == a.view.kv_heads) head = 0, ++pair;
+    fence_proxy_async_smem();  // the next item's copies overwrite what was written and read here
+    __syncthreads();
   }
+}
 
-  // ---- this warp's result, then the block's
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
-#pragma unroll
-        for (int j = 0; j < NG; ++j) zsum[nt][j][c] += __shfl_xor_sync(0xffffffffu, zsum[nt][j][c], d);
-      }
-    }
-  float* mine = reinterpret_cast<float*>(ring);  // [8 NT][D]
-  const float unit = pm_limit < 0.f ? 0.f : 1.f / pm;
-  const float low = kCentred ? unit : unit * kCodeLow, high = kCentred ? unit * 0.0625f : unit * kCodeHigh;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int col = 8 * nt + 2 * static_cast<int>(i4) + c;
-      // a column that saw no key; one whose scores are all NaN has l = NaN and is none
-      const bool none = trigger[nt][c] == -INFINITY && l[nt][c] == 0.f;
-      if (g == 0) warp_ml[warp][col] = make_float2(none ? -INFINITY : m[nt][c], l[nt][c]);
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        float2* to = reinterpret_cast<float2*>(mine + col * D + 32 * j + 4 * g);
-#pragma unroll
-        for (int m2 = 0; m2 < 2; ++m2)
-          to[m2] = make_float2(fmaf(o[nt][j][m2][c], low, zsum[nt][j][c]), fmaf(o[nt][j][m2][2 + c], high, zsum[nt][j][c]));
-      }
-    }
-  __syncthreads();
-  const float* all = reinterpret_cast<const float*>(smem);
-  constexpr int kWarpFloats = G::kStages * G::kBytes / 4;
-  for (uint32_t e = threadIdx.x; e < rows.count * (D / 4); e += kThreads) {
-    const uint32_t col = e / (D / 4), c4 = e % (D / 4);
+// Joins the parts of every item that was split: block x looks at what block x of the first kernel
+// began and did not finish, whose other parts lie in slot 0 of the blocks behind it; grid y deals out
+// the channels.  The parts of a (row, four channels) are dealt to `lanes` threads and their sums added
+// in a fixed order.
+constexpr int kJoinThreads = 512;
+template <int D> constexpr int kJoinColumns = D / 4 < 16 ? D / 4 : 16;  // float4 columns of a block
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const KernelArgs a, uint32_t rows_per_tile) {
+  constexpr int kCols = kJoinColumns<D>;
+  constexpr int kParts = kJoinThreads / kCols;  // threads over (row, part)
+  __shared__ float4 part[kJoinThreads];
+  __shared__ float part_l[kParts], part_top[kParts];
+  griddep_wait();
+  const uint4 of = a.part_of[blockIdx.x];
+  if (of.x == 0u) return;
+  const uint32_t parts = of.w - blockIdx.x + 1;
+  Kv4Seq seq;
+  Rows rows;
+  if (!item_rows(a, of.y, rows_per_tile, &seq, &rows)) return;
+  const uint32_t c4 = threadIdx.x % kCols, who = threadIdx.x / kCols;
+  uint32_t lanes = kParts;  // threads per row: a power of two
+  while (lanes > 1 && lanes * rows.count > static_cast<uint32_t>(kParts)) lanes >>= 1;
+  const uint32_t per_pass = kParts / lanes, sub = who % lanes;
+  for (uint32_t r0 = 0; r0 < rows.count; r0 += per_pass) {
+    const uint32_t col = r0 + who / lanes;
+    const bool live = col < rows.count;
+    auto place = [&](uint32_t p) {
+      return (static_cast<uint64_t>(blockIdx.x + p) * 2 + (p == 0 ? 1u : 0u)) * rows_per_tile + col;
+    };
     float top = -INFINITY;
-#pragma unroll
-    for (int wi = 0; wi < kWarps; ++wi) top = fmaxf(top, warp_ml[wi][col].x);
+    if (live)
+#pragma unroll 4
+      for (uint32_t p = sub; p < parts; p += lanes) top = fmaxf(top, a.part_ml[place(p)].x);
+    if (c4 == 0) part_top[who] = top;
+    __syncthreads();
+    for (uint32_t i = 0; i < lanes; ++i) top = fmaxf(top, part_top[who - sub + i]);
     const float base = top == -INFINITY ? 0.f : top;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     float total = 0.f;
-#pragma unroll
-    for (int wi = 0; wi < kWarps; ++wi) {
-      const float2 ml = warp_ml[wi][col];
-      if (ml.x == -INFINITY) continue;
-      const float f = exp2_approx(ml.x - base);
-      const float4 x = *reinterpret_cast<const float4*>(all + wi * kWarpFloats + col * D + 4 * c4);
-      total = fmaf(f, ml.y, total);
-      sum.x = fmaf(f, x.x, sum.x);
-      sum.y = fmaf(f, x.y, sum.y);
-      sum.z = fmaf(f, x.z, sum.z);
-      sum.w = fmaf(f, x.w, sum.w);
-    }
-    const uint32_t row = rows.first + col;
-    const uint64_t token = seq.row0 + row / a.share;
-    const uint32_t qh = head * a.share + row % a.share;
-    if (a.splits == 1) {
+    if (live)
+#pragma unroll 8
+      for (uint32_t p = sub; p < parts; p += lanes) {
+        const uint64_t at = place(p);
+        const float2 ml = a.part_ml[at];
+        const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * D + 4 * (blockIdx.y * kCols + c4));
+        if (ml.x == -INFINITY) continue;
+        const float f = exp2_approx(ml.x - base);
+        total = fmaf(f, ml.y, total);
+        sum.x = fmaf(f, x.x, sum.x);
+        sum.y = fmaf(f, x.y, sum.y);
+        sum.z = fmaf(f, x.z, sum.z);
+        sum.w = fmaf(f, x.w, sum.w);
+      }
+    part[threadIdx.x] = sum;
+    if (c4 == 0) part_l[who] = total;
+    __syncthreads();
+    if (live && sub == 0) {
+      for (uint32_t i = 1; i < lanes; ++i) {
+        const float4 x = part[threadIdx.x + i * kCols];
+        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+        total += part_l[who + i];
+      }
+      const uint32_t row = rows.first + col;
+      const uint64_t token = seq.row0 + row / a.share;
+      const uint32_t qh = of.z * a.share + row % a.share;
       const float inv = top == -INFINITY ? 0.f : 1.0f / total;
-      store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c4,
+      store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * (blockIdx.y * kCols + c4),
              make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
-      if (c4 == 0 && a.lse != nullptr)
+      if (c4 == 0 && blockIdx.y == 0 && a.lse != nullptr)
         a.lse[token * a.heads + qh] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
-    } else {
-      const uint64_t at = (split * a.view.tokens + token) * a.heads + qh;
-      *reinterpret_cast<float4*>(a.part_o + at * D + 4 * c4) = sum;
-      if (c4 == 0) a.part_ml[at] = make_float2(top, total);
     }
+    __syncthreads();
   }
 }
 
-// Joins the splits of every row: four warps take the splits in turn.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) kv4_join_kernel(const KernelArgs a, uint32_t rows_per_tile) {
-  __shared__ float4 part[kWarps][D / 4];
-  __shared__ float part_l[kWarps];
-  griddep_wait();
-  Kv4Seq seq;
-  if (!kv4_seq(a.view, blockIdx.y, &seq)) return;
-  const uint32_t r = blockIdx.x;  // token * heads + head
-  if (r >= seq.n * a.heads) return;
-  const uint32_t t = r / a.heads, qh = r % a.heads;
-  // the splits that have keys: those of the row tile this row was computed in
-  const uint32_t row = t * a.share + qh % a.share;
-  Rows rows;
-  row_range(a, seq, row / rows_per_tile, rows_per_tile, &rows);
-  const uint32_t tiles = static_cast<uint32_t>(rows.t_end - rows.t_begin);
-  const uint32_t splits = max(1u, min(a.splits, (tiles + a.span - 1) / a.span));
-  const uint64_t token = seq.row0 + t, stride = a.view.tokens * a.heads, at = token * a.heads + qh;
-  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  float top = -INFINITY;
-  for (uint32_t s = lane; s < splits; s += 32) top = fmaxf(top, a.part_ml[s * stride + at].x);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  const float base = top == -INFINITY ? 0.f : top;
-  constexpr int kVec = (D / 4 + 31) / 32;
-  float4 sum[kVec];
-  float total = 0.f;
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (uint32_t s = warp; s < splits; s += kWarps) {
-    const float2 ml = a.part_ml[s * stride + at];
-    if (ml.x == -INFINITY) continue;
-    const float f = exp2_approx(ml.x - base);
-    total = fmaf(f, ml.y, total);
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const uint32_t c = lane + 32 * i;
-      if (c >= D / 4) continue;
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + (s * stride + at) * D + 4 * c);
-      sum[i].x = fmaf(f, x.x, sum[i].x);
-      sum[i].y = fmaf(f, x.y, sum[i].y);
-      sum[i].z = fmaf(f, x.z, sum[i].z);
-      sum[i].w = fmaf(f, x.w, sum[i].w);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kVec; ++i)
-    if (lane + 32 * i < D / 4) part[warp][lane + 32 * i] = sum[i];
-  if (lane == 0) part_l[warp] = total;
-  __syncthreads();
-  total = part_l[0] + part_l[1] + part_l[2] + part_l[3];
-  for (uint32_t c = threadIdx.x; c < D / 4; c += kThreads) {
-    float4 v = part[0][c];
-#pragma unroll
-    for (int wi = 1; wi < kWarps; ++wi) {
-      const float4 x = part[wi][c];
-      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-    }
-    const float inv = top == -INFINITY ? 0.f : 1.0f / total;
-    store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c,
-           make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-  }
-  if (threadIdx.x == 0 && a.lse != nullptr)
-    a.lse[at] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
-}
-
+template <typename T> constexpr int kQueryParts = sizeof(T) == 4 ? 2 : 1;
 template <typename T, int D, int NT>
-cudaError_t launch(const KernelArgs& a, uint32_t kv_heads, cudaStream_t stream) {
+cudaError_t launch(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream) {
   using G = Geometry<D>;
-  constexpr int QP = sizeof(T) == 4 ? 2 : 1;
+  constexpr int QP = kQueryParts<T>;
   constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
   constexpr size_t kSmem = static_cast<size_t>(kWarps) * G::kStages * G::kBytes;
   static_assert(G::kStages * G::kBytes >= 8 * NT * D * 4, "the ring holds the warp's result at the end");
   const auto kernel = kv4_attention_kernel<T, D, NT, QP, PP>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
   if (e != cudaSuccess) return e;
-  const dim3 grid(a.splits, kv_heads * a.row_tiles, a.view.batch);
-  kernel<<<grid, kThreads, kSmem, stream>>>(a);
+  kernel<<<plan.blocks, kThreads, kSmem, stream>>>(a);
   e = cudaGetLastError();
-  if (e != cudaSuccess || a.splits == 1) return e;
+  if (e != cudaSuccess || plan.workspace == 0) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.view.max_tokens * a.heads, a.view.batch);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(plan.blocks, D / 4 / kJoinColumns<D>);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -708,12 +887,12 @@ cudaError_t launch(const KernelArgs& a, uint32_t kv_heads, cudaStream_t stream) 
 template <typename T, int D>
 cudaError_t dispatch(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream) {
   switch (plan.row_tile) {
-    case 8: return launch<T, D, 1>(a, a.view.kv_heads, stream);
+    case 8: return launch<T, D, 1>(a, plan, stream);
     case 16:
-      if constexpr (kMaxRowGroups<D> >= 2) return launch<T, D, 2>(a, a.view.kv_heads, stream);
+      if constexpr (kMaxRowGroups<D> >= 2) return launch<T, D, 2>(a, plan, stream);
       return cudaErrorInvalidValue;
     case 32:
-      if constexpr (kMaxRowGroups<D> >= 4) return launch<T, D, 4>(a, a.view.kv_heads, stream);
+      if constexpr (kMaxRowGroups<D> >= 4) return launch<T, D, 4>(a, plan, stream);
       return cudaErrorInvalidValue;
     default: return cudaErrorInvalidValue;
   }
@@ -734,27 +913,23 @@ cudaError_t dispatch_dim(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t 
 bool kv4_attention_supported(uint32_t dim) { return dim == 64 || dim == 128 || dim == 256; }
 
 Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint32_t batch, uint32_t max_tokens,
-                           uint32_t max_kv_len, uint64_t tokens, uint32_t window) {
+                           uint32_t max_kv_len, ElementType type) {
   Kv4Plan p;
   const uint64_t rows = static_cast<uint64_t>(max_tokens) * (heads / kv_heads);
-  const uint32_t most = dim == 64 ? 32 : (dim == 128 ? 16 : 8);
+  const uint32_t most = dim == 64 ? 8 * kMaxRowGroups<64> : 8 * (dim == 128 ? kMaxRowGroups<128> : kMaxRowGroups<256>);
   p.row_tile = 8;
   while (p.row_tile < most && p.row_tile < rows) p.row_tile *= 2;
-  p.row_tiles = static_cast<uint32_t>((rows + p.row_tile - 1) / p.row_tile);
-  uint64_t keys = max_kv_len;
-  // a row tile spans at most row_tile tokens; its window's first key may start mid-tile
-  if (window != 0 && keys > static_cast<uint64_t>(window) + p.row_tile) keys = static_cast<uint64_t>(window) + p.row_tile + 15;
-  const uint64_t tiles = (keys + kKv4Tile - 1) / kKv4Tile + (window != 0 ? 1 : 0);
+  p.row_tiles = (rows + p.row_tile - 1) / p.row_tile;
+  // One wave: as many blocks as the SMs hold, each with an equal share of the units, or a block per
+  // unit where there are fewer (of the longest sequences the call allows).
+  const uint64_t resident = 148ull * blocks_per_sm(static_cast<int>(dim), static_cast<int>(p.row_tile / 8), type == kF32 ? 2 : 1);
+  const uint64_t tiles = (static_cast<uint64_t>(max_kv_len) + kKv4Tile - 1) / kKv4Tile;
+  const uint64_t item = tiles <= kWarps ? 1 : (tiles + kWarps - 1) / kWarps;
   const uint64_t items = static_cast<uint64_t>(batch) * kv_heads * p.row_tiles;
-  // Two blocks per SM and two waves of them; a block takes at least two tiles per warp.
-  const uint64_t want = 148ull * 4;
-  uint64_t splits = items >= want ? 1 : (want + items - 1) / (items == 0 ? 1 : items);
-  uint64_t span = splits == 0 ? tiles : (tiles + splits - 1) / splits;
-  span = (span + kWarps - 1) / kWarps * kWarps;
-  if (span < 2 * kWarps) span = 2 * kWarps;
-  p.span = static_cast<uint32_t>(span);
-  p.splits = static_cast<uint32_t>(tiles == 0 ? 1 : (tiles + span - 1) / span);
-  if (p.splits > 1) p.workspace = (p.splits * tokens * heads) * (static_cast<uint64_t>(dim) * 4 + 8);
+  p.blocks = static_cast<uint32_t>(items >= resident || items * item >= resident ? resident : items * item);
+  // an item of one unit is never split
+  if (item > 1)
+    p.workspace = static_cast<uint64_t>(p.blocks) * (2 * p.row_tile * (static_cast<uint64_t>(dim) * 4 + 8) + 16);
   return p;
 }
 
@@ -774,11 +949,13 @@ cudaError_t kv4_attention(const Kv4AttnArgs& in, const Kv4Plan& plan, cudaStream
   a.share = in.heads / in.view.kv_heads;
   a.causal = in.causal ? 1 : 0;
   a.window = in.window;
-  a.row_tiles = plan.row_tiles;
-  a.span = plan.span;
-  a.splits = plan.splits;
-  a.part_o = static_cast<float*>(in.workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<uint64_t>(plan.splits) * in.view.tokens * in.heads * in.view.dim);
+  a.row_tiles = static_cast<uint32_t>(plan.row_tiles);
+  if (plan.workspace > 0) {
+    const uint64_t parts = 2ull * plan.blocks * plan.row_tile;
+    a.part_o = static_cast<float*>(in.workspace);
+    a.part_of = reinterpret_cast<uint4*>(a.part_o + parts * in.view.dim);
+    a.part_ml = reinterpret_cast<float2*>(a.part_of + plan.blocks);
+  }
   a.err = in.err;
   switch (in.type) {
     case kF32: return dispatch_dim<float>(a, plan, stream);

@@ -84,7 +84,7 @@ __device__ __forceinline__ bool kv4_seq(const Kv4View& v, uint32_t b, Kv4Seq* s)
   const bool ok = len >= 0 && static_cast<uint32_t>(len) <= v.max_kv_len && r0 >= 0 && r1 >= r0 &&
                   static_cast<uint64_t>(r1) <= v.tokens && static_cast<uint32_t>(r1 - r0) <= v.max_tokens;
   if (!ok) {
-    if (threadIdx.x == 0) atomicOr(v.bad, 1u);
+    atomicOr(v.bad, 1u);
     return false;
   }
   s->row0 = static_cast<uint64_t>(r0);

@@ -65,16 +65,15 @@ cudaError_t kv4_load(const Kv4RowArgs& a, cudaStream_t stream);
 
 // ---------------------------------------------------------------- attention over it
 bool kv4_attention_supported(uint32_t dim);
-// How a call's keys are split over thread blocks, from sizes the host knows.
+// How a call is laid out over thread blocks, from sizes the host knows.
 struct Kv4Plan {
-  uint32_t row_tile = 0;   // query rows of one block
-  uint32_t row_tiles = 0;  // blocks' row tiles per (sequence, key head)
-  uint32_t span = 0;       // 16-key tiles of one block
-  uint32_t splits = 0;     // blocks along the keys
-  uint64_t workspace = 0;  // bytes; 0 when splits == 1
+  uint32_t row_tile = 0;   // query rows (token, head of a key head's share) of one item
+  uint64_t row_tiles = 0;  // items per (sequence, key head)
+  uint32_t blocks = 0;
+  uint64_t workspace = 0;  // bytes; 0 when no item can be split
 };
 Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint32_t batch, uint32_t max_tokens,
-                           uint32_t max_kv_len, uint64_t tokens, uint32_t window);
+                           uint32_t max_kv_len, ElementType type);
 struct Kv4AttnArgs {
   Kv4View view;
   ElementType type = kF32;

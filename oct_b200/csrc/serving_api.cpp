@@ -181,10 +181,9 @@ int check_attention(const OctB200Kv4Cache* c, const OctB200Kv4Batch* b, const Oc
   if (r->q_heads > 65535u || static_cast<uint64_t>(b->max_tokens) * r->q_heads > 0x7fffffffull)
     return OCT_B200_DETAIL_UNSUPPORTED_SHAPE;
   *plan = oct::kv4_attention_plan(c->head_dim, c->kv_heads, r->q_heads, b->batch, b->max_tokens, b->max_kv_len,
-                                  r->tokens, r->window);
-  // blocks along y: one per key head and tile of rows
-  if (static_cast<uint64_t>(plan->row_tiles) * c->kv_heads > 65535ull) return OCT_B200_DETAIL_UNSUPPORTED_SHAPE;
-  return 0;
+                                  static_cast<oct::ElementType>(r->dtype));
+  // every block looks through the (sequence, row tile) pairs
+  return plan->row_tiles * b->batch > 0x3fffffffull ? OCT_B200_DETAIL_UNSUPPORTED_SHAPE : 0;
 }
 
 }  // namespace

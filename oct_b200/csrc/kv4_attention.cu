@@ -27,8 +27,10 @@
 // has nothing to do beside it, which is why this runs on warp-level matrix
 // instructions whose operands come from registers instead of through tcgen05
 // and tensor memory.  Each warp streams its own tiles (16 tokens, keys and
-// values side by side, one bulk copy) through a private ring in shared memory:
-// no barrier between warps until the end.
+// values side by side) through a private ring in shared memory, by 16-byte
+// asynchronous copies: no barrier between warps until an item's end, and none
+// of the per-copy cost that bulk copies have at these sizes (a bulk copy a tile
+// streamed at 4.6 TB/s with no arithmetic at all).
 //
 // Blocks take equal runs of the call's tiles, whatever the sequences' lengths:
 // each adds up the lengths on the device and finds its own run.  An item that
@@ -49,6 +51,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum is renewed only when a score exceeds it by this much (in
 // powers of two): weights stay below 2^8, and most tiles skip the exchange.
 constexpr float kSlack = 8.f;
+constexpr uint32_t kNoTile = 0xffffffffu;
 constexpr float kCodeLow = 16777216.f, kCodeHigh = 1048576.f;  // 2^24, 2^20
 
 template <int D>
@@ -117,6 +120,16 @@ __device__ __forceinline__ float pow2_toward(float x, int target) {
   return __uint_as_float(static_cast<uint32_t>(f < 1 ? 1 : (f > 254 ? 254 : f)) << 23);
 }
 
+// 16 bytes from global into shared memory, past the L1 cache; waits count commit groups.
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void lds(uint32_t (&w)[N], const uint8_t* p) {
   if constexpr (N == 1) {
@@ -146,7 +159,6 @@ struct KernelArgs {
   float* part_o;    // [blocks][2][rows of a tile][D]
   float2* part_ml;  // [blocks][2][rows of a tile]
   uint4* part_of;   // [blocks]: what the block's unfinished last item is, for the join
-  unsigned int* err;
 };
 
 // The keys that the rows of one row tile see: row r of a sequence is query
@@ -190,55 +202,69 @@ __device__ __forceinline__ bool item_rows(const KernelArgs& a, uint32_t pair, ui
   const uint32_t b = pair / a.row_tiles;
   return kv4_seq(a.view, b, s) && row_range(a, *s, pair - b * a.row_tiles, rows_per_tile, r);
 }
+// What an item costs beside its units, in units: finding its pages, loading its queries, joining its
+// warps (about 5 us against 1.4 us of a unit).  Counted where blocks get several units, so that one
+// with many short items gets fewer of them; where units are few, latency counts and each has its block.
+constexpr uint32_t kItemCost = 3;
 struct Share {
-  unsigned long long begin, end, per;  // this block's units; units of every block
-  uint32_t pair, head, offset;         // where its first unit lies
+  unsigned long long begin, end, per;  // this block's run of all items' units and costs; every block's
+  uint32_t cost;                       // kItemCost or 0
+  uint32_t pair, head, offset;         // where it begins
 };
 // Called by the whole block.
 __device__ __forceinline__ bool find_share(const KernelArgs& a, uint32_t rows_per_tile, Share* out) {
-  __shared__ unsigned long long warp_sums[kWarps];
+  __shared__ unsigned long long warp_sums[2][kWarps];
   __shared__ uint32_t found[3];
   const uint32_t pairs = a.view.batch * a.row_tiles, chunk = (pairs + kThreads - 1) / kThreads;
   const uint32_t p0 = min(pairs, threadIdx.x * chunk), p1 = min(pairs, p0 + chunk);
-  unsigned long long mine = 0;
+  unsigned long long sums[2] = {0, 0};  // units, items
   Kv4Seq s;
   Rows r;
   for (uint32_t p = p0; p < p1; ++p)
-    if (item_rows(a, p, rows_per_tile, &s, &r)) mine += item_units(r);
-  mine *= a.view.kv_heads;
-  unsigned long long upto = mine;
+    if (item_rows(a, p, rows_per_tile, &s, &r)) sums[0] += item_units(r), ++sums[1];
+  unsigned long long upto[2];
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const unsigned long long v = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= static_cast<uint32_t>(d)) upto += v;
-  }
-  if (lane == 31) warp_sums[warp] = upto;
-  __syncthreads();
-  unsigned long long total = 0;
+  for (int i = 0; i < 2; ++i) {
+    sums[i] *= a.view.kv_heads;
+    upto[i] = sums[i];
 #pragma unroll
-  for (uint32_t w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += warp_sums[w];
-    total += warp_sums[w];
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned long long v = __shfl_up_sync(0xffffffffu, upto[i], d);
+      if (lane >= static_cast<uint32_t>(d)) upto[i] += v;
+    }
+    if (lane == 31) warp_sums[i][warp] = upto[i];
   }
-  out->per = (total + gridDim.x - 1) / gridDim.x;
+  __syncthreads();
+  unsigned long long total[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) {
+      if (w < warp) upto[i] += warp_sums[i][w];
+      total[i] += warp_sums[i][w];
+    }
+  out->cost = total[0] > 4ull * gridDim.x ? kItemCost : 0;
+  const unsigned long long all = total[0] + out->cost * total[1];
+  out->per = all <= gridDim.x ? 1 : (all + gridDim.x - 1) / gridDim.x;
   out->begin = blockIdx.x * out->per;
-  out->end = min(total, out->begin + out->per);
-  if (out->begin >= total) return false;
-  unsigned long long at = upto - mine;
-  if (out->begin >= at && out->begin < upto)
+  out->end = min(all, out->begin + out->per);
+  if (out->begin >= all) return false;
+  const unsigned long long last = upto[0] + out->cost * upto[1];
+  unsigned long long at = last - (sums[0] + out->cost * sums[1]);
+  if (out->begin >= at && out->begin < last)
     for (uint32_t p = p0; p < p1; ++p)
       if (item_rows(a, p, rows_per_tile, &s, &r)) {
-        const uint32_t units = item_units(r);
-        const unsigned long long all = static_cast<unsigned long long>(units) * a.view.kv_heads;
-        if (out->begin < at + all) {
+        const uint32_t size = item_units(r) + out->cost;
+        const unsigned long long heads = static_cast<unsigned long long>(size) * a.view.kv_heads;
+        if (out->begin < at + heads) {
           const uint32_t rest = static_cast<uint32_t>(out->begin - at);
           found[0] = p;
-          found[1] = rest / units;
-          found[2] = rest % units;
+          found[1] = rest / size;
+          found[2] = rest % size;
           break;
         }
-        at += all;
+        at += heads;
       }
   __syncthreads();
   out->pair = found[0];
@@ -257,7 +283,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   constexpr int kRows = 8 * NT;
   constexpr bool kCentred = std::is_same<T, float>::value;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t bars[kWarps][G::kStages];
   __shared__ uint32_t loaded[kWarps][G::kStages];
   __shared__ float2 warp_ml[kWarps][kRows];
 
@@ -269,14 +294,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
 
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, i4 = lane % 4;
   uint8_t* ring = smem + warp * (G::kStages * G::kBytes);
-  if (lane == 0) {
-    for (int st = 0; st < G::kStages; ++st) mbar_init(&bars[warp][st], 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
-  uint32_t used = 0;   // tiles this warp has had in its ring before the current item
-  bool failed = false;  // a wait gave up (reported in *err)
-
   // Token of score row g (and, 8 further, of row g + 8): an order in which a
   // quarter warp's key loads touch every bank once and the value loads twice.
   const int32_t tok_g = (g & 1) ? 4 + static_cast<int32_t>((g >> 1) ^ 1u) : static_cast<int32_t>(g >> 1);
@@ -292,42 +309,48 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       ++pair;
       continue;
     }
-    const uint32_t units = item_units(rows);
-    const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(units - offset), share.end - unit));
-    const int32_t t0 = rows.t_begin + static_cast<int32_t>(offset * kWarps);
-    const int32_t t1 = min(rows.t_end, t0 + static_cast<int32_t>(take * kWarps));
+    const uint32_t size = item_units(rows) + share.cost;
+    const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(size - offset), share.end - unit));
+    // the item's cost comes first in its run; the units behind it are its tiles
+    const uint32_t unit0 = max(offset, share.cost) - share.cost, unit1 = max(offset + take, share.cost) - share.cost;
+    const int32_t t0 = rows.t_begin + static_cast<int32_t>(unit0 * kWarps);
+    const int32_t t1 = min(rows.t_end, rows.t_begin + static_cast<int32_t>(unit1 * kWarps));
     const int32_t first_tile = t0 + static_cast<int32_t>(warp);
-    const int32_t tiles = !failed && first_tile < t1 ? (t1 - first_tile + kWarps - 1) / kWarps : 0;
+    const int32_t tiles = first_tile < t1 ? (t1 - first_tile + kWarps - 1) / kWarps : 0;
 
-    // Where this warp's next 32 tiles lie, one per lane (null: no page of the cache).
+    // Which of the cache's tiles this warp's next 32 are, one per lane (kNoTile: no page of the cache).
     const int32_t* table = a.view.table + pair / a.row_tiles * a.view.table_stride;
-    const uint8_t* source = nullptr;
+    uint32_t source = kNoTile;
     auto locate = [&](int32_t k0) {
       const int32_t k = k0 + static_cast<int32_t>(lane);
-      source = nullptr;
+      source = kNoTile;
       if (k >= tiles) return;
       const uint32_t t = static_cast<uint32_t>(first_tile + k * kWarps);
       const uint32_t in_table = t / a.view.page_tiles;
       const uint32_t page = static_cast<uint32_t>(table[in_table]);
       if (page < a.view.pages)
-        source = kv4_tile(a.view, page, head, t - in_table * a.view.page_tiles, G::kBytes);
+        source = (page * a.view.kv_heads + head) * a.view.page_tiles + t - in_table * a.view.page_tiles;
       else
         atomicOr(a.view.bad, 1u);
     };
-    auto issue = [&](int32_t k) {  // tile k of this warp into its stage (whole warp)
-      if (k % 32 == 0) locate(k);
-      const uint32_t st = (used + k) % G::kStages;
-      if (lane == static_cast<uint32_t>(k % 32)) {
-        loaded[warp][st] = source != nullptr;
-        if (source != nullptr) {
-          mbar_arrive_expect_tx(&bars[warp][st], G::kBytes);
-          bulk_load(ring + st * G::kBytes, source, G::kBytes, &bars[warp][st]);
-        } else {
-          mbar_arrive(&bars[warp][st]);
+    // Tile k of this warp into its stage; one commit group per call, empty behind the last tile.
+    auto issue = [&](int32_t k) {
+      if (k < tiles) {
+        if (k % 32 == 0) locate(k);
+        const uint32_t tile = __shfl_sync(0xffffffffu, source, k % 32);
+        const uint32_t st = static_cast<uint32_t>(k) % G::kStages;
+        if (lane == 0) loaded[warp][st] = tile != kNoTile;
+        if (tile != kNoTile) {
+          const uint8_t* from = a.view.data + static_cast<uint64_t>(tile) * G::kBytes + 16 * lane;
+          uint8_t* to = ring + st * G::kBytes + 16 * lane;
+#pragma unroll
+          for (int c = 0; c < G::kBytes; c += 512)
+            if (c + 512 <= G::kBytes || c + 16 * static_cast<int>(lane) < G::kBytes) copy16(to + c, from + c);
         }
       }
+      commit_copies();
     };
-    for (int32_t k = 0; k < min(tiles, G::kStages - 1); ++k) issue(k);
+    for (int32_t k = 0; k < G::kStages - 1; ++k) issue(k);
 
     // Query fragments: column g of group nt is row rows.first + 8 nt + g.
     uint32_t qf[NT][NG][2][2][QP];
@@ -675,18 +698,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       }
     };
 
-    auto arrived = [&](int32_t k) {
-      const uint32_t at = used + static_cast<uint32_t>(k);
-      return __all_sync(0xffffffffu, mbar_wait(&bars[warp][at % G::kStages], (at / G::kStages) & 1u, a.err, kErrWaitFull));
-    };
     for (int32_t k = 0; k < tiles; ++k) {
-      if (k + G::kStages - 1 < tiles) issue(k + G::kStages - 1);
-      if (!arrived(k)) {  // the copies in flight still land in this ring
-        for (int32_t d = k + 1; d < min(tiles, k + G::kStages); ++d) arrived(d);
-        failed = true;
-        break;
-      }
-      const uint32_t st = (used + k) % G::kStages;
+      issue(k + G::kStages - 1);
+      wait_copies<G::kStages - 1>();  // this lane's share of tile k
+      __syncwarp();                   // and every other lane's
+      const uint32_t st = static_cast<uint32_t>(k) % G::kStages;
       if (loaded[warp][st]) {
         const int32_t key0 = (first_tile + k * kWarps) * static_cast<int32_t>(kKv4Tile);
         const uint8_t* p = ring + st * G::kBytes;
@@ -697,7 +713,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       }
       __syncwarp();  // every lane has read the stage before it is filled again
     }
-    used += static_cast<uint32_t>(tiles);
 
     // ---- this warp's result, then the block's
     float* mine = reinterpret_cast<float*>(ring);  // [8 NT][D]
@@ -731,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
         }
       }
     __syncthreads();
-    const bool whole = take == units;
+    const bool whole = take == size;
     const uint32_t slot = blockIdx.x * 2 + (offset == 0 ? 1u : 0u);
     const float* all = reinterpret_cast<const float*>(smem);
     constexpr int kWarpFloats = G::kStages * G::kBytes / 4;
@@ -771,14 +786,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       }
     }
     if (!whole && offset == 0 && threadIdx.x == 0) {
-      const uint32_t last = static_cast<uint32_t>((unit + units - 1) / share.per);
+      const uint32_t last = static_cast<uint32_t>((unit + size - 1) / share.per);
       a.part_of[blockIdx.x] = make_uint4(1u, pair, head, min(last, gridDim.x - 1));
     }
     unit += take;
     offset = 0;
     if (++head == a.view.kv_heads) head = 0, ++pair;
-    fence_proxy_async_smem();  // the next item's copies overwrite what was written and read here
-    __syncthreads();
+    __syncthreads();  // the next item's copies overwrite what was written and read here
   }
 }
 
@@ -956,7 +970,6 @@ cudaError_t kv4_attention(const Kv4AttnArgs& in, const Kv4Plan& plan, cudaStream
     a.part_of = reinterpret_cast<uint4*>(a.part_o + parts * in.view.dim);
     a.part_ml = reinterpret_cast<float2*>(a.part_of + plan.blocks);
   }
-  a.err = in.err;
   switch (in.type) {
     case kF32: return dispatch_dim<float>(a, plan, stream);
     case kBf16: return dispatch_dim<__nv_bfloat16>(a, plan, stream);

@@ -86,7 +86,6 @@ struct Kv4AttnArgs {
   bool causal = true;
   uint32_t window = 0;
   void* workspace = nullptr;
-  unsigned int* err = nullptr;
 };
 cudaError_t kv4_attention(const Kv4AttnArgs& a, const Kv4Plan& plan, cudaStream_t stream);
 

@@ -74,10 +74,13 @@ class OnDevice {
 // Cache and batch of a call with `tokens` rows.
 int check_cache(const OctB200Kv4Cache* c) {
   if (c == nullptr || c->struct_size < sizeof(OctB200Kv4Cache) || c->data == nullptr || c->pages == 0 ||
-      c->pages > 0x7fffffffu || c->kv_heads == 0 || c->reserved != 0)
+      c->kv_heads == 0 || c->reserved != 0)
     return OCT_B200_DETAIL_INVALID_ARGUMENT;
   if (c->page_size == 0 || c->page_size % oct::kKv4Tile != 0 || c->page_size > 65536u || c->kv_heads > 4096u ||
       !oct::kv4_attention_supported(c->head_dim))
+    return OCT_B200_DETAIL_UNSUPPORTED_SHAPE;
+  // tiles are counted in 32 bits (5 TB of cache)
+  if (static_cast<uint64_t>(c->pages) * c->kv_heads * (c->page_size / oct::kKv4Tile) > 0xfffffff0ull)
     return OCT_B200_DETAIL_UNSUPPORTED_SHAPE;
   return aligned16(c->data) ? 0 : OCT_B200_DETAIL_UNALIGNED;
 }
@@ -346,7 +349,6 @@ int oct_b200_kv4_attention_device(void* handle, const OctB200Kv4Cache* cache, co
     a.causal = r->causal != 0;
     a.window = r->window;
     a.workspace = r->workspace;
-    a.err = rt->err_word();
     if (oct::kv4_attention(a, plan, static_cast<cudaStream_t>(stream)) != cudaSuccess)
       return fail(out_detail_code, OCT_B200_DETAIL_CUDA_ERROR);
     return PROM_OK;

@@ -49,8 +49,8 @@ constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum is renewed only when a score exceeds it by this much (in
-// powers of two): weights stay below 2^8, and most tiles skip the exchange.
-constexpr float kSlack = 8.f;
+// powers of two): weights stay below 2^4, and most tiles skip the exchange.
+constexpr float kSlack = 4.f;
 constexpr uint32_t kNoTile = 0xffffffffu;
 constexpr float kCodeLow = 16777216.f, kCodeHigh = 1048576.f;  // 2^24, 2^20
 
@@ -95,6 +95,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
+// 8 x 8 matrices of 16-bit elements from shared memory, transposed: lanes 8 m .. 8 m + 7 name the rows of matrix m.
+__device__ __forceinline__ void load_transposed(uint32_t& m0, uint32_t& m1, const void* row) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(m0), "=r"(m1) : "r"(smem_addr(row)) : "memory");
+}
+__device__ __forceinline__ void load_transposed(uint32_t& m0, uint32_t& m1, uint32_t& m2, uint32_t& m3, const void* row) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(m0), "=r"(m1), "=r"(m2), "=r"(m3)
+               : "r"(smem_addr(row))
+               : "memory");
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -107,6 +117,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
+  const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float max_half(uint32_t a) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&a);
+  return __half2float(__hmax(__low2half(h), __high2half(h)));
+}
+// both halves of a times the low half of b
+__device__ __forceinline__ uint32_t times_low(uint32_t a, uint32_t b) {
+  const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), __low2half2(*reinterpret_cast<const __half2*>(&b)));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t w) {
@@ -281,7 +304,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   using G = Geometry<D>;
   constexpr int NG = G::kGroups;
   constexpr int kRows = 8 * NT;
+  constexpr int kZeroWords = NG == 8 ? 2 : 1;
   constexpr bool kCentred = std::is_same<T, float>::value;
+  constexpr bool kPacked = PP == 1;  // weight * scale is formed in float16
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t loaded[kWarps][G::kStages];
   __shared__ float2 warp_ml[kWarps][kRows];
@@ -298,6 +323,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   // quarter warp's key loads touch every bank once and the value loads twice.
   const int32_t tok_g = (g & 1) ? 4 + static_cast<int32_t>((g >> 1) ^ 1u) : static_cast<int32_t>(g >> 1);
   const int32_t tok_v[2] = {static_cast<int32_t>(i4), 4 + static_cast<int32_t>(i4 ^ 1u)};  // rows 2 i4, 2 i4 + 1
+
+  const int32_t tok_ld = static_cast<int32_t>((lane & 1) ? 4 + (((lane % 8) >> 1) ^ 1u) : (lane % 8) >> 1) + 8 * static_cast<int32_t>((lane >> 3) & 1);
+  const bool looks = kCentred || (g % 2 == 0 && g < 2 * NG);  // whether its row of the zeros' operand holds scales
 
   unsigned long long unit = share.begin;
   uint32_t pair = share.pair, head = share.head, offset = share.offset;
@@ -354,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
 
     // Query fragments: column g of group nt is row rows.first + 8 nt + g.
     uint32_t qf[NT][NG][2][2][QP];
-    uint32_t qz[NT][2];   // the sums of q over the groups, in two parts: the zeros' operand
+    uint32_t qz[NT][2][kZeroWords];  // the sums of q over the groups, in two parts: the zeros' operand
     float kf[NT][2], zf[NT][2];  // factors of this lane's score columns 2 i4, 2 i4 + 1
     int32_t hi[NT][2];
 #pragma unroll
@@ -392,21 +420,19 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const float nq = pow2_toward(amax, 10), nz = pow2_toward(smax, 10);
-      // zeros: slot k of 16 is group k % NG; the first NG slots hold the high part, the next the low one
-      uint32_t zh = 0, zl = 0;
+      // The zeros' operand: slot 2 j of 16 meets the scale of group j and is zero, slot 2 j + 1 its zero.
+      // Four groups (or two) fill eight slots: the sums' high part there, the low part in the next
+      // eight; eight groups fill all sixteen, and the low part is a second operand.
+      float mine[kZeroWords];
 #pragma unroll
-      for (int j = 0; j < NG; j += 2) {
-        const float x = sums[j] * nz, y = sums[j + 1] * nz;
-        const uint32_t h = pack_half2(x, y);
-        const float2 f = unpack_half2(h);
-        const uint32_t lo = pack_half2(x - f.x, y - f.y);
-        if (static_cast<int>(i4) % (NG / 2) == j / 2) zh = h, zl = lo;
-      }
-      if constexpr (NG == 8) {
-        qz[nt][0] = zh, qz[nt][1] = zl;  // slots 0..7 and 8..15
-      } else {
-        qz[nt][0] = static_cast<int>(i4) < NG / 2 ? zh : (static_cast<int>(i4) < NG ? zl : 0u);
-        qz[nt][1] = 0u;
+      for (int x = 0; x < kZeroWords; ++x) {
+        mine[x] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4 && j < NG; ++j)
+          if (static_cast<int>(i4) == j) mine[x] = sums[4 * x + j] * nz;
+        const uint32_t h = pack_half2(0.f, mine[x]);
+        qz[nt][0][x] = h;
+        qz[nt][1][x] = pack_half2(0.f, mine[x] - unpack_half2(h).y);
       }
       const float kfac = kCodeLow / nq * a.scale_log2, zfac = a.scale_log2 / nz;
 #pragma unroll
@@ -434,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     }
 
     float o[NT][NG][2][4];  // out^T: channels 32 j + 4 g + 2 m2 (+ 1, 16 times as large), columns 2 i4, 2 i4 + 1
-    float oz[NT][4];        // the zeros' share, by group: row g is group g (16-bit results)
+    float oz[NT][4];        // the zeros' share, in the rows of their operand below (16-bit results)
     float zsum[NT][NG][2];  // the same of the zeros + 8 s, of this lane's tokens (fp32 results)
     float l[NT][2], m[NT][2], trigger[NT][2];
 #pragma unroll
@@ -477,12 +503,22 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
         lds(p0, st + G::kKeyParams + tok_g * 4 * NG);
         lds(p1, st + G::kKeyParams + (tok_g + 8) * 4 * NG);
         {
-          uint32_t z0[2], z1[2];  // (s, z) of groups 2 i4 and 2 i4 + 1, modulo the groups
-          lds(z0, st + G::kKeyParams + tok_g * 4 * NG + 8 * (i4 % (NG / 2)));
-          lds(z1, st + G::kKeyParams + (tok_g + 8) * 4 * NG + 8 * (i4 % (NG / 2)));
-          const uint32_t a0 = __byte_perm(z0[0], z0[1], 0x7632u), a1 = __byte_perm(z1[0], z1[1], 0x7632u);
+          uint32_t z0[kZeroWords], z1[kZeroWords];  // (s, z) of group i4 (and 4 + i4)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(zz[nt], a0, a1, a0, a1, qz[nt][0], qz[nt][1]);
+          for (int x = 0; x < kZeroWords; ++x) {
+            const int at = G::kKeyParams + 4 * (static_cast<int>(i4) % NG) + 16 * x;
+            z0[x] = *reinterpret_cast<const uint32_t*>(st + at + tok_g * 4 * NG);
+            z1[x] = *reinterpret_cast<const uint32_t*>(st + at + (tok_g + 8) * 4 * NG);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if constexpr (NG == 8) {
+              mma_f16(zz[nt], z0[0], z1[0], z0[1], z1[1], qz[nt][0][0], qz[nt][0][1]);
+              mma_f16(zz[nt], z0[0], z1[0], z0[1], z1[1], qz[nt][1][0], qz[nt][1][1]);
+            } else {
+              mma_f16(zz[nt], z0[0], z1[0], z0[0], z1[0], qz[nt][0][0], qz[nt][1][0]);
+            }
+          }
         }
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
@@ -586,100 +622,122 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
           if (!keep[1]) p1[j] = 0u;
         }
       }
-      // The zeros: rows of the operand are groups, its columns the tile's tokens.  fp32 results sum them
-      // beside the weights below instead, rounded to nearest.
+      // The zeros' operand (16-bit results): rows 2 j and 2 j + 1 are the scales and zeros of group j
+      // (of group 4 + j from row 8 on), columns the tile's tokens.
+      [[maybe_unused]] uint32_t pa[4] = {0u, 0u, 0u, 0u};
+      float smax = 0.f;  // the largest scale that this lane looks at
       if constexpr (!kCentred) {
-        uint32_t z[4] = {0u, 0u, 0u, 0u};
-        if (static_cast<int>(g) < NG) {
+        if constexpr (NG == 8) {
+          load_transposed(pa[0], pa[2], pa[1], pa[3], st + G::kValueParams + tok_ld * 4 * NG + 16 * (lane / 16));
+        } else if constexpr (NG == 4) {
+          load_transposed(pa[0], pa[2], st + G::kValueParams + tok_ld * 4 * NG);
+        } else if (g < 4) {
+          uint32_t h[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            h[r] = *reinterpret_cast<const uint16_t*>(st + G::kValueParams + (tok_v[r & 1] + 8 * (r >> 1)) * 4 * NG + 2 * g);
+          pa[0] = h[0] | (h[1] << 16), pa[2] = h[2] | (h[3] << 16);
+        }
+        if constexpr (kMasked) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int32_t token = tok_v[r & 1] + 8 * (r >> 1);
-            z[r] = *reinterpret_cast<const uint16_t*>(st + G::kValueParams + token * 4 * NG + 4 * g + 2);
-            if constexpr (kMasked) {
-              // a zero that is no number is seen through its codes' weights, by the rows that see it
-              z[r] = key0 + token >= rows.lo_min && key0 + token <= rows.hi_max ? finite_half(z[r]) : 0u;
-            }
+            // tokens 2 i4 and 2 i4 + 1 (r < 2) of the order above, or 8 further on.  A zero that is no
+            // number reaches, through its codes' weights, the rows that see it
+            const int32_t at = key0 + 8 * (r >> 1);
+            const uint32_t lo = at + tok_v[0] >= rows.lo_min && at + tok_v[0] <= rows.hi_max ? finite_half(pa[r] & 0xffffu) : 0u;
+            const uint32_t hi16 = at + tok_v[1] >= rows.lo_min && at + tok_v[1] <= rows.hi_max ? finite_half(pa[r] >> 16) : 0u;
+            pa[r] = lo | (hi16 << 16);
           }
         }
-        const uint32_t a0 = z[0] | (z[1] << 16), a2 = z[2] | (z[3] << 16);
+        smax = max_half(max_half2(max_half2(pa[0], pa[2]), max_half2(pa[1], pa[3])));
+      } else {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const uint32_t h0 = pack_half2(w[nt][0], w[nt][1]), h1 = pack_half2(w[nt][2], w[nt][3]);
-          mma_f16(oz[nt], a0, 0u, a2, 0u, transpose8x8(h0), transpose8x8(h1));
-          if constexpr (PP == 2) {
-            const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
-            mma_f16(oz[nt], a0, 0u, a2, 0u, transpose8x8(pack_half2(w[nt][0] - f0.x, w[nt][1] - f0.y)),
-                    transpose8x8(pack_half2(w[nt][2] - f1.x, w[nt][3] - f1.y)));
-          }
-        }
+        for (int j = 0; j < NG; ++j) smax = max3(smax, unpack_half2(p0[j]).x, unpack_half2(p1[j]).x);
       }
-      if constexpr (kCentred) {
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
-          const float z0 = fmaf(8.f, f0.x, f0.y), z1 = fmaf(8.f, f1.x, f1.y);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              zsum[nt][j][c] = vis[nt][c] ? fmaf(w[nt][c], z0, zsum[nt][j][c]) : zsum[nt][j][c];
-              zsum[nt][j][c] = vis[nt][2 + c] ? fmaf(w[nt][2 + c], z1, zsum[nt][j][c]) : zsum[nt][j][c];
-            }
-        }
-      }
-      float smax = 0.f;
-#pragma unroll
-      for (int j = 0; j < NG; ++j) smax = max3(smax, unpack_half2(p0[j]).x, unpack_half2(p1[j]).x);
-      if (__any_sync(0xffffffffu, smax > pm_limit)) {
+      if (__any_sync(0xffffffffu, smax > (looks ? pm_limit : INFINITY))) {
+        if (!looks) smax = 0.f;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
         // a largest scale of zero sets no measure for those to come
-        const float next = pow2_toward(smax, 5);
+        const float next = kPacked ? fminf(pow2_toward(smax, 9), 2048.f) : pow2_toward(smax, 9);
         const float ratio = pm_limit < 0.f ? 0.f : next / pm;
         pm = next;
-        pm_limit = smax > 0.f ? 128.f / next : 0.f;
+        pm_limit = smax > 0.f ? 2048.f / next : 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int j = 0; j < NG; ++j)
 #pragma unroll
             for (int m2 = 0; m2 < 2; ++m2)
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[nt][j][m2][e] *= ratio;
+          if constexpr (kPacked) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) oz[nt][e] *= ratio;
+          }
+        }
       }
+      [[maybe_unused]] uint32_t wh[NT][2];  // kPacked: w * pm
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (kCentred) {  // zeros + 8 s, summed beside the weights and rounded to nearest
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[nt][e] *= pm;
+          for (int j = 0; j < NG; ++j) {
+            const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
+            const float z0 = fmaf(8.f, f0.x, f0.y), z1 = fmaf(8.f, f1.x, f1.y);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              zsum[nt][j][c] = vis[nt][c] ? fmaf(w[nt][c], z0, zsum[nt][j][c]) : zsum[nt][j][c];
+              zsum[nt][j][c] = vis[nt][2 + c] ? fmaf(w[nt][2 + c], z1, zsum[nt][j][c]) : zsum[nt][j][c];
+            }
+          }
+        }
+        if constexpr (kPacked) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) wh[nt][r] = pack_half2(w[nt][2 * r] * pm, w[nt][2 * r + 1] * pm);
+          mma_f16(oz[nt], pa[0], pa[1], pa[2], pa[3], transpose8x8(wh[nt][0]), transpose8x8(wh[nt][1]));
+        } else {
+          if constexpr (!kCentred) {
+            const uint32_t h0 = pack_half2(w[nt][0], w[nt][1]), h1 = pack_half2(w[nt][2], w[nt][3]);
+            mma_f16(oz[nt], pa[0], pa[1], pa[2], pa[3], transpose8x8(h0), transpose8x8(h1));
+            const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
+            mma_f16(oz[nt], pa[0], pa[1], pa[2], pa[3], transpose8x8(pack_half2(w[nt][0] - f0.x, w[nt][1] - f0.y)),
+                    transpose8x8(pack_half2(w[nt][2] - f1.x, w[nt][3] - f1.y)));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[nt][e] *= pm;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
         uint32_t x01 = __byte_perm(vw[0][j / 2], vw[1][j / 2], sel);
         uint32_t x23 = __byte_perm(vw[2][j / 2], vw[3][j / 2], sel);
-        const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
         uint32_t bf[NT][2][PP];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float u[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = e < 2 ? f0 : f1;
-            u[e] = w[nt][e] * f.x;
-            if constexpr (kMasked) {
-              if (!vis[nt][e]) u[e] = 0.f;
-              else if (!kCentred && !(fabsf(f.y) < INFINITY)) u[e] = NAN;
-            }
-          }
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint32_t h = pack_half2(u[2 * r], u[2 * r + 1]);
-            bf[nt][r][0] = transpose8x8(h);
-            if constexpr (PP == 2) {
-              const float2 f = unpack_half2(h);
-              bf[nt][r][1] = transpose8x8(pack_half2(u[2 * r] - f.x, u[2 * r + 1] - f.y));
+            const uint32_t sz = r == 0 ? p0[j] : p1[j];
+            uint32_t h, rest = 0u;
+            if constexpr (kPacked) {
+              h = times_low(wh[nt][r], sz);
+            } else {
+              const float f = unpack_half2(sz).x;
+              const float u = w[nt][2 * r] * f, v = w[nt][2 * r + 1] * f;
+              h = pack_half2(u, v);
+              const float2 x = unpack_half2(h);
+              rest = pack_half2(u - x.x, v - x.y);
             }
+            if constexpr (kMasked) {
+              const bool number = kCentred || ((sz >> 16) & 0x7c00u) != 0x7c00u;
+              if (!number) rest = 0u, h = 0x7fff7fffu;
+              h &= (vis[nt][2 * r] ? 0xffffu : 0u) | (vis[nt][2 * r + 1] ? 0xffff0000u : 0u);
+              rest &= (vis[nt][2 * r] ? 0xffffu : 0u) | (vis[nt][2 * r + 1] ? 0xffff0000u : 0u);
+            }
+            bf[nt][r][0] = transpose8x8(h);
+            if constexpr (PP == 2) bf[nt][r][1] = transpose8x8(rest);
           }
-        }
 #pragma unroll
         for (int m2 = 0; m2 < 2; ++m2) {
           uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
@@ -731,13 +789,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
         if (g == 0) warp_ml[warp][col] = make_float2(none ? -INFINITY : m[nt][c], l[nt][c]);
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          float z;
+          float z;  // 16-bit results: from the rows of the zeros' accumulators
           if constexpr (kCentred) {
             z = zsum[nt][j][c];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
           } else {
-            z = __shfl_sync(0xffffffffu, oz[nt][c], 4 * j + i4);
+            z = __shfl_sync(0xffffffffu, oz[nt][j < 4 ? c : 2 + c], 4 * (2 * (j % 4) + 1) + i4);
+            if constexpr (kPacked) z *= unit_f;
           }
           float2* to = reinterpret_cast<float2*>(mine + col * D + 32 * j + 4 * g);
 #pragma unroll

@@ -114,14 +114,16 @@ class Cache:
 def attention(cache: Cache, table_row, length: int, q: np.ndarray, scale: float, causal=True, window=0) -> tuple:
     """q [n][heads][dim] of one sequence that holds `length` tokens, the n of q the last of them.
     -> out [n][heads][dim], lse [n][heads], weight [n][heads][dim] (the mean of |z| + 15 s of the
-    values under the softmax) and reach [n][heads] (the largest scale * sum |q| (|z| + 15 s) of the keys)."""
+    values under the softmax), reach [n][heads] (the largest scale * sum |q| (|z| + 15 s) of the keys)
+    and the largest |z| + 15 s of a value."""
     n, heads, dim = q.shape
     share = heads // cache.kv_heads
     out, weight = np.zeros(q.shape), np.zeros(q.shape)
-    lse, reach = np.full((n, heads), -np.inf), np.zeros((n, heads))
+    lse, reach, largest = np.full((n, heads), -np.inf), np.zeros((n, heads)), 0.0
     for kvh in range(cache.kv_heads):
         k, ks = cache.rows(table_row, 0, length, kvh, 0)
         v, vs = cache.rows(table_row, 0, length, kvh, 1)
+        largest = max(largest, np.nanmax(vs, initial=0.0))
         for t in range(n):
             last = length - n + t if causal else length - 1
             first = max(0, last - window + 1) if window else 0
@@ -136,4 +138,4 @@ def attention(cache: Cache, table_row, length: int, q: np.ndarray, scale: float,
                 out[t, h], lse[t, h] = e @ v[sl] / total, top + np.log(total)
                 weight[t, h] = e @ vs[sl] / total
                 reach[t, h] = (ks[sl] @ np.abs(q[t, h])).max() * abs(scale)
-    return out, lse, weight, reach
+    return out, lse, weight, reach, largest

@@ -9,9 +9,12 @@ Tolerances, derived from the arithmetic (u = half a step of the output type):
 * attention: with M the largest scale * sum |q| (|z| + 15 s) of a key and W the mean of
   |z| + 15 s of a channel's values under the softmax, scores are off by at most
   d = 2^-20 M (fp32 sums of D / 16 tensor products and 2 D / 32 scaled parts, q in 22 bits or
-  exact) + 2^-21 (the exponent), weights by 2 d + 2^-21, the float16 weight * scale by 2^-12
-  for bf16 (one part; 2^-21 in two parts otherwise), fp32 sums over n keys by
-  (n / 16 + 48) 2^-24, all relative to W; then one rounding.
+  exact) + 2^-21 (the exponent), weights by 2 d + 2^-21, the float16 weights by 2^-12 for bf16
+  and their products with the scales by 2^-12 more (2^-21 in two parts for the other types),
+  fp32 sums over n keys by (n / 16 + 48) 2^-24, all relative to W.  Weights and products below
+  float16's normal numbers are off by 2^-25 of a unit that is at least 2^-8 of the largest scale
+  s: n keys, each 2^-33 s of the largest |z| + 15 s (s at most a fifteenth of that).  Then one
+  rounding.
 """
 from __future__ import annotations
 
@@ -385,13 +388,13 @@ def _check_attention(host, kind, q, out, lse, *, window=0, causal=True, scale=No
         sl = slice(int(host.starts[b]), int(host.starts[b + 1]))
         if sl.start == sl.stop:
             continue
-        want, want_lse, weight, reach = O.attention(host.cache, host.table[b], host.held[b], qn[sl], scale, causal, window)
+        want, want_lse, weight, reach, largest = O.attention(host.cache, host.table[b], host.held[b], qn[sl], scale, causal, window)
         n = host.held[b]
         d = 2.0 ** -20 * reach + 2.0 ** -21
-        rel = 2 * d + 2.0 ** -21 + (2.0 ** -12 if kind == "bf16" else 2.0 ** -21) + (n / 16 + 48) * 2.0 ** -24
+        rel = 2 * d + 2.0 ** -21 + (2.0 ** -11 if kind == "bf16" else 2.0 ** -21) + (n / 16 + 48) * 2.0 ** -24
         nan = np.isnan(want)
         assert np.array_equal(np.isnan(got[sl]), nan), b
-        tiny = 2.0 ** -25 if kind == "f16" else 0.0
+        tiny = (2.0 ** -25 if kind == "f16" else 0.0) + n * 2.0 ** -33 * largest ** 2 / 15
         _near(np.where(nan, 0, got[sl]), np.where(nan, 0, want),
               np.where(nan, 0, u * np.abs(want) * 1.01 + rel[..., None] * weight + tiny), f"sequence {b}")
         nan = np.isnan(want_lse)

@@ -52,6 +52,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 // powers of two): weights stay below 2^4, and most tiles skip the exchange.
 constexpr float kSlack = 4.f;
 constexpr uint32_t kNoTile = 0xffffffffu;
+constexpr int32_t kNowhere = 0x7fffffff - 64;  // no sequence is that long
 constexpr float kCodeLow = 16777216.f, kCodeHigh = 1048576.f;  // 2^24, 2^20
 
 template <int D>
@@ -62,16 +63,16 @@ struct Geometry {
   static constexpr int kValues = kKeyParams + 16 * kGroups * 4;
   static constexpr int kValueParams = kValues + 16 * kRowBytes;
   static constexpr int kBytes = 2 * kValues;
-  // ring of tiles per warp: about 10 to 20 KB, and room for the warp's result at the end
-  static constexpr int kStages = D == 64 ? 8 : 4;
+  // ring of tiles per warp: 10 to 20 KB, and room for the warp's result at the end
+  static constexpr int kStages = D == 64 ? 8 : (D == 128 ? 6 : 4);
 };
 
 // Query rows of one block in groups of 8, by what the accumulators leave of the registers.
-// Blocks per SM that the compiler leaves registers for, and that a launch fills: latencies here are
-// hidden by warps, accumulators and query fragments grow with the channels and the row groups.
-constexpr int blocks_per_sm(int dim, int row_groups, int query_parts) {
-  return row_groups == 1 && dim <= 128 ? (query_parts == 1 || dim == 64 ? 4 : 3) : (dim * row_groups <= 128 ? 3 : 2);
-}
+// Tiles that a warp works through at a time: with two, one vote on the maximum and one on the scales
+// serve 32 keys and their operands' latencies overlap.
+constexpr int tiles_per_step(int dim, int row_groups) { return dim * row_groups <= 128 ? 2 : 1; }
+// Blocks per SM that the compiler leaves registers for, and that a launch fills.
+constexpr int blocks_per_sm(int dim, int row_groups, int query_parts) { return dim * row_groups <= 128 ? 3 : 2; }
 template <int D> constexpr int kMaxRowGroups = D == 64 ? 4 : (D == 128 ? 2 : 1);
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -214,11 +215,11 @@ __device__ __forceinline__ bool row_range(const KernelArgs& a, const Kv4Seq& s, 
   return true;
 }
 
-// An item is one (sequence, row tile, key head); its units are runs of kWarps
-// tiles, at least one so that a row without keys is written too.  Items stand
+// An item is one (sequence, row tile, key head); its units are runs of one
+// step's tiles for every warp, at least one so that a row without keys is written too.  Items stand
 // in that order, and every block takes an equal run of all the call's units.
-__device__ __forceinline__ uint32_t item_units(const Rows& r) {
-  return static_cast<uint32_t>(max(1, (r.t_end - r.t_begin + kWarps - 1) / kWarps));
+__device__ __forceinline__ uint32_t item_units(const Rows& r, int32_t unit_tiles) {
+  return static_cast<uint32_t>(max(1, (r.t_end - r.t_begin + unit_tiles - 1) / unit_tiles));
 }
 __device__ __forceinline__ bool item_rows(const KernelArgs& a, uint32_t pair, uint32_t rows_per_tile, Kv4Seq* s,
                                           Rows* r) {
@@ -235,7 +236,7 @@ struct Share {
   uint32_t pair, head, offset;         // where it begins
 };
 // Called by the whole block.
-__device__ __forceinline__ bool find_share(const KernelArgs& a, uint32_t rows_per_tile, Share* out) {
+__device__ __forceinline__ bool find_share(const KernelArgs& a, uint32_t rows_per_tile, int32_t unit_tiles, Share* out) {
   __shared__ unsigned long long warp_sums[2][kWarps];
   __shared__ uint32_t found[3];
   const uint32_t pairs = a.view.batch * a.row_tiles, chunk = (pairs + kThreads - 1) / kThreads;
@@ -244,7 +245,7 @@ __device__ __forceinline__ bool find_share(const KernelArgs& a, uint32_t rows_pe
   Kv4Seq s;
   Rows r;
   for (uint32_t p = p0; p < p1; ++p)
-    if (item_rows(a, p, rows_per_tile, &s, &r)) sums[0] += item_units(r), ++sums[1];
+    if (item_rows(a, p, rows_per_tile, &s, &r)) sums[0] += item_units(r, unit_tiles), ++sums[1];
   unsigned long long upto[2];
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
@@ -278,7 +279,7 @@ __device__ __forceinline__ bool find_share(const KernelArgs& a, uint32_t rows_pe
   if (out->begin >= at && out->begin < last)
     for (uint32_t p = p0; p < p1; ++p)
       if (item_rows(a, p, rows_per_tile, &s, &r)) {
-        const uint32_t size = item_units(r) + out->cost;
+        const uint32_t size = item_units(r, unit_tiles) + out->cost;
         const unsigned long long heads = static_cast<unsigned long long>(size) * a.view.kv_heads;
         if (out->begin < at + heads) {
           const uint32_t rest = static_cast<uint32_t>(out->begin - at);
@@ -305,15 +306,17 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   constexpr int NG = G::kGroups;
   constexpr int kRows = 8 * NT;
   constexpr int kZeroWords = NG == 8 ? 2 : 1;
+  constexpr int H = tiles_per_step(D, NT), kUnit = kWarps * H;
+  constexpr int kStages = G::kStages / H, kStageBytes = H * G::kBytes;
   constexpr bool kCentred = std::is_same<T, float>::value;
   constexpr bool kPacked = PP == 1;  // weight * scale is formed in float16
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t loaded[kWarps][G::kStages];
+  __shared__ uint32_t loaded[kWarps][kStages];
   __shared__ float2 warp_ml[kWarps][kRows];
 
   griddep_launch_dependents();
   Share share;
-  const bool any = find_share(a, kRows, &share);
+  const bool any = find_share(a, kRows, kUnit, &share);
   if (threadIdx.x == 0 && a.part_of != nullptr) a.part_of[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
   if (!any) return;
 
@@ -337,48 +340,55 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       ++pair;
       continue;
     }
-    const uint32_t size = item_units(rows) + share.cost;
+    const uint32_t size = item_units(rows, kUnit) + share.cost;
     const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(size - offset), share.end - unit));
     // the item's cost comes first in its run; the units behind it are its tiles
     const uint32_t unit0 = max(offset, share.cost) - share.cost, unit1 = max(offset + take, share.cost) - share.cost;
-    const int32_t t0 = rows.t_begin + static_cast<int32_t>(unit0 * kWarps);
-    const int32_t t1 = min(rows.t_end, rows.t_begin + static_cast<int32_t>(unit1 * kWarps));
-    const int32_t first_tile = t0 + static_cast<int32_t>(warp);
-    const int32_t tiles = first_tile < t1 ? (t1 - first_tile + kWarps - 1) / kWarps : 0;
+    const int32_t t0 = rows.t_begin + static_cast<int32_t>(unit0 * kUnit);
+    const int32_t t1 = min(rows.t_end, rows.t_begin + static_cast<int32_t>(unit1 * kUnit));
+    const int32_t first_tile = t0 + static_cast<int32_t>(warp) * H;  // of step 0; each step is kUnit further
+    const int32_t steps = first_tile < t1 ? (t1 - first_tile + kUnit - 1) / kUnit : 0;
 
-    // Which of the cache's tiles this warp's next 32 are, one per lane (kNoTile: no page of the cache).
+    // Which of the cache's tiles this warp's next 32 steps take, one step per lane (kNoTile: no page
+    // of the cache, or behind the last key).
     const int32_t* table = a.view.table + pair / a.row_tiles * a.view.table_stride;
-    uint32_t source = kNoTile;
+    uint32_t source[H];
     auto locate = [&](int32_t k0) {
-      const int32_t k = k0 + static_cast<int32_t>(lane);
-      source = kNoTile;
-      if (k >= tiles) return;
-      const uint32_t t = static_cast<uint32_t>(first_tile + k * kWarps);
-      const uint32_t in_table = t / a.view.page_tiles;
-      const uint32_t page = static_cast<uint32_t>(table[in_table]);
-      if (page < a.view.pages)
-        source = (page * a.view.kv_heads + head) * a.view.page_tiles + t - in_table * a.view.page_tiles;
-      else
-        atomicOr(a.view.bad, 1u);
+      const int32_t t = first_tile + (k0 + static_cast<int32_t>(lane)) * kUnit;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        source[h] = kNoTile;
+        if (t + h >= t1) continue;
+        const uint32_t in_table = static_cast<uint32_t>(t + h) / a.view.page_tiles;
+        const uint32_t page = static_cast<uint32_t>(table[in_table]);
+        if (page < a.view.pages)
+          source[h] = (page * a.view.kv_heads + head) * a.view.page_tiles + (t + h) - in_table * a.view.page_tiles;
+        else
+          atomicOr(a.view.bad, 1u);
+      }
     };
-    // Tile k of this warp into its stage; one commit group per call, empty behind the last tile.
+    // The tiles of step k into its stage; one commit group per call, empty behind the last step.
     auto issue = [&](int32_t k) {
-      if (k < tiles) {
+      if (k < steps) {
         if (k % 32 == 0) locate(k);
-        const uint32_t tile = __shfl_sync(0xffffffffu, source, k % 32);
-        const uint32_t st = static_cast<uint32_t>(k) % G::kStages;
-        if (lane == 0) loaded[warp][st] = tile != kNoTile;
-        if (tile != kNoTile) {
+        const uint32_t st = static_cast<uint32_t>(k) % kStages;
+        uint32_t there = 0;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const uint32_t tile = __shfl_sync(0xffffffffu, source[h], k % 32);
+          if (tile == kNoTile) continue;
+          there |= 1u << h;
           const uint8_t* from = a.view.data + static_cast<uint64_t>(tile) * G::kBytes + 16 * lane;
-          uint8_t* to = ring + st * G::kBytes + 16 * lane;
+          uint8_t* to = ring + st * kStageBytes + h * G::kBytes + 16 * lane;
 #pragma unroll
           for (int c = 0; c < G::kBytes; c += 512)
             if (c + 512 <= G::kBytes || c + 16 * static_cast<int>(lane) < G::kBytes) copy16(to + c, from + c);
         }
+        if (lane == 0) loaded[warp][st] = there;
       }
       commit_copies();
     };
-    for (int32_t k = 0; k < G::kStages - 1; ++k) issue(k);
+    for (int32_t k = 0; k < kStages - 1; ++k) issue(k);
 
     // Query fragments: column g of group nt is row rows.first + 8 nt + g.
     uint32_t qf[NT][NG][2][2][QP];
@@ -482,42 +492,48 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     }
     float pm = 0.f, pm_limit = -1.f;  // weights enter as w * s * pm; s <= pm_limit keeps that in float16
 
-    auto tile_step = [&](const uint8_t* st, int32_t key0, auto masked_tag) {
+    // One step: H tiles (key0: position of the first token; there: which of them are in the stage).
+    auto step = [&](const uint8_t* stage, int32_t key0, uint32_t there, auto masked_tag) {
       constexpr bool kMasked = decltype(masked_tag)::value;
-      const int32_t pos[2] = {key0 + tok_g, key0 + tok_g + 8};
-      bool keep[2] = {true, true};  // tokens that some row sees: what lies outside may be any bits
-      if constexpr (kMasked) {
-        keep[0] = pos[0] >= rows.lo_min && pos[0] <= rows.hi_max;
-        keep[1] = pos[1] >= rows.lo_min && pos[1] <= rows.hi_max;
+      int32_t at[H];            // position of a tile's first token; behind every key when it is not there
+      bool keep[H][2];          // tokens that some row sees: what lies outside may be any bits
+      bool vis[H][NT][4];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        at[h] = kMasked && !((there >> h) & 1u) ? kNowhere : key0 + 16 * h;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          keep[h][r] = !kMasked || (at[h] + tok_g + 8 * r >= rows.lo_min && at[h] + tok_g + 8 * r <= rows.hi_max);
       }
       // ---- scores
-      float raw[NT][4], zz[NT][4];
+      float raw[H][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int h = 0; h < H; ++h) {
+        const uint8_t* st = stage + h * G::kBytes;
+        float zz[NT][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) raw[nt][e] = zz[nt][e] = 0.f;
-      {
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) raw[h][nt][e] = zz[nt][e] = 0.f;
         uint32_t w0[NG], w1[NG], p0[NG], p1[NG];
         lds(w0, st + tok_g * G::kRowBytes + i4 * 4 * NG);
         lds(w1, st + (tok_g + 8) * G::kRowBytes + i4 * 4 * NG);
         lds(p0, st + G::kKeyParams + tok_g * 4 * NG);
         lds(p1, st + G::kKeyParams + (tok_g + 8) * 4 * NG);
-        {
-          uint32_t z0[kZeroWords], z1[kZeroWords];  // (s, z) of group i4 (and 4 + i4)
+        uint32_t z0[kZeroWords], z1[kZeroWords];  // (s, z) of group i4 (and 4 + i4)
 #pragma unroll
-          for (int x = 0; x < kZeroWords; ++x) {
-            const int at = G::kKeyParams + 4 * (static_cast<int>(i4) % NG) + 16 * x;
-            z0[x] = *reinterpret_cast<const uint32_t*>(st + at + tok_g * 4 * NG);
-            z1[x] = *reinterpret_cast<const uint32_t*>(st + at + (tok_g + 8) * 4 * NG);
-          }
+        for (int x = 0; x < kZeroWords; ++x) {
+          const int to = G::kKeyParams + 4 * (static_cast<int>(i4) % NG) + 16 * x;
+          z0[x] = *reinterpret_cast<const uint32_t*>(st + to + tok_g * 4 * NG);
+          z1[x] = *reinterpret_cast<const uint32_t*>(st + to + (tok_g + 8) * 4 * NG);
+        }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if constexpr (NG == 8) {
-              mma_f16(zz[nt], z0[0], z1[0], z0[1], z1[1], qz[nt][0][0], qz[nt][0][1]);
-              mma_f16(zz[nt], z0[0], z1[0], z0[1], z1[1], qz[nt][1][0], qz[nt][1][1]);
-            } else {
-              mma_f16(zz[nt], z0[0], z1[0], z0[0], z1[0], qz[nt][0][0], qz[nt][1][0]);
-            }
+        for (int nt = 0; nt < NT; ++nt) {
+          if constexpr (NG == 8) {
+            mma_f16(zz[nt], z0[0], z1[0], z0[1], z1[1], qz[nt][0][0], qz[nt][0][1]);
+            mma_f16(zz[nt], z0[0], z1[0], z0[1], z1[1], qz[nt][1][0], qz[nt][1][1]);
+          } else {
+            mma_f16(zz[nt], z0[0], z1[0], z0[0], z1[0], qz[nt][0][0], qz[nt][1][0]);
           }
         }
 #pragma unroll
@@ -547,35 +563,41 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              raw[nt][c] = fmaf(s0, acc[nt][c], raw[nt][c]);
-              raw[nt][2 + c] = fmaf(s1, acc[nt][2 + c], raw[nt][2 + c]);
+              raw[h][nt][c] = fmaf(s0, acc[nt][c], raw[h][nt][c]);
+              raw[h][nt][2 + c] = fmaf(s1, acc[nt][2 + c], raw[h][nt][2 + c]);
             }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = e & 1;
+            float x = fmaf(raw[h][nt][e], kf[nt][c], zz[nt][e] * zf[nt][c]);
+            vis[h][nt][e] = true;
+            if constexpr (kMasked) {
+              const int32_t pos = at[h] + tok_g + 8 * (e >> 1);
+              vis[h][nt][e] = pos <= hi[nt][c] && pos >= row_lo(a, hi[nt][c]);
+              if (!vis[h][nt][e]) x = -INFINITY;
+            }
+            raw[h][nt][e] = x;
+          }
       }
-      bool vis[NT][4];
       bool renew = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float s = fmaf(raw[nt][2 * r + c], kf[nt][c], zz[nt][2 * r + c] * zf[nt][c]);
-            vis[nt][2 * r + c] = true;
-            if constexpr (kMasked) {
-              vis[nt][2 * r + c] = pos[r] <= hi[nt][c] && pos[r] >= row_lo(a, hi[nt][c]);
-              if (!vis[nt][2 * r + c]) s = -INFINITY;
-            }
-            raw[nt][2 * r + c] = s;
-          }
-          renew |= fmaxf(raw[nt][c], raw[nt][2 + c]) > trigger[nt][c];
+          float top = fmaxf(raw[0][nt][c], raw[0][nt][2 + c]);
+          if constexpr (H == 2) top = max3(top, raw[H - 1][nt][c], raw[H - 1][nt][2 + c]);
+          renew |= top > trigger[nt][c];
         }
       if (__any_sync(0xffffffffu, renew)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(raw[nt][c], raw[nt][2 + c]);
+            float top = fmaxf(raw[0][nt][c], raw[0][nt][2 + c]);
+            if constexpr (H == 2) top = max3(top, raw[H - 1][nt][c], raw[H - 1][nt][2 + c]);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -599,60 +621,58 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
             }
           }
       }
-      // ---- weights
-      float w[NT][4];
+      // ---- weights, in place of the scores
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          w[nt][c] = exp2_approx(raw[nt][c] - m[nt][c]);
-          w[nt][2 + c] = exp2_approx(raw[nt][2 + c] - m[nt][c]);
-          l[nt][c] += w[nt][c] + w[nt][2 + c];
-        }
-      // ---- values
-      uint32_t vw[4][NG / 2], p0[NG], p1[NG];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) lds(vw[r], st + G::kValues + (tok_v[r & 1] + 8 * (r >> 1)) * G::kRowBytes + g * 2 * NG);
-      lds(p0, st + G::kValueParams + tok_g * 4 * NG);
-      lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
-      if constexpr (kMasked) {
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          if (!keep[0]) p0[j] = 0u;
-          if (!keep[1]) p1[j] = 0u;
-        }
-      }
-      // The zeros' operand (16-bit results): rows 2 j and 2 j + 1 are the scales and zeros of group j
-      // (of group 4 + j from row 8 on), columns the tile's tokens.
-      [[maybe_unused]] uint32_t pa[4] = {0u, 0u, 0u, 0u};
-      float smax = 0.f;  // the largest scale that this lane looks at
-      if constexpr (!kCentred) {
-        if constexpr (NG == 8) {
-          load_transposed(pa[0], pa[2], pa[1], pa[3], st + G::kValueParams + tok_ld * 4 * NG + 16 * (lane / 16));
-        } else if constexpr (NG == 4) {
-          load_transposed(pa[0], pa[2], st + G::kValueParams + tok_ld * 4 * NG);
-        } else if (g < 4) {
-          uint32_t h[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            h[r] = *reinterpret_cast<const uint16_t*>(st + G::kValueParams + (tok_v[r & 1] + 8 * (r >> 1)) * 4 * NG + 2 * g);
-          pa[0] = h[0] | (h[1] << 16), pa[2] = h[2] | (h[3] << 16);
-        }
-        if constexpr (kMasked) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            // tokens 2 i4 and 2 i4 + 1 (r < 2) of the order above, or 8 further on.  A zero that is no
-            // number reaches, through its codes' weights, the rows that see it
-            const int32_t at = key0 + 8 * (r >> 1);
-            const uint32_t lo = at + tok_v[0] >= rows.lo_min && at + tok_v[0] <= rows.hi_max ? finite_half(pa[r] & 0xffffu) : 0u;
-            const uint32_t hi16 = at + tok_v[1] >= rows.lo_min && at + tok_v[1] <= rows.hi_max ? finite_half(pa[r] >> 16) : 0u;
-            pa[r] = lo | (hi16 << 16);
+          for (int e = 0; e < 4; ++e) {
+            raw[h][nt][e] = exp2_approx(raw[h][nt][e] - m[nt][e & 1]);
+            l[nt][e & 1] += raw[h][nt][e];
           }
-        }
-        smax = max_half(max_half2(max_half2(pa[0], pa[2]), max_half2(pa[1], pa[3])));
-      } else {
+      // ---- values.  The zeros' operand (16-bit results): rows 2 j and 2 j + 1 are the scales and zeros
+      // of group j (of group 4 + j from row 8 on), columns a tile's tokens.
+      [[maybe_unused]] uint32_t pa[H][4];
+      float smax = 0.f;  // the largest scale that this lane looks at
 #pragma unroll
-        for (int j = 0; j < NG; ++j) smax = max3(smax, unpack_half2(p0[j]).x, unpack_half2(p1[j]).x);
+      for (int h = 0; h < H; ++h) {
+        const uint8_t* st = stage + h * G::kBytes;
+        if constexpr (!kCentred) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) pa[h][r] = 0u;
+          if constexpr (NG == 8) {
+            load_transposed(pa[h][0], pa[h][2], pa[h][1], pa[h][3],
+                            st + G::kValueParams + tok_ld * 4 * NG + 16 * (lane / 16));
+          } else if constexpr (NG == 4) {
+            load_transposed(pa[h][0], pa[h][2], st + G::kValueParams + tok_ld * 4 * NG);
+          } else if (g < 4) {
+            uint32_t x[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              x[r] = *reinterpret_cast<const uint16_t*>(st + G::kValueParams + (tok_v[r & 1] + 8 * (r >> 1)) * 4 * NG + 2 * g);
+            pa[h][0] = x[0] | (x[1] << 16), pa[h][2] = x[2] | (x[3] << 16);
+          }
+          if constexpr (kMasked) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              // rows 2 i4 and 2 i4 + 1 (r < 2) of the order above, or 8 further on.  A zero that is no
+              // number reaches, through its codes' weights, the rows that see it
+              const int32_t x = at[h] + 8 * (r >> 1) + tok_v[0], y = at[h] + 8 * (r >> 1) + tok_v[1];
+              const uint32_t lo = x >= rows.lo_min && x <= rows.hi_max ? finite_half(pa[h][r] & 0xffffu) : 0u;
+              const uint32_t up = y >= rows.lo_min && y <= rows.hi_max ? finite_half(pa[h][r] >> 16) : 0u;
+              pa[h][r] = lo | (up << 16);
+            }
+          }
+          smax = fmaxf(smax, max_half(max_half2(max_half2(pa[h][0], pa[h][2]), max_half2(pa[h][1], pa[h][3]))));
+        } else {
+          uint32_t p0[NG], p1[NG];
+          lds(p0, st + G::kValueParams + tok_g * 4 * NG);
+          lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+            smax = max3(smax, keep[h][0] ? unpack_half2(p0[j]).x : 0.f, keep[h][1] ? unpack_half2(p1[j]).x : 0.f);
+        }
       }
       if (__any_sync(0xffffffffu, smax > (looks ? pm_limit : INFINITY))) {
         if (!looks) smax = 0.f;
@@ -677,97 +697,118 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
           }
         }
       }
-      [[maybe_unused]] uint32_t wh[NT][2];  // kPacked: w * pm
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if constexpr (kCentred) {  // zeros + 8 s, summed beside the weights and rounded to nearest
+      for (int h = 0; h < H; ++h) {
+        const uint8_t* st = stage + h * G::kBytes;
+        uint32_t vw[4][NG / 2], p0[NG], p1[NG];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          lds(vw[r], st + G::kValues + (tok_v[r & 1] + 8 * (r >> 1)) * G::kRowBytes + g * 2 * NG);
+        lds(p0, st + G::kValueParams + tok_g * 4 * NG);
+        lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
+        if constexpr (kMasked) {
 #pragma unroll
           for (int j = 0; j < NG; ++j) {
-            const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
-            const float z0 = fmaf(8.f, f0.x, f0.y), z1 = fmaf(8.f, f1.x, f1.y);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              zsum[nt][j][c] = vis[nt][c] ? fmaf(w[nt][c], z0, zsum[nt][j][c]) : zsum[nt][j][c];
-              zsum[nt][j][c] = vis[nt][2 + c] ? fmaf(w[nt][2 + c], z1, zsum[nt][j][c]) : zsum[nt][j][c];
-            }
+            if (!keep[h][0]) p0[j] = 0u;
+            if (!keep[h][1]) p1[j] = 0u;
           }
         }
-        if constexpr (kPacked) {
+        [[maybe_unused]] uint32_t wh[NT][2];  // kPacked: w * pm
+        float(&w)[NT][4] = raw[h];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) wh[nt][r] = pack_half2(w[nt][2 * r] * pm, w[nt][2 * r + 1] * pm);
-          mma_f16(oz[nt], pa[0], pa[1], pa[2], pa[3], transpose8x8(wh[nt][0]), transpose8x8(wh[nt][1]));
-        } else {
-          if constexpr (!kCentred) {
-            const uint32_t h0 = pack_half2(w[nt][0], w[nt][1]), h1 = pack_half2(w[nt][2], w[nt][3]);
-            mma_f16(oz[nt], pa[0], pa[1], pa[2], pa[3], transpose8x8(h0), transpose8x8(h1));
-            const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
-            mma_f16(oz[nt], pa[0], pa[1], pa[2], pa[3], transpose8x8(pack_half2(w[nt][0] - f0.x, w[nt][1] - f0.y)),
-                    transpose8x8(pack_half2(w[nt][2] - f1.x, w[nt][3] - f1.y)));
+        for (int nt = 0; nt < NT; ++nt) {
+          if constexpr (kCentred) {  // zeros + 8 s, summed beside the weights and rounded to nearest
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+              const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
+              const float z0 = fmaf(8.f, f0.x, f0.y), z1 = fmaf(8.f, f1.x, f1.y);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                zsum[nt][j][c] = vis[h][nt][c] ? fmaf(w[nt][c], z0, zsum[nt][j][c]) : zsum[nt][j][c];
+                zsum[nt][j][c] = vis[h][nt][2 + c] ? fmaf(w[nt][2 + c], z1, zsum[nt][j][c]) : zsum[nt][j][c];
+              }
+            }
           }
+          if constexpr (kPacked) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[nt][e] *= pm;
+            for (int r = 0; r < 2; ++r) wh[nt][r] = pack_half2(w[nt][2 * r] * pm, w[nt][2 * r + 1] * pm);
+            mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], transpose8x8(wh[nt][0]), transpose8x8(wh[nt][1]));
+          } else {
+            if constexpr (!kCentred) {
+              const uint32_t h0 = pack_half2(w[nt][0], w[nt][1]), h1 = pack_half2(w[nt][2], w[nt][3]);
+              mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], transpose8x8(h0), transpose8x8(h1));
+              const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
+              mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3],
+                      transpose8x8(pack_half2(w[nt][0] - f0.x, w[nt][1] - f0.y)),
+                      transpose8x8(pack_half2(w[nt][2] - f1.x, w[nt][3] - f1.y)));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[nt][e] *= pm;
+          }
         }
-      }
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-        uint32_t x01 = __byte_perm(vw[0][j / 2], vw[1][j / 2], sel);
-        uint32_t x23 = __byte_perm(vw[2][j / 2], vw[3][j / 2], sel);
-        uint32_t bf[NT][2][PP];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint32_t sz = r == 0 ? p0[j] : p1[j];
-            uint32_t h, rest = 0u;
-            if constexpr (kPacked) {
-              h = times_low(wh[nt][r], sz);
-            } else {
-              const float f = unpack_half2(sz).x;
-              const float u = w[nt][2 * r] * f, v = w[nt][2 * r + 1] * f;
-              h = pack_half2(u, v);
-              const float2 x = unpack_half2(h);
-              rest = pack_half2(u - x.x, v - x.y);
-            }
-            if constexpr (kMasked) {
-              const bool number = kCentred || ((sz >> 16) & 0x7c00u) != 0x7c00u;
-              if (!number) rest = 0u, h = 0x7fff7fffu;
-              h &= (vis[nt][2 * r] ? 0xffffu : 0u) | (vis[nt][2 * r + 1] ? 0xffff0000u : 0u);
-              rest &= (vis[nt][2 * r] ? 0xffffu : 0u) | (vis[nt][2 * r + 1] ? 0xffff0000u : 0u);
-            }
-            bf[nt][r][0] = transpose8x8(h);
-            if constexpr (PP == 2) bf[nt][r][1] = transpose8x8(rest);
-          }
-#pragma unroll
-        for (int m2 = 0; m2 < 2; ++m2) {
-          uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
-          uint32_t a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
-          if constexpr (kCentred) {
-            a0 = centred(a0, kMiddleLow), a1 = centred(a1, kMiddleHigh);
-            a2 = centred(a2, kMiddleLow), a3 = centred(a3, kMiddleHigh);
-          }
+        for (int j = 0; j < NG; ++j) {
+          const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+          uint32_t x01 = __byte_perm(vw[0][j / 2], vw[1][j / 2], sel);
+          uint32_t x23 = __byte_perm(vw[2][j / 2], vw[3][j / 2], sel);
+          uint32_t bf[NT][2][PP];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int pp = 0; pp < PP; ++pp) mma_f16(o[nt][j][m2], a0, a1, a2, a3, bf[nt][0][pp], bf[nt][1][pp]);
-          x01 >>= 8;
-          x23 >>= 8;
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t sz = r == 0 ? p0[j] : p1[j];
+              uint32_t x, rest = 0u;
+              if constexpr (kPacked) {
+                x = times_low(wh[nt][r], sz);
+              } else {
+                const float f = unpack_half2(sz).x;
+                const float u = w[nt][2 * r] * f, v = w[nt][2 * r + 1] * f;
+                x = pack_half2(u, v);
+                const float2 y = unpack_half2(x);
+                rest = pack_half2(u - y.x, v - y.y);
+              }
+              if constexpr (kMasked) {
+                const bool number = kCentred || ((sz >> 16) & 0x7c00u) != 0x7c00u;
+                if (!number) rest = 0u, x = 0x7fff7fffu;
+                const uint32_t seen = (vis[h][nt][2 * r] ? 0xffffu : 0u) | (vis[h][nt][2 * r + 1] ? 0xffff0000u : 0u);
+                x &= seen;
+                rest &= seen;
+              }
+              bf[nt][r][0] = transpose8x8(x);
+              if constexpr (PP == 2) bf[nt][r][1] = transpose8x8(rest);
+            }
+#pragma unroll
+          for (int m2 = 0; m2 < 2; ++m2) {
+            uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
+            uint32_t a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
+            if constexpr (kCentred) {
+              a0 = centred(a0, kMiddleLow), a1 = centred(a1, kMiddleHigh);
+              a2 = centred(a2, kMiddleLow), a3 = centred(a3, kMiddleHigh);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int pp = 0; pp < PP; ++pp) mma_f16(o[nt][j][m2], a0, a1, a2, a3, bf[nt][0][pp], bf[nt][1][pp]);
+            x01 >>= 8;
+            x23 >>= 8;
+          }
         }
       }
     };
 
-    for (int32_t k = 0; k < tiles; ++k) {
-      issue(k + G::kStages - 1);
-      wait_copies<G::kStages - 1>();  // this lane's share of tile k
-      __syncwarp();                   // and every other lane's
-      const uint32_t st = static_cast<uint32_t>(k) % G::kStages;
-      if (loaded[warp][st]) {
-        const int32_t key0 = (first_tile + k * kWarps) * static_cast<int32_t>(kKv4Tile);
-        const uint8_t* p = ring + st * G::kBytes;
-        if (key0 >= rows.lo_max && key0 + static_cast<int32_t>(kKv4Tile) - 1 <= rows.hi_min)
-          tile_step(p, key0, std::false_type{});
+    for (int32_t k = 0; k < steps; ++k) {
+      issue(k + kStages - 1);
+      wait_copies<kStages - 1>();  // this lane's share of step k
+      __syncwarp();                // and every other lane's
+      const uint32_t st = static_cast<uint32_t>(k) % kStages;
+      const uint32_t there = loaded[warp][st];
+      if (there != 0) {
+        const int32_t key0 = (first_tile + k * kUnit) * static_cast<int32_t>(kKv4Tile);
+        const uint8_t* p = ring + st * kStageBytes;
+        if (there == (1u << H) - 1u && key0 >= rows.lo_max && key0 + 16 * H - 1 <= rows.hi_min)
+          step(p, key0, there, std::false_type{});
         else
-          tile_step(p, key0, std::true_type{});
+          step(p, key0, there, std::true_type{});
       }
       __syncwarp();  // every lane has read the stage before it is filled again
     }
@@ -997,7 +1038,8 @@ Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint
   // unit where there are fewer (of the longest sequences the call allows).
   const uint64_t resident = 148ull * blocks_per_sm(static_cast<int>(dim), static_cast<int>(p.row_tile / 8), type == kF32 ? 2 : 1);
   const uint64_t tiles = (static_cast<uint64_t>(max_kv_len) + kKv4Tile - 1) / kKv4Tile;
-  const uint64_t item = tiles <= kWarps ? 1 : (tiles + kWarps - 1) / kWarps;
+  const uint64_t unit = kWarps * tiles_per_step(static_cast<int>(dim), static_cast<int>(p.row_tile / 8));
+  const uint64_t item = tiles <= unit ? 1 : (tiles + unit - 1) / unit;
   const uint64_t items = static_cast<uint64_t>(batch) * kv_heads * p.row_tiles;
   p.blocks = static_cast<uint32_t>(items >= resident || items * item >= resident ? resident : items * item);
   // an item of one unit is never split

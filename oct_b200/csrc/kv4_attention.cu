@@ -170,6 +170,12 @@ __device__ __forceinline__ void lds(uint32_t (&w)[N], const uint8_t* p) {
   }
 }
 
+// What a block began and did not finish, for the join.
+struct PartOf {
+  uint32_t last1 = 0;  // the last block with a part of it, plus 1; 0: nothing was left unfinished
+  uint32_t head = 0, first = 0, count = 0;  // its key head and rows
+  uint64_t row0 = 0, pad = 0;
+};
 struct KernelArgs {
   Kv4View view;
   const void* q;
@@ -182,7 +188,7 @@ struct KernelArgs {
   uint32_t row_tiles;
   float* part_o;    // [blocks][2][rows of a tile][D]
   float2* part_ml;  // [blocks][2][rows of a tile]
-  uint4* part_of;   // [blocks]: what the block's unfinished last item is, for the join
+  PartOf* part_of;  // [blocks]
 };
 
 // The keys that the rows of one row tile see: row r of a sequence is query
@@ -317,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   griddep_launch_dependents();
   Share share;
   const bool any = find_share(a, kRows, kUnit, &share);
-  if (threadIdx.x == 0 && a.part_of != nullptr) a.part_of[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+  if (threadIdx.x == 0 && a.part_of != nullptr) a.part_of[blockIdx.x] = PartOf{};
   if (!any) return;
 
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, i4 = lane % 4;
@@ -330,65 +336,87 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   const int32_t tok_ld = static_cast<int32_t>((lane & 1) ? 4 + (((lane % 8) >> 1) ^ 1u) : (lane % 8) >> 1) + 8 * static_cast<int32_t>((lane >> 3) & 1);
   const bool looks = kCentred || (g % 2 == 0 && g < 2 * NG);  // whether its row of the zeros' operand holds scales
 
-  unsigned long long unit = share.begin;
-  uint32_t pair = share.pair, head = share.head, offset = share.offset;
-  while (unit < share.end) {
+  // The item at `unit`, if it is this block's.
+  struct Item {
     Kv4Seq seq;
     Rows rows;
-    if (pair >= a.view.batch * a.row_tiles) break;  // lengths that changed under the call
-    if (!item_rows(a, pair, kRows, &seq, &rows)) {  // a sequence or row tile without rows has no units
-      ++pair;
-      continue;
+    uint32_t pair, head, offset, size, take;
+    int32_t first_tile, t1, steps;  // of this warp: tiles of step 0, of step 1 kUnit further, ... up to t1
+  };
+  unsigned long long unit = share.begin;
+  auto open = [&](Item* it, uint32_t pair, uint32_t head, uint32_t offset) {
+    if (unit >= share.end) return false;
+    while (true) {
+      if (pair >= a.view.batch * a.row_tiles) return false;  // lengths that changed under the call
+      if (item_rows(a, pair, kRows, &it->seq, &it->rows)) break;
+      ++pair;  // a sequence or row tile without rows has no units
     }
-    const uint32_t size = item_units(rows, kUnit) + share.cost;
-    const uint32_t take = static_cast<uint32_t>(min(static_cast<unsigned long long>(size - offset), share.end - unit));
+    it->pair = pair, it->head = head, it->offset = offset;
+    it->size = item_units(it->rows, kUnit) + share.cost;
+    it->take = static_cast<uint32_t>(min(static_cast<unsigned long long>(it->size - offset), share.end - unit));
     // the item's cost comes first in its run; the units behind it are its tiles
-    const uint32_t unit0 = max(offset, share.cost) - share.cost, unit1 = max(offset + take, share.cost) - share.cost;
-    const int32_t t0 = rows.t_begin + static_cast<int32_t>(unit0 * kUnit);
-    const int32_t t1 = min(rows.t_end, rows.t_begin + static_cast<int32_t>(unit1 * kUnit));
-    const int32_t first_tile = t0 + static_cast<int32_t>(warp) * H;  // of step 0; each step is kUnit further
-    const int32_t steps = first_tile < t1 ? (t1 - first_tile + kUnit - 1) / kUnit : 0;
-
-    // Which of the cache's tiles this warp's next 32 steps take, one step per lane (kNoTile: no page
-    // of the cache, or behind the last key).
-    const int32_t* table = a.view.table + pair / a.row_tiles * a.view.table_stride;
-    uint32_t source[H];
-    auto locate = [&](int32_t k0) {
-      const int32_t t = first_tile + (k0 + static_cast<int32_t>(lane)) * kUnit;
+    const uint32_t unit0 = max(offset, share.cost) - share.cost;
+    const uint32_t unit1 = max(offset + it->take, share.cost) - share.cost;
+    it->first_tile = it->rows.t_begin + static_cast<int32_t>(unit0 * kUnit + warp * H);
+    it->t1 = min(it->rows.t_end, it->rows.t_begin + static_cast<int32_t>(unit1 * kUnit));
+    it->steps = it->first_tile < it->t1 ? (it->t1 - it->first_tile + kUnit - 1) / kUnit : 0;
+    return true;
+  };
+  // Which of the cache's tiles this warp's next 32 steps take, one step per lane (kNoTile: no page
+  // of the cache, or behind the last key).
+  uint32_t source[H];
+  auto locate = [&](const Item& it, int32_t k0) {
+    const int32_t* table = a.view.table + it.pair / a.row_tiles * a.view.table_stride;
+    const int32_t t = it.first_tile + (k0 + static_cast<int32_t>(lane)) * kUnit;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      source[h] = kNoTile;
+      if (t + h >= it.t1) continue;
+      const uint32_t in_table = static_cast<uint32_t>(t + h) / a.view.page_tiles;
+      const uint32_t page = static_cast<uint32_t>(table[in_table]);
+      if (page < a.view.pages)
+        source[h] = (page * a.view.kv_heads + it.head) * a.view.page_tiles + (t + h) - in_table * a.view.page_tiles;
+      else
+        atomicOr(a.view.bad, 1u);
+    }
+  };
+  // The tiles of step k into its stage; one commit group per call, empty behind the last step.
+  auto issue = [&](const Item& it, int32_t k) {
+    if (k < it.steps) {
+      if (k % 32 == 0) locate(it, k);
+      const uint32_t st = static_cast<uint32_t>(k) % kStages;
+      uint32_t there = 0;
 #pragma unroll
       for (int h = 0; h < H; ++h) {
-        source[h] = kNoTile;
-        if (t + h >= t1) continue;
-        const uint32_t in_table = static_cast<uint32_t>(t + h) / a.view.page_tiles;
-        const uint32_t page = static_cast<uint32_t>(table[in_table]);
-        if (page < a.view.pages)
-          source[h] = (page * a.view.kv_heads + head) * a.view.page_tiles + (t + h) - in_table * a.view.page_tiles;
-        else
-          atomicOr(a.view.bad, 1u);
-      }
-    };
-    // The tiles of step k into its stage; one commit group per call, empty behind the last step.
-    auto issue = [&](int32_t k) {
-      if (k < steps) {
-        if (k % 32 == 0) locate(k);
-        const uint32_t st = static_cast<uint32_t>(k) % kStages;
-        uint32_t there = 0;
+        const uint32_t tile = __shfl_sync(0xffffffffu, source[h], k % 32);
+        if (tile == kNoTile) continue;
+        there |= 1u << h;
+        const uint8_t* from = a.view.data + static_cast<uint64_t>(tile) * G::kBytes + 16 * lane;
+        uint8_t* to = ring + st * kStageBytes + h * G::kBytes + 16 * lane;
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-          const uint32_t tile = __shfl_sync(0xffffffffu, source[h], k % 32);
-          if (tile == kNoTile) continue;
-          there |= 1u << h;
-          const uint8_t* from = a.view.data + static_cast<uint64_t>(tile) * G::kBytes + 16 * lane;
-          uint8_t* to = ring + st * kStageBytes + h * G::kBytes + 16 * lane;
-#pragma unroll
-          for (int c = 0; c < G::kBytes; c += 512)
-            if (c + 512 <= G::kBytes || c + 16 * static_cast<int>(lane) < G::kBytes) copy16(to + c, from + c);
-        }
-        if (lane == 0) loaded[warp][st] = there;
+        for (int c = 0; c < G::kBytes; c += 512)
+          if (c + 512 <= G::kBytes || c + 16 * static_cast<int>(lane) < G::kBytes) copy16(to + c, from + c);
       }
-      commit_copies();
-    };
-    for (int32_t k = 0; k < kStages - 1; ++k) issue(k);
+      if (lane == 0) loaded[warp][st] = there;
+    }
+    commit_copies();
+  };
+  // A warp's result lies in the last stages of its ring; the next item's first steps are on their way
+  // to the stages before them while the block's warps are joined.
+  constexpr int kResultStages = (kRows * D * 4 + kStageBytes - 1) / kStageBytes;
+  constexpr int kAhead = kStages - kResultStages < kStages - 1 ? kStages - kResultStages : kStages - 1;
+  static_assert(kAhead >= 0, "the ring holds the warp's result at the end");
+  float* const mine = reinterpret_cast<float*>(ring + (kStages - kResultStages) * kStageBytes);  // [8 NT][D]
+
+  Item item;
+  bool more = open(&item, share.pair, share.head, share.offset);
+  if (more)
+    for (int32_t k = 0; k < kAhead; ++k) issue(item, k);
+  while (more) {
+    const Kv4Seq& seq = item.seq;
+    const Rows& rows = item.rows;
+    const uint32_t head = item.head;
+    for (int32_t k = kAhead; k < kStages - 1; ++k) issue(item, k);
 
     // Query fragments: column g of group nt is row rows.first + 8 nt + g.
     uint32_t qf[NT][NG][2][2][QP];
@@ -796,14 +824,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       }
     };
 
-    for (int32_t k = 0; k < steps; ++k) {
-      issue(k + kStages - 1);
+    for (int32_t k = 0; k < item.steps; ++k) {
+      issue(item, k + kStages - 1);
       wait_copies<kStages - 1>();  // this lane's share of step k
       __syncwarp();                // and every other lane's
       const uint32_t st = static_cast<uint32_t>(k) % kStages;
       const uint32_t there = loaded[warp][st];
       if (there != 0) {
-        const int32_t key0 = (first_tile + k * kUnit) * static_cast<int32_t>(kKv4Tile);
+        const int32_t key0 = (item.first_tile + k * kUnit) * static_cast<int32_t>(kKv4Tile);
         const uint8_t* p = ring + st * kStageBytes;
         if (there == (1u << H) - 1u && key0 >= rows.lo_max && key0 + 16 * H - 1 <= rows.hi_min)
           step(p, key0, there, std::false_type{});
@@ -814,7 +842,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     }
 
     // ---- this warp's result, then the block's
-    float* mine = reinterpret_cast<float*>(ring);  // [8 NT][D]
     const float unit_f = pm_limit < 0.f ? 0.f : 1.f / pm;
     const float low = kCentred ? unit_f : unit_f * kCodeLow, high = kCentred ? unit_f * 0.0625f : unit_f * kCodeHigh;
     __syncwarp();
@@ -845,12 +872,23 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
             to[m2] = make_float2(fmaf(o[nt][j][m2][c], low, z), fmaf(o[nt][j][m2][2 + c], high, z));
         }
       }
+    const uint64_t row0 = seq.row0;
+    const uint32_t first_row = rows.first, count = rows.count;
+    const bool whole = item.take == item.size;
+    const uint32_t slot = blockIdx.x * 2 + (item.offset == 0 ? 1u : 0u);
+    if (!whole && item.offset == 0 && threadIdx.x == 0) {
+      const uint32_t last = static_cast<uint32_t>((unit + item.size - 1) / share.per);
+      a.part_of[blockIdx.x] = PartOf{min(last, gridDim.x - 1) + 1, head, first_row, count, row0};
+    }
+    unit += item.take;
+    const bool next_pair = head + 1 == a.view.kv_heads;
+    more = open(&item, item.pair + (next_pair ? 1 : 0), next_pair ? 0 : head + 1, 0);
+    if (more)
+      for (int32_t k = 0; k < kAhead; ++k) issue(item, k);
     __syncthreads();
-    const bool whole = take == size;
-    const uint32_t slot = blockIdx.x * 2 + (offset == 0 ? 1u : 0u);
-    const float* all = reinterpret_cast<const float*>(smem);
+    const float* all = reinterpret_cast<const float*>(smem + (kStages - kResultStages) * kStageBytes);
     constexpr int kWarpFloats = G::kStages * G::kBytes / 4;
-    for (uint32_t e = threadIdx.x; e < rows.count * (D / 4); e += kThreads) {
+    for (uint32_t e = threadIdx.x; e < count * (D / 4); e += kThreads) {
       const uint32_t col = e / (D / 4), c4 = e % (D / 4);
       float top = -INFINITY;
 #pragma unroll
@@ -871,8 +909,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
         sum.w = fmaf(f, x.w, sum.w);
       }
       if (whole) {
-        const uint32_t row = rows.first + col;
-        const uint64_t token = seq.row0 + row / a.share;
+        const uint32_t row = first_row + col;
+        const uint64_t token = row0 + row / a.share;
         const uint32_t qh = head * a.share + row % a.share;
         const float inv = top == -INFINITY ? 0.f : 1.0f / total;
         store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c4,
@@ -885,88 +923,78 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
         if (c4 == 0) a.part_ml[at] = make_float2(top, total);
       }
     }
-    if (!whole && offset == 0 && threadIdx.x == 0) {
-      const uint32_t last = static_cast<uint32_t>((unit + size - 1) / share.per);
-      a.part_of[blockIdx.x] = make_uint4(1u, pair, head, min(last, gridDim.x - 1));
-    }
-    unit += take;
-    offset = 0;
-    if (++head == a.view.kv_heads) head = 0, ++pair;
     __syncthreads();  // the next item's copies overwrite what was written and read here
   }
 }
 
 // Joins the parts of every item that was split: block x looks at what block x of the first kernel
 // began and did not finish, whose other parts lie in slot 0 of the blocks behind it; grid y deals out
-// the channels.  The parts of a (row, four channels) are dealt to `lanes` threads and their sums added
-// in a fixed order.
-constexpr int kJoinThreads = 512;
-template <int D> constexpr int kJoinColumns = D / 4 < 16 ? D / 4 : 16;  // float4 columns of a block
+// the channels.  The parts of a (row, four channels) are dealt to `lanes` threads and what they make
+// of them is joined in a fixed order.
+constexpr int kJoinThreads = 256, kJoinColumns = 16;  // 16 float4 columns of a row per block
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const KernelArgs a, uint32_t rows_per_tile) {
-  constexpr int kCols = kJoinColumns<D>;
-  constexpr int kParts = kJoinThreads / kCols;  // threads over (row, part)
+  constexpr uint32_t kWho = kJoinThreads / kJoinColumns;  // threads over (row, part)
   __shared__ float4 part[kJoinThreads];
-  __shared__ float part_l[kParts], part_top[kParts];
+  __shared__ float2 part_ml[kWho];
   griddep_wait();
-  const uint4 of = a.part_of[blockIdx.x];
-  if (of.x == 0u) return;
-  const uint32_t parts = of.w - blockIdx.x + 1;
-  Kv4Seq seq;
-  Rows rows;
-  if (!item_rows(a, of.y, rows_per_tile, &seq, &rows)) return;
-  const uint32_t c4 = threadIdx.x % kCols, who = threadIdx.x / kCols;
-  uint32_t lanes = kParts;  // threads per row: a power of two
-  while (lanes > 1 && lanes * rows.count > static_cast<uint32_t>(kParts)) lanes >>= 1;
-  const uint32_t per_pass = kParts / lanes, sub = who % lanes;
-  for (uint32_t r0 = 0; r0 < rows.count; r0 += per_pass) {
+  const PartOf of = a.part_of[blockIdx.x];
+  if (of.last1 == 0u) return;
+  const uint32_t parts = of.last1 - blockIdx.x;
+  const uint32_t c4 = threadIdx.x % kJoinColumns, who = threadIdx.x / kJoinColumns;
+  const uint32_t channel = 4 * (blockIdx.y * kJoinColumns + c4);
+  uint32_t lanes = kWho;  // threads per row: a power of two
+  while (lanes > 1 && lanes * of.count > kWho) lanes >>= 1;
+  const uint32_t sub = who % lanes;
+  for (uint32_t r0 = 0; r0 < of.count; r0 += kWho / lanes) {
     const uint32_t col = r0 + who / lanes;
-    const bool live = col < rows.count;
-    auto place = [&](uint32_t p) {
-      return (static_cast<uint64_t>(blockIdx.x + p) * 2 + (p == 0 ? 1u : 0u)) * rows_per_tile + col;
-    };
-    float top = -INFINITY;
-    if (live)
-#pragma unroll 4
-      for (uint32_t p = sub; p < parts; p += lanes) top = fmaxf(top, a.part_ml[place(p)].x);
-    if (c4 == 0) part_top[who] = top;
-    __syncthreads();
-    for (uint32_t i = 0; i < lanes; ++i) top = fmaxf(top, part_top[who - sub + i]);
-    const float base = top == -INFINITY ? 0.f : top;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float total = 0.f;
-    if (live)
-#pragma unroll 8
-      for (uint32_t p = sub; p < parts; p += lanes) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    auto add = [&](float2 n, float4 x) {
+      const float top = fmaxf(ml.x, n.x), base = top == -INFINITY ? 0.f : top;
+      const float f = exp2_approx(ml.x - base), g = exp2_approx(n.x - base);
+      ml = make_float2(top, fmaf(f, ml.y, g * n.y));
+      sum.x = fmaf(f, sum.x, g * x.x);
+      sum.y = fmaf(f, sum.y, g * x.y);
+      sum.z = fmaf(f, sum.z, g * x.z);
+      sum.w = fmaf(f, sum.w, g * x.w);
+    };
+    if (col < of.count) {
+      auto place = [&](uint32_t p) {
+        return (static_cast<uint64_t>(blockIdx.x + p) * 2 + (p == 0 ? 1u : 0u)) * rows_per_tile + col;
+      };
+      uint32_t p = sub;
+      for (; p + 3 * lanes < parts; p += 4 * lanes) {  // four parts' loads together
+        float2 n[4];
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint64_t at = place(p + i * lanes);
+          n[i] = a.part_ml[at];
+          x[i] = *reinterpret_cast<const float4*>(a.part_o + at * D + channel);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add(n[i], x[i]);
+      }
+      for (; p < parts; p += lanes) {
         const uint64_t at = place(p);
-        const float2 ml = a.part_ml[at];
-        const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * D + 4 * (blockIdx.y * kCols + c4));
-        if (ml.x == -INFINITY) continue;
-        const float f = exp2_approx(ml.x - base);
-        total = fmaf(f, ml.y, total);
-        sum.x = fmaf(f, x.x, sum.x);
-        sum.y = fmaf(f, x.y, sum.y);
-        sum.z = fmaf(f, x.z, sum.z);
-        sum.w = fmaf(f, x.w, sum.w);
+        add(a.part_ml[at], *reinterpret_cast<const float4*>(a.part_o + at * D + channel));
       }
+    }
     part[threadIdx.x] = sum;
-    if (c4 == 0) part_l[who] = total;
+    if (c4 == 0) part_ml[who] = ml;
     __syncthreads();
-    if (live && sub == 0) {
-      for (uint32_t i = 1; i < lanes; ++i) {
-        const float4 x = part[threadIdx.x + i * kCols];
-        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
-        total += part_l[who + i];
-      }
-      const uint32_t row = rows.first + col;
-      const uint64_t token = seq.row0 + row / a.share;
-      const uint32_t qh = of.z * a.share + row % a.share;
-      const float inv = top == -INFINITY ? 0.f : 1.0f / total;
-      store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * (blockIdx.y * kCols + c4),
+    if (col < of.count && sub == 0) {
+      for (uint32_t i = 1; i < lanes; ++i) add(part_ml[who + i], part[threadIdx.x + i * kJoinColumns]);
+      const uint32_t row = of.first + col;
+      const uint64_t token = of.row0 + row / a.share;
+      const uint32_t qh = of.head * a.share + row % a.share;
+      const float inv = ml.x == -INFINITY ? 0.f : 1.0f / ml.y;
+      store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + channel,
              make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
-      if (c4 == 0 && blockIdx.y == 0 && a.lse != nullptr)
-        a.lse[token * a.heads + qh] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
+      if (channel == 0 && a.lse != nullptr)
+        a.lse[token * a.heads + qh] = ml.x == -INFINITY ? -INFINITY : (ml.x + log2f(ml.y)) * kLn2;
     }
     __syncthreads();
   }
@@ -979,7 +1007,6 @@ cudaError_t launch(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream
   constexpr int QP = kQueryParts<T>;
   constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
   constexpr size_t kSmem = static_cast<size_t>(kWarps) * G::kStages * G::kBytes;
-  static_assert(G::kStages * G::kBytes >= 8 * NT * D * 4, "the ring holds the warp's result at the end");
   const auto kernel = kv4_attention_kernel<T, D, NT, QP, PP>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
   if (e != cudaSuccess) return e;
@@ -987,7 +1014,7 @@ cudaError_t launch(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream
   e = cudaGetLastError();
   if (e != cudaSuccess || plan.workspace == 0) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(plan.blocks, D / 4 / kJoinColumns<D>);
+  cfg.gridDim = dim3(plan.blocks, D / 4 / kJoinColumns);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -1044,7 +1071,7 @@ Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint
   p.blocks = static_cast<uint32_t>(items >= resident || items * item >= resident ? resident : items * item);
   // an item of one unit is never split
   if (item > 1)
-    p.workspace = static_cast<uint64_t>(p.blocks) * (2 * p.row_tile * (static_cast<uint64_t>(dim) * 4 + 8) + 16);
+    p.workspace = static_cast<uint64_t>(p.blocks) * (2 * p.row_tile * (static_cast<uint64_t>(dim) * 4 + 8) + sizeof(PartOf));
   return p;
 }
 
@@ -1068,7 +1095,7 @@ cudaError_t kv4_attention(const Kv4AttnArgs& in, const Kv4Plan& plan, cudaStream
   if (plan.workspace > 0) {
     const uint64_t parts = 2ull * plan.blocks * plan.row_tile;
     a.part_o = static_cast<float*>(in.workspace);
-    a.part_of = reinterpret_cast<uint4*>(a.part_o + parts * in.view.dim);
+    a.part_of = reinterpret_cast<PartOf*>(a.part_o + parts * in.view.dim);
     a.part_ml = reinterpret_cast<float2*>(a.part_of + plan.blocks);
   }
   switch (in.type) {

@@ -133,6 +133,12 @@ __device__ __forceinline__ uint32_t times_low(uint32_t a, uint32_t b) {
   const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), __low2half2(*reinterpret_cast<const __half2*>(&b)));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// a times the low half of b, plus c
+__device__ __forceinline__ uint32_t fma_low(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), __low2half2(*reinterpret_cast<const __half2*>(&b)),
+                            *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 __device__ __forceinline__ float2 unpack_half2(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
@@ -233,68 +239,79 @@ __device__ __forceinline__ bool item_rows(const KernelArgs& a, uint32_t pair, ui
   return kv4_seq(a.view, b, s) && row_range(a, *s, pair - b * a.row_tiles, rows_per_tile, r);
 }
 // What an item costs beside its units, in units: finding its pages, loading its queries, joining its
-// warps (about 5 us against 1.4 us of a unit).  Counted where blocks get several units, so that one
-// with many short items gets fewer of them; where units are few, latency counts and each has its block.
-constexpr uint32_t kItemCost = 3;
+// warps.  Counted where blocks get several units, so that one with many short items gets fewer of them
+// (64 sequences of up to 16384 keys: 151 us at a cost of 1, 127 at 5, 129 at 8).  Where units are few,
+// latency counts: there no block gets parts of two items, an item's run is filled up to whole shares.
+constexpr uint32_t kItemCost = 5;
 struct Share {
-  unsigned long long begin, end, per;  // this block's run of all items' units and costs; every block's
-  uint32_t cost;                       // kItemCost or 0
-  uint32_t pair, head, offset;         // where it begins
+  uint32_t begin, end, per;     // this block's run of all items' runs; every block's length
+  uint32_t cost, pad;           // kItemCost or 0; shares that an item's run is filled up to, or 1
+  uint32_t pair, head, offset;  // where it begins
+  __device__ __forceinline__ uint32_t size(uint32_t units) const { return (units + cost + pad - 1) / pad * pad; }
 };
-// Called by the whole block.
+// Called by the whole block.  Sums fit in 32 bits: the host refuses calls whose bounds do not.
 __device__ __forceinline__ bool find_share(const KernelArgs& a, uint32_t rows_per_tile, int32_t unit_tiles, Share* out) {
-  __shared__ unsigned long long warp_sums[2][kWarps];
+  __shared__ uint32_t warp_sums[3][kWarps];
   __shared__ uint32_t found[3];
   const uint32_t pairs = a.view.batch * a.row_tiles, chunk = (pairs + kThreads - 1) / kThreads;
   const uint32_t p0 = min(pairs, threadIdx.x * chunk), p1 = min(pairs, p0 + chunk);
-  unsigned long long sums[2] = {0, 0};  // units, items
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   Kv4Seq s;
   Rows r;
+  uint32_t units = 0, items = 0;
   for (uint32_t p = p0; p < p1; ++p)
-    if (item_rows(a, p, rows_per_tile, &s, &r)) sums[0] += item_units(r, unit_tiles), ++sums[1];
-  unsigned long long upto[2];
-  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    sums[i] *= a.view.kv_heads;
-    upto[i] = sums[i];
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const unsigned long long v = __shfl_up_sync(0xffffffffu, upto[i], d);
-      if (lane >= static_cast<uint32_t>(d)) upto[i] += v;
-    }
-    if (lane == 31) warp_sums[i][warp] = upto[i];
-  }
+    if (item_rows(a, p, rows_per_tile, &s, &r)) units += item_units(r, unit_tiles), ++items;
+  const uint32_t unit_sum = __reduce_add_sync(0xffffffffu, units), item_sum = __reduce_add_sync(0xffffffffu, items);
+  if (lane == 0) warp_sums[0][warp] = unit_sum, warp_sums[1][warp] = item_sum;
   __syncthreads();
-  unsigned long long total[2] = {0, 0};
+  uint32_t total = 0, all_items = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int w = 0; w < kWarps; ++w) total += warp_sums[0][w], all_items += warp_sums[1][w];
+  total *= a.view.kv_heads;
+  all_items *= a.view.kv_heads;
+  const bool few = total <= 4 * gridDim.x && all_items <= gridDim.x / 2;
+  out->cost = few ? 0 : kItemCost;
+  const uint32_t run = total + out->cost * all_items, blocks = few ? gridDim.x - all_items : gridDim.x;
+  out->per = max(1u, (run + blocks - 1) / blocks);
+  out->pad = few ? out->per : 1;
+  // runs of the threads before this one
+  uint32_t mine = units + out->cost * items;
+  if (few) {
+    mine = 0;
+    for (uint32_t p = p0; p < p1; ++p)
+      if (item_rows(a, p, rows_per_tile, &s, &r)) mine += out->size(item_units(r, unit_tiles));
+  }
+  mine *= a.view.kv_heads;
+  uint32_t upto = mine;
 #pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) {
-      if (w < warp) upto[i] += warp_sums[i][w];
-      total[i] += warp_sums[i][w];
-    }
-  out->cost = total[0] > 4ull * gridDim.x ? kItemCost : 0;
-  const unsigned long long all = total[0] + out->cost * total[1];
-  out->per = all <= gridDim.x ? 1 : (all + gridDim.x - 1) / gridDim.x;
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= static_cast<uint32_t>(d)) upto += v;
+  }
+  if (lane == 31) warp_sums[2][warp] = upto;
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kWarps; ++w) {
+    if (w < warp) upto += warp_sums[2][w];
+    all += warp_sums[2][w];
+  }
   out->begin = blockIdx.x * out->per;
   out->end = min(all, out->begin + out->per);
   if (out->begin >= all) return false;
-  const unsigned long long last = upto[0] + out->cost * upto[1];
-  unsigned long long at = last - (sums[0] + out->cost * sums[1]);
-  if (out->begin >= at && out->begin < last)
+  uint32_t at = upto - mine;
+  if (out->begin >= at && out->begin < upto)
     for (uint32_t p = p0; p < p1; ++p)
       if (item_rows(a, p, rows_per_tile, &s, &r)) {
-        const uint32_t size = item_units(r, unit_tiles) + out->cost;
-        const unsigned long long heads = static_cast<unsigned long long>(size) * a.view.kv_heads;
-        if (out->begin < at + heads) {
-          const uint32_t rest = static_cast<uint32_t>(out->begin - at);
+        const uint32_t size = out->size(item_units(r, unit_tiles));
+        if (out->begin < at + size * a.view.kv_heads) {
+          const uint32_t rest = out->begin - at;
           found[0] = p;
           found[1] = rest / size;
           found[2] = rest % size;
           break;
         }
-        at += heads;
+        at += size * a.view.kv_heads;
       }
   __syncthreads();
   out->pair = found[0];
@@ -315,7 +332,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   constexpr int H = tiles_per_step(D, NT), kUnit = kWarps * H;
   constexpr int kStages = G::kStages / H, kStageBytes = H * G::kBytes;
   constexpr bool kCentred = std::is_same<T, float>::value;
-  constexpr bool kPacked = PP == 1;  // weight * scale is formed in float16
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t loaded[kWarps][kStages];
   __shared__ float2 warp_ml[kWarps][kRows];
@@ -343,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     uint32_t pair, head, offset, size, take;
     int32_t first_tile, t1, steps;  // of this warp: tiles of step 0, of step 1 kUnit further, ... up to t1
   };
-  unsigned long long unit = share.begin;
+  uint32_t unit = share.begin;
   auto open = [&](Item* it, uint32_t pair, uint32_t head, uint32_t offset) {
     if (unit >= share.end) return false;
     while (true) {
@@ -352,8 +368,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       ++pair;  // a sequence or row tile without rows has no units
     }
     it->pair = pair, it->head = head, it->offset = offset;
-    it->size = item_units(it->rows, kUnit) + share.cost;
-    it->take = static_cast<uint32_t>(min(static_cast<unsigned long long>(it->size - offset), share.end - unit));
+    it->size = share.size(item_units(it->rows, kUnit));
+    it->take = min(it->size - offset, share.end - unit);
     // the item's cost comes first in its run; the units behind it are its tiles
     const uint32_t unit0 = max(offset, share.cost) - share.cost;
     const uint32_t unit1 = max(offset + it->take, share.cost) - share.cost;
@@ -518,7 +534,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
 #pragma unroll
       for (int e = 0; e < 4; ++e) oz[nt][e] = 0.f;
     }
-    float pm = 0.f, pm_limit = -1.f;  // weights enter as w * s * pm; s <= pm_limit keeps that in float16
+    // weights enter as w * pm and w * pm * s in float16: pm <= 2^11 and s <= pm_limit keep both below 2^15
+    float pm = 0.f, pm_limit = -1.f;
 
     // One step: H tiles (key0: position of the first token; there: which of them are in the stage).
     auto step = [&](const uint8_t* stage, int32_t key0, uint32_t there, auto masked_tag) {
@@ -707,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
         // a largest scale of zero sets no measure for those to come
-        const float next = kPacked ? fminf(pow2_toward(smax, 9), 2048.f) : pow2_toward(smax, 9);
+        const float next = fminf(pow2_toward(smax, 9), 2048.f);
         const float ratio = pm_limit < 0.f ? 0.f : next / pm;
         pm = next;
         pm_limit = smax > 0.f ? 2048.f / next : 0.f;
@@ -719,10 +736,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
             for (int m2 = 0; m2 < 2; ++m2)
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[nt][j][m2][e] *= ratio;
-          if constexpr (kPacked) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) oz[nt][e] *= ratio;
-          }
+          for (int e = 0; e < 4; ++e) oz[nt][e] *= ratio;
         }
       }
 #pragma unroll
@@ -741,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
             if (!keep[h][1]) p1[j] = 0u;
           }
         }
-        [[maybe_unused]] uint32_t wh[NT][2];  // kPacked: w * pm
+        [[maybe_unused]] uint32_t wh[NT][2], wl[NT][2];  // w * pm in float16, and what that leaves
         float(&w)[NT][4] = raw[h];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -757,21 +772,19 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
               }
             }
           }
-          if constexpr (kPacked) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) wh[nt][r] = pack_half2(w[nt][2 * r] * pm, w[nt][2 * r + 1] * pm);
-            mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], transpose8x8(wh[nt][0]), transpose8x8(wh[nt][1]));
-          } else {
-            if constexpr (!kCentred) {
-              const uint32_t h0 = pack_half2(w[nt][0], w[nt][1]), h1 = pack_half2(w[nt][2], w[nt][3]);
-              mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], transpose8x8(h0), transpose8x8(h1));
-              const float2 f0 = unpack_half2(h0), f1 = unpack_half2(h1);
-              mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3],
-                      transpose8x8(pack_half2(w[nt][0] - f0.x, w[nt][1] - f0.y)),
-                      transpose8x8(pack_half2(w[nt][2] - f1.x, w[nt][3] - f1.y)));
+          for (int r = 0; r < 2; ++r) {
+            const float u = w[nt][2 * r] * pm, v = w[nt][2 * r + 1] * pm;
+            wh[nt][r] = pack_half2(u, v);
+            if constexpr (PP == 2) {
+              const float2 f = unpack_half2(wh[nt][r]);
+              wl[nt][r] = pack_half2(u - f.x, v - f.y);
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[nt][e] *= pm;
+          }
+          if constexpr (!kCentred) {
+            mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], transpose8x8(wh[nt][0]), transpose8x8(wh[nt][1]));
+            if constexpr (PP == 2)
+              mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], transpose8x8(wl[nt][0]), transpose8x8(wl[nt][1]));
           }
         }
 #pragma unroll
@@ -785,16 +798,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const uint32_t sz = r == 0 ? p0[j] : p1[j];
-              uint32_t x, rest = 0u;
-              if constexpr (kPacked) {
-                x = times_low(wh[nt][r], sz);
-              } else {
-                const float f = unpack_half2(sz).x;
-                const float u = w[nt][2 * r] * f, v = w[nt][2 * r + 1] * f;
-                x = pack_half2(u, v);
-                const float2 y = unpack_half2(x);
-                rest = pack_half2(u - y.x, v - y.y);
-              }
+              // weight * scale: the product rounded to float16, and in two parts what the rounding left,
+              // exactly, plus the weight's own second part
+              uint32_t x = times_low(wh[nt][r], sz), rest = 0u;
+              if constexpr (PP == 2) rest = fma_low(wl[nt][r], sz, fma_low(wh[nt][r], sz, x ^ 0x80008000u));
               if constexpr (kMasked) {
                 const bool number = kCentred || ((sz >> 16) & 0x7c00u) != 0x7c00u;
                 if (!number) rest = 0u, x = 0x7fff7fffu;
@@ -864,7 +871,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
             for (int d = 4; d < 32; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
           } else {
             z = __shfl_sync(0xffffffffu, oz[nt][j < 4 ? c : 2 + c], 4 * (2 * (j % 4) + 1) + i4);
-            if constexpr (kPacked) z *= unit_f;
+            z *= unit_f;
           }
           float2* to = reinterpret_cast<float2*>(mine + col * D + 32 * j + 4 * g);
 #pragma unroll
@@ -877,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     const bool whole = item.take == item.size;
     const uint32_t slot = blockIdx.x * 2 + (item.offset == 0 ? 1u : 0u);
     if (!whole && item.offset == 0 && threadIdx.x == 0) {
-      const uint32_t last = static_cast<uint32_t>((unit + item.size - 1) / share.per);
+      const uint32_t last = (unit + item.size - 1) / share.per;
       a.part_of[blockIdx.x] = PartOf{min(last, gridDim.x - 1) + 1, head, first_row, count, row0};
     }
     unit += item.take;
@@ -1068,7 +1075,8 @@ Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint
   const uint64_t unit = kWarps * tiles_per_step(static_cast<int>(dim), static_cast<int>(p.row_tile / 8));
   const uint64_t item = tiles <= unit ? 1 : (tiles + unit - 1) / unit;
   const uint64_t items = static_cast<uint64_t>(batch) * kv_heads * p.row_tiles;
-  p.blocks = static_cast<uint32_t>(items >= resident || items * item >= resident ? resident : items * item);
+  p.blocks = static_cast<uint32_t>(items >= resident || items * (item + 1) >= resident ? resident : items * (item + 1));
+  p.run = items * (item + kItemCost);
   // an item of one unit is never split
   if (item > 1)
     p.workspace = static_cast<uint64_t>(p.blocks) * (2 * p.row_tile * (static_cast<uint64_t>(dim) * 4 + 8) + sizeof(PartOf));

@@ -185,8 +185,8 @@ int check_attention(const OctB200Kv4Cache* c, const OctB200Kv4Batch* b, const Oc
     return OCT_B200_DETAIL_UNSUPPORTED_SHAPE;
   *plan = oct::kv4_attention_plan(c->head_dim, c->kv_heads, r->q_heads, b->batch, b->max_tokens, b->max_kv_len,
                                   static_cast<oct::ElementType>(r->dtype));
-  // every block looks through the (sequence, row tile) pairs
-  return plan->row_tiles * b->batch > 0x3fffffffull ? OCT_B200_DETAIL_UNSUPPORTED_SHAPE : 0;
+  // work is counted in 32 bits, in units of 64 or 128 keys of an item
+  return plan->row_tiles * b->batch > 0x3fffffffull || plan->run > 0x3fffffffull ? OCT_B200_DETAIL_UNSUPPORTED_SHAPE : 0;
 }
 
 }  // namespace

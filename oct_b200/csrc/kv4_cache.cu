@@ -15,9 +15,9 @@
 // fragments both read their operands from that one order without unpacking a
 // code twice.
 //
-// Bound: HBM.  A warp takes one tile's keys or values of one head: one page
-// lookup serves up to 16 rows, and the loads of four passes are in flight at
-// once.  A lane holds 8 channels of a row (one 16-byte load of a 16-bit type),
+// Bound: HBM.  A warp takes rows of one tile's keys or values of one head: one page
+// lookup serves them all, and the loads of four passes over its lanes are in flight
+// at once.  A lane holds 8 channels of a row (one 16-byte load of a 16-bit type),
 // a group is 4 lanes and a row dim/8, so a group's bounds need two shuffles;
 // one more pairs the halfwords of neighbouring groups into whole words.
 #include <type_traits>
@@ -73,57 +73,71 @@ __device__ __forceinline__ __half2 group_params(float lo, float hi) {
   return __halves2half2(s, z);
 }
 
-// The integer nearest to (x - z) / s, exactly: where the remainder of the guess reaches half a
-// step it decides, and at exactly half a step the rounding error of x - z does, or the even integer.
-__device__ __noinline__ uint32_t exact_code(float x, float z, float s) {
-  const float d = x - z;
-  float c = rintf(d / s);
-  const float rem = fmaf(-c, s, d);  // one rounding: its comparison with s / 2 is exact
-  const float half = 0.5f * s;
-  if (rem > half) {
-    c += 1.f;
-  } else if (rem < -half) {
-    c -= 1.f;
-  } else if (fabsf(rem) == half) {
-    const float err = difference_error(x, z, d);
-    const float low = rem > 0.f ? c : c - 1.f;  // d = (low + 1/2) s
-    c = err > 0.f ? low + 1.f : (err < 0.f ? low : 2.f * rintf(0.5f * (low + 0.5f)));
-  }
-  return static_cast<uint32_t>(c);
+// What a guess c of (x - z) / s is corrected by when its remainder d - c s reaches half a step: beyond
+// it by one; at exactly half a step the rounding error of d = x - z decides, or the even integer.
+__device__ __forceinline__ int correction(float x, float z, float s, float d, float c) {
+  const float rem = fmaf(-c, s, d), half = 0.5f * s;  // one rounding: its comparison with s / 2 is exact
+  if (rem > half) return 1;
+  if (rem < -half) return -1;
+  const bool above = rem > 0.f;  // c and, above or below it, the other neighbour are equally near d
+  const float err = difference_error(x, z, d);
+  const bool odd = (static_cast<int>(c) & 1) != 0;
+  const bool other = err != 0.f ? (err > 0.f) == above : odd;
+  return other ? (above ? 1 : -1) : 0;
 }
 
-// Eight codes, the first in the lowest bits.
+// Two fp32 values in one register pair: sm_100 adds and multiplies both with one instruction.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ Pair add(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Eight codes, the first in the lowest bits: each the integer nearest to (x - z) / s, exactly.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float z, float s) {
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, in the low bits
   constexpr uint32_t kRoundBits = 0x4B400000u;
-  const float inv = __frcp_rn(s), half = 0.5f * s;
+  float inv;  // within an ulp: what a guess lacks the remainder shows
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const float half = 0.5f * s;
+  const Pair z2 = pair_of(-z, -z), s2 = pair_of(-s, -s), inv2 = pair_of(inv, inv);
+  const Pair up = pair_of(kRound, kRound), down = pair_of(-kRound, -kRound);
   uint32_t codes = 0, bias = 0;
   bool near = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float d = x[i] - z;
-    const float t = fmaf(d, inv, kRound);
-    near |= fabsf(fmaf(kRound - t, s, d)) >= half;
-    codes += __float_as_uint(t) << (4 * i);
-    bias += kRoundBits << (4 * i);
+  for (int i = 0; i < 8; i += 2) {
+    const Pair d = add(pair_of(x[i], x[i + 1]), z2);
+    const Pair t = fma(d, inv2, up);
+    const Pair rem = fma(add(t, down), s2, d);  // d - code * s
+    float t0, t1, r0, r1;
+    split(t, t0, t1);
+    split(rem, r0, r1);
+    near |= fabsf(r0) >= half || fabsf(r1) >= half;
+    codes += (__float_as_uint(t0) << (4 * i)) + (__float_as_uint(t1) << (4 * i + 4));
+    bias += (kRoundBits << (4 * i)) + (kRoundBits << (4 * i + 4));
   }
   codes -= bias;
   if (near && s > 0.f) {
-    codes = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) codes |= exact_code(x[i], z, s) << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+      const float d = x[i] - z, c = static_cast<float>((codes >> (4 * i)) & 15u);
+      if (fabsf(fmaf(-c, s, d)) >= half) codes += static_cast<uint32_t>(correction(x[i], z, s, d, c)) << (4 * i);
+    }
   }
   return s > 0.f ? codes : 0u;
 }
-
-template <int D>
-struct Geometry {
-  static constexpr int kGroups = D / 32, kRowBytes = D / 2, kLanes = D / 8;
-  static constexpr int kRowsPerPass = 32 / kLanes;
-  static constexpr int kParams = 16 * kRowBytes;            // (s, z) pairs behind the codes
-  static constexpr int kHalf = kParams + 16 * kGroups * 4;  // keys; the values behind them
-  static constexpr int kBytes = 2 * kHalf;
-};
 
 // Eight elements as they lie in memory.
 template <typename T> struct Raw { uint4 v[sizeof(T) / 2]; };
@@ -135,61 +149,125 @@ __device__ __forceinline__ Raw<T> load_raw(const T* p) {
   return r;
 }
 
-// Calls body(tile half, first live slot, last live slot, row of slot 0 relative to the call's first
-// row, key head, keys / values) for each of the tile halves that this warp works on.
-template <int D, typename Body>
-__device__ __forceinline__ void each_half_tile(const Kv4View& v, const Kv4Seq& s, uint32_t b, Body body) {
-  const int32_t first = static_cast<int32_t>(s.len) - static_cast<int32_t>(s.n);  // position of the first row
-  if (first < 0 && threadIdx.x == 0 && blockIdx.x == 0) atomicOr(v.bad, 1u);  // rows before position 0 are skipped
-  const uint32_t tile0 = static_cast<uint32_t>(max(first, 0)) / kKv4Tile;
-  const uint32_t tiles = (s.len + kKv4Tile - 1) / kKv4Tile - tile0;
-  if (s.n == 0 || s.len == 0) return;
-  const uint32_t units = tiles * v.kv_heads * 2;
-  for (uint32_t u = blockIdx.x * kWarps + threadIdx.x / 32; u < units; u += gridDim.x * kWarps) {
-    const uint32_t which = u & 1u, th = u >> 1, t = th / v.kv_heads, h = th - t * v.kv_heads;
-    const uint32_t tile = tile0 + t, in_table = tile / v.page_tiles;
-    const uint32_t page = static_cast<uint32_t>(v.table[b * v.table_stride + in_table]);
-    if (page >= v.pages) {
-      if (threadIdx.x % 32 == 0) atomicOr(v.bad, 1u);
-      continue;
-    }
-    const int32_t pos0 = static_cast<int32_t>(tile * kKv4Tile);
-    const int32_t slot0 = max(first - pos0, 0);
-    const int32_t slot1 = min(static_cast<int32_t>(s.len) - pos0, static_cast<int32_t>(kKv4Tile)) - 1;
-    body(kv4_tile(v, page, h, tile - in_table * v.page_tiles, Geometry<D>::kBytes) + which * Geometry<D>::kHalf, slot0,
-         slot1, pos0 - first, h, which);
-  }
+// Smallest and largest of a lane's eight elements, NaN where one is NaN.
+__device__ __forceinline__ void bounds(const Raw<float>&, const float (&x)[8], float& lo, float& hi) {
+  lo = min_nan(min_nan(x[0], x[1], x[2]), min_nan(x[3], x[4], x[5]), min_nan(x[6], x[7]));
+  hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7]));
+}
+template <typename T>
+__device__ __forceinline__ void bounds(const Raw<T>& raw, const float (&)[8], float& lo, float& hi) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const T2* w = reinterpret_cast<const T2*>(raw.v);
+  const T2 l = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
+  const T2 h = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+  lo = static_cast<float>(__hmin_nan(l.x, l.y));
+  hi = static_cast<float>(__hmax_nan(h.x, h.y));
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) kv4_store_kernel(const Kv4RowArgs a) {
+template <int D>
+struct Geometry {
+  static constexpr int kGroups = D / 32, kRowBytes = D / 2, kLanes = D / 8;
+  static constexpr int kRowsPerPass = 32 / kLanes;
+  static constexpr int kStrips = 16 / (kRowsPerPass * kPasses);  // warps' shares of a tile's rows
+  static constexpr int kParams = 16 * kRowBytes;            // (s, z) pairs behind the codes
+  static constexpr int kHalf = kParams + 16 * kGroups * 4;  // keys; the values behind them
+  static constexpr int kBytes = 2 * kHalf;
+};
+
+// What one warp works on: slots slot0 .. slot1 of a tile, from slot base0 on in runs of kPasses passes
+// over its lanes; its keys and values, or one of them.
+struct Strip {
+  uint8_t* tile;
+  int32_t base0, slot0, slot1;
+  int64_t row;                 // row of slot 0 in the call's tensors (may lie before the sequence)
+  uint32_t head, which0, which1;  // key head; first of keys (0) and values (1), and the one behind the last
+};
+// Strip u of a sequence.  Whole: (tile, key head), keys and values, so that one page lookup serves 32
+// rows.  Else (tile, key head, keys or values, run of passes).
+template <int D, bool kWhole>
+__device__ __forceinline__ bool find_strip(const Kv4View& v, const Kv4Seq& s, uint32_t b, uint32_t u, Strip* p) {
+  using G = Geometry<D>;
+  const int32_t first = static_cast<int32_t>(s.len) - static_cast<int32_t>(s.n);  // position of the first row
+  const uint32_t th = kWhole ? u : u / (2 * G::kStrips);
+  const uint32_t t = th / v.kv_heads, tile = static_cast<uint32_t>(max(first, 0)) / kKv4Tile + t;
+  const int32_t pos0 = static_cast<int32_t>(tile * kKv4Tile);
+  p->head = th - t * v.kv_heads;
+  constexpr int32_t kSlots = kWhole ? 16 : 16 / G::kStrips;
+  const int32_t begin = kWhole ? 0 : static_cast<int32_t>(u % G::kStrips) * kSlots;
+  p->which0 = kWhole ? 0 : u / G::kStrips % 2;
+  p->which1 = kWhole ? 2 : p->which0 + 1;
+  p->slot0 = max(first - pos0, begin);
+  p->slot1 = min(static_cast<int32_t>(s.len) - pos0, begin + kSlots) - 1;
+  if (p->slot0 > p->slot1) return false;
+  p->base0 = p->slot0 / (kPasses * G::kRowsPerPass) * (kPasses * G::kRowsPerPass);
+  const uint32_t in_table = tile / v.page_tiles;
+  const uint32_t page = static_cast<uint32_t>(v.table[b * v.table_stride + in_table]);
+  if (page >= v.pages) {
+    if (threadIdx.x % 32 == 0) atomicOr(v.bad, 1u);
+    return false;
+  }
+  p->tile = kv4_tile(v, page, p->head, tile - in_table * v.page_tiles, G::kBytes);
+  p->row = static_cast<int64_t>(s.row0) + pos0 - first;
+  return true;
+}
+// Strips of a sequence; reports rows before position 0, which none covers.
+template <int D, bool kWhole>
+__device__ __forceinline__ uint32_t strips_of(const Kv4View& v, const Kv4Seq& s) {
+  if (s.n > s.len && threadIdx.x == 0 && blockIdx.x == 0) atomicOr(v.bad, 1u);
+  if (s.n == 0 || s.len == 0) return 0;
+  const uint32_t tile0 = (s.n > s.len ? 0u : s.len - s.n) / kKv4Tile;
+  return ((s.len + kKv4Tile - 1) / kKv4Tile - tile0) * v.kv_heads * (kWhole ? 1 : 2 * Geometry<D>::kStrips);
+}
+
+// Runs of passes of a strip: keys first, then values.
+template <int D>
+struct Runs {
+  static constexpr int kRun = kPasses * Geometry<D>::kRowsPerPass;
+  int32_t per, count;  // of one half; of all
+  __device__ __forceinline__ explicit Runs(const Strip& r)
+      : per((r.slot1 - r.base0) / kRun + 1), count(per * static_cast<int32_t>(r.which1 - r.which0)) {}
+  __device__ __forceinline__ uint32_t which(const Strip& r, int32_t q) const { return r.which0 + (q >= per ? 1u : 0u); }
+  __device__ __forceinline__ int32_t base(const Strip& r, int32_t q) const { return r.base0 + (q >= per ? q - per : q) * kRun; }
+};
+
+template <typename T, int D, bool kWhole>
+__global__ void __launch_bounds__(kThreads, 8) kv4_store_kernel(const Kv4RowArgs a) {
   using G = Geometry<D>;
   Kv4Seq s;
   if (!kv4_seq(a.view, blockIdx.y, &s)) return;
   const int lane = threadIdx.x % G::kLanes, sub = threadIdx.x % 32 / G::kLanes;
   const int j = lane / 4, i4 = lane % 4;  // channels 32 j + 8 i4 .. + 7: halfwords 2 i4 and 2 i4 + 1 of group j
   const int word = (j & 1) ? ((2 * i4 + 1) * G::kGroups + j - 1) / 2 : (2 * i4 * G::kGroups + j) / 2;
-  each_half_tile<D>(a.view, s, blockIdx.y, [&](uint8_t* half, int32_t slot0, int32_t slot1, int32_t row0, uint32_t h,
-                                               uint32_t which) {
-    const T* in = static_cast<const T*>(a.rows[which]) + h * a.head_stride[which] + 8 * lane;
-    for (int32_t base = slot0 / G::kRowsPerPass * G::kRowsPerPass; base <= slot1; base += kPasses * G::kRowsPerPass) {
-      Raw<T> raw[kPasses];
+  const uint32_t units = strips_of<D, kWhole>(a.view, s);
+  for (uint32_t u = blockIdx.x * kWarps + threadIdx.x / 32; u < units; u += gridDim.x * kWarps) {
+    Strip r;
+    if (!find_strip<D, kWhole>(a.view, s, blockIdx.y, u, &r)) continue;
+    const Runs<D> runs(r);
+    auto fetch = [&](int32_t q, Raw<T>(&raw)[kPasses]) {
+      const uint32_t which = runs.which(r, q);
+      const int32_t base = runs.base(r, q);
+      const int64_t stride = static_cast<int64_t>(a.token_stride[which]);
+      const T* in = static_cast<const T*>(a.rows[which]) + r.head * a.head_stride[which] + 8 * lane + (r.row + base + sub) * stride;
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
         const int32_t slot = base + p * G::kRowsPerPass + sub;
-        if (slot >= slot0 && slot <= slot1)
-          raw[p] = load_raw(in + (s.row0 + static_cast<uint64_t>(static_cast<int64_t>(row0 + slot))) * a.token_stride[which]);
-        else
-          raw[p] = Raw<T>{};
+        raw[p] = slot >= r.slot0 && slot <= r.slot1 ? load_raw(in + p * G::kRowsPerPass * stride) : Raw<T>{};
       }
+    };
+#pragma unroll 1
+    for (int32_t q = 0; q < runs.count; ++q) {
+      Raw<T> raw[kPasses];
+      fetch(q, raw);
+      uint8_t* const half = r.tile + runs.which(r, q) * G::kHalf;
+      const int32_t base = runs.base(r, q);
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
-        const int32_t slot = base + p * G::kRowsPerPass + sub;
-        if (base + p * G::kRowsPerPass > slot1) break;
+        const int32_t slot0 = base + p * G::kRowsPerPass, slot = slot0 + sub;
+        if (slot0 > r.slot1 || slot0 + G::kRowsPerPass <= r.slot0) continue;  // the whole warp's
         float x[8];
         load8(reinterpret_cast<const T*>(raw[p].v), x);
-        float lo = min_nan(min_nan(x[0], x[1], x[2]), min_nan(x[3], x[4], x[5]), min_nan(x[6], x[7]));
-        float hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7]));
+        float lo, hi;
+        bounds(raw[p], x, lo, hi);
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
           lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -204,66 +282,91 @@ __global__ void __launch_bounds__(kThreads) kv4_store_kernel(const Kv4RowArgs a)
         const __half2 sz = group_params(lo, hi);
         const uint32_t codes = codes_of(x, __high2float(sz), __low2float(sz));
         const uint32_t other = __shfl_xor_sync(0xffffffffu, (j & 1) ? codes & 0xffffu : codes >> 16, 4);
-        if (slot < slot0 || slot > slot1) continue;
+        if (slot < r.slot0 || slot > r.slot1) continue;
         reinterpret_cast<uint32_t*>(half + slot * G::kRowBytes)[word] =
             (j & 1) ? other | (codes & 0xffff0000u) : (codes & 0xffffu) | (other << 16);
         if (i4 == 0) reinterpret_cast<__half2*>(half + G::kParams)[slot * G::kGroups + j] = sz;
       }
     }
-  });
+  }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) kv4_load_kernel(const Kv4RowArgs a) {
+template <typename T, int D, bool kWhole>
+__global__ void __launch_bounds__(kThreads, 12) kv4_load_kernel(const Kv4RowArgs a) {
   using G = Geometry<D>;
   Kv4Seq s;
   if (!kv4_seq(a.view, blockIdx.y, &s)) return;
   const int lane = threadIdx.x % G::kLanes, sub = threadIdx.x % 32 / G::kLanes;
   const int j = lane / 4, i4 = lane % 4;
   const int word = (j & 1) ? ((2 * i4 + 1) * G::kGroups + j - 1) / 2 : (2 * i4 * G::kGroups + j) / 2;
-  each_half_tile<D>(a.view, s, blockIdx.y, [&](const uint8_t* half, int32_t slot0, int32_t slot1, int32_t row0,
-                                               uint32_t h, uint32_t which) {
-    T* out = static_cast<T*>(a.rows[which]) + h * a.head_stride[which] + 8 * lane;
-    for (int32_t base = slot0 / G::kRowsPerPass * G::kRowsPerPass; base <= slot1; base += kPasses * G::kRowsPerPass) {
-      uint32_t words[kPasses], params[kPasses];
+  const uint32_t units = strips_of<D, kWhole>(a.view, s);
+  for (uint32_t u = blockIdx.x * kWarps + threadIdx.x / 32; u < units; u += gridDim.x * kWarps) {
+    Strip r;
+    if (!find_strip<D, kWhole>(a.view, s, blockIdx.y, u, &r)) continue;
+    const Runs<D> runs(r);
+    auto fetch = [&](int32_t q, uint32_t(&words)[kPasses], uint32_t(&params)[kPasses]) {
+      const uint8_t* const half = r.tile + runs.which(r, q) * G::kHalf;
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
-        const int32_t slot = min(base + p * G::kRowsPerPass + sub, static_cast<int32_t>(kKv4Tile) - 1);
+        const int32_t slot = runs.base(r, q) + p * G::kRowsPerPass + sub;  // inside the tile, whether live or not
         words[p] = reinterpret_cast<const uint32_t*>(half + slot * G::kRowBytes)[word];
         params[p] = reinterpret_cast<const uint32_t*>(half + G::kParams)[slot * G::kGroups + j];
       }
+    };
+#pragma unroll 1
+    for (int32_t q = 0; q < runs.count; ++q) {
+      uint32_t words[kPasses], params[kPasses];
+      fetch(q, words, params);
+      const uint32_t which = runs.which(r, q);
+      const int32_t base = runs.base(r, q);
+      const int64_t stride = static_cast<int64_t>(a.token_stride[which]);
+      T* out = static_cast<T*>(a.rows[which]) + r.head * a.head_stride[which] + 8 * lane + (r.row + base + sub) * stride;
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
         const int32_t slot = base + p * G::kRowsPerPass + sub;
         const uint32_t other = __shfl_xor_sync(0xffffffffu, (j & 1) ? words[p] & 0xffffu : words[p] >> 16, 4);
         const uint32_t codes = (j & 1) ? other | (words[p] & 0xffff0000u) : (words[p] & 0xffffu) | (other << 16);
-        if (slot < slot0 || slot > slot1) continue;
+        if (slot < r.slot0 || slot > r.slot1) continue;
         const float2 sz = __half22float2(*reinterpret_cast<const __half2*>(&params[p]));
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; i += 2) {
           // 2^23 + code by its bits: exact, and no conversion instruction
-          const float c = __uint_as_float(((codes >> (4 * i)) & 15u) | 0x4B000000u) - 8388608.f;
-          x[i] = fmaf(c, sz.x, sz.y);
-          // z + 15 s may lie a step behind a clamped row's 65504: no finite row reads back as infinite
-          if constexpr (std::is_same<T, __half>::value) x[i] = min_nan(max_nan(x[i], -kF16Max), kF16Max);
+          const Pair c = add(pair_of(__uint_as_float(((codes >> (4 * i)) & 15u) | 0x4B000000u),
+                                     __uint_as_float(((codes >> (4 * i + 4)) & 15u) | 0x4B000000u)),
+                             pair_of(-8388608.f, -8388608.f));
+          split(fma(c, pair_of(sz.x, sz.x), pair_of(sz.y, sz.y)), x[i], x[i + 1]);
         }
-        store8(out + (s.row0 + static_cast<uint64_t>(static_cast<int64_t>(row0 + slot))) * a.token_stride[which], x);
+        if constexpr (std::is_same<T, __half>::value) {
+          // z + 15 s may lie a step behind a clamped row's 65504: no finite row reads back as infinite
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = min_nan(max_nan(x[i], -kF16Max), kF16Max);
+        }
+        store8(out + p * G::kRowsPerPass * stride, x);
       }
     }
-  });
+  }
 }
 
 template <typename T, int D>
 cudaError_t launch(const Kv4RowArgs& a, bool store, cudaStream_t stream) {
   // a sequence's rows may start and end inside a tile
   const uint64_t tiles = (static_cast<uint64_t>(a.view.max_tokens) + 2 * (kKv4Tile - 1)) / kKv4Tile;
-  const uint64_t blocks = (tiles * a.view.kv_heads * 2 + kWarps - 1) / kWarps;
+  // A warp takes a whole tile of a head where that fills the SMs (one page lookup for 32 rows), else one
+  // run of passes of its keys or values, so that a few tiles' rows are in flight at once (8.0 us against
+  // 11.3 to store 8192 rows of 256).
+  const uint64_t whole = tiles * a.view.kv_heads;
+  const bool fills = whole * a.view.batch >= 148ull * 32;
+  const uint64_t blocks = ((fills ? whole : whole * 2 * Geometry<D>::kStrips) + kWarps - 1) / kWarps;
   const dim3 grid(static_cast<uint32_t>(blocks < 65536 ? blocks : 65536), a.view.batch);
-  if (store)
-    kv4_store_kernel<T, D><<<grid, kThreads, 0, stream>>>(a);
+  if (store && fills)
+    kv4_store_kernel<T, D, true><<<grid, kThreads, 0, stream>>>(a);
+  else if (store)
+    kv4_store_kernel<T, D, false><<<grid, kThreads, 0, stream>>>(a);
+  else if (fills)
+    kv4_load_kernel<T, D, true><<<grid, kThreads, 0, stream>>>(a);
   else
-    kv4_load_kernel<T, D><<<grid, kThreads, 0, stream>>>(a);
+    kv4_load_kernel<T, D, false><<<grid, kThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from dataclasses import dataclass
 from pathlib import Path
 from typing import Optional
@@ -1228,6 +1229,12 @@ class Runtime:
             raise RuntimeError(f"device attention rc={rc} detail={detail.value}")
 
     # -- token-by-token serving (torch tensors on the handle's GPU)
+    def _serving(self) -> "_ServingCalls":
+        calls = getattr(self.lib, "_oct_serving", None)
+        if calls is None:
+            calls = self.lib._oct_serving = _ServingCalls(self.lib)
+        return calls
+
     def qk_norm_rope_device(self, q, k, q_out, k_out, positions, frequencies, *, axis_pairs=None,
                             interleaved: bool = False, normalize: bool = True, q_weight=None, k_weight=None,
                             eps: float = 1e-6, stream=None) -> None:
@@ -1256,12 +1263,12 @@ class Runtime:
             k_rows, ko_rows = _rows(k, "k", q.dtype, k_shape), _rows(k_out, "k_out", q.dtype, k_shape)
         q_rows, qo_rows = _rows(q, "q", q.dtype, shape), _rows(q_out, "q_out", q.dtype, shape)
         detail = C.c_int()
-        rc = self.lib.oct_b200_qk_norm_rope_device(self.handle, OctB200QkNormRopeRequest(
+        rc = self._serving().rope(self.handle, _ROPE.pack(
             _SIZEOF_ROPE, dtype, tokens, heads, k_heads, dim, 2 * pairs, interleaved, normalize, eps, axes,
-            tuple(axis_pairs), q_rows[0], k_rows[0], qo_rows[0], ko_rows[0], q_rows[1], q_rows[2], k_rows[1], k_rows[2],
-            qo_rows[1], qo_rows[2], ko_rows[1], ko_rows[2], _vector(q_weight, "q_weight", "f32", dim),
-            _vector(k_weight, "k_weight", "f32", dim), positions.data_ptr(), positions.stride(0),
-            _vector(frequencies, "frequencies", "f64", pairs)), _stream_ptr(stream), detail)
+            *axis_pairs, *_NO_PAIRS[axes:], q_rows[0], k_rows[0], qo_rows[0], ko_rows[0], q_rows[1], q_rows[2],
+            k_rows[1], k_rows[2], qo_rows[1], qo_rows[2], ko_rows[1], ko_rows[2],
+            _vector(q_weight, "q_weight", "f32", dim), _vector(k_weight, "k_weight", "f32", dim), positions.data_ptr(),
+            positions.stride(0), _vector(frequencies, "frequencies", "f64", pairs)), _stream_ptr(stream), detail)
         if rc != PROM_OK:
             raise RuntimeError(f"device qk norm rope rc={rc} detail={detail.value}")
 
@@ -1272,8 +1279,8 @@ class Runtime:
         k_ptr, k_token, k_head = _rows(k, "k", k.dtype, shape)
         v_ptr, v_token, v_head = _rows(v, "v", k.dtype, shape)
         detail = C.c_int()
-        rc = fn(self.handle, cache.desc, batch.desc,
-                OctB200Kv4Rows(_SIZEOF_ROWS, dtype, tokens, k_ptr, v_ptr, k_token, k_head, v_token, v_head),
+        rc = fn(self.handle, cache.address, batch.address,
+                _ROWS.pack(_SIZEOF_ROWS, dtype, tokens, k_ptr, v_ptr, k_token, k_head, v_token, v_head),
                 _stream_ptr(stream), detail)
         if rc != PROM_OK:
             raise RuntimeError(f"device kv4 rows rc={rc} detail={detail.value}")
@@ -1281,11 +1288,11 @@ class Runtime:
     def kv4_store_device(self, cache: "Kv4Cache", batch: "Kv4Batch", k, v, stream=None) -> None:
         """Quantises rows k, v [tokens][kv_heads][head_dim] (fp32, bf16, fp16) into the cache, as the last
         tokens of the batch's sequences."""
-        self._kv4_rows(self.lib.oct_b200_kv4_store_device, cache, batch, k, v, stream)
+        self._kv4_rows(self._serving().store, cache, batch, k, v, stream)
 
     def kv4_load_device(self, cache: "Kv4Cache", batch: "Kv4Batch", k, v, stream=None) -> None:
         """Reads the rows that the same batch would store back into k, v."""
-        self._kv4_rows(self.lib.oct_b200_kv4_load_device, cache, batch, k, v, stream)
+        self._kv4_rows(self._serving().load, cache, batch, k, v, stream)
 
     def kv4_attention_workspace_bytes(self, cache: "Kv4Cache", batch: "Kv4Batch", q, *, causal: bool = True,
                                       window: int = 0) -> int:
@@ -1314,12 +1321,12 @@ class Runtime:
             ws_bytes = workspace.numel()
             ws_ptr = _vector(workspace, "workspace", "u8", ws_bytes)
         detail = C.c_int()
-        rc = self.lib.oct_b200_kv4_attention_device(
-            self.handle, cache.desc, batch.desc,
-            OctB200Kv4AttentionRequest(_SIZEOF_ATTENTION, dtype, heads, causal, window,
-                                       cache.default_scale if scale is None else scale, tokens, q_ptr, out_ptr, q_token,
-                                       q_head, out_token, out_head, _vector(lse, "lse", "f32", tokens * heads), ws_ptr,
-                                       ws_bytes), _stream_ptr(stream), detail)
+        rc = self._serving().attention(
+            self.handle, cache.address, batch.address,
+            _ATTENTION.pack(_SIZEOF_ATTENTION, dtype, heads, causal, window,
+                            cache.default_scale if scale is None else scale, tokens, q_ptr, out_ptr, q_token, q_head,
+                            out_token, out_head, _vector(lse, "lse", "f32", tokens * heads), ws_ptr, ws_bytes),
+            _stream_ptr(stream), detail)
         if rc != PROM_OK:
             raise RuntimeError(f"device kv4 attention rc={rc} detail={detail.value}")
 
@@ -1368,9 +1375,29 @@ def nccl_unique_id(lib) -> bytes:
     return bytes(buf)
 
 
+# The serving calls are short, so their requests are packed in one go instead of field by field, and the
+# entry points are bound a second time with plain addresses as arguments.
+_ROPE = struct.Struct("@IIQIIIIIIfI4I4P8Q3PQP")
+_ROWS = struct.Struct("@IIQ2P4Q")
+_ATTENTION = struct.Struct("@IIIIIfQ2P4Q2PQ")
 _SIZEOF_ROPE, _SIZEOF_ROWS, _SIZEOF_ATTENTION = (
     C.sizeof(OctB200QkNormRopeRequest), C.sizeof(OctB200Kv4Rows), C.sizeof(OctB200Kv4AttentionRequest))
-_NO_ROWS = (0, 0, 0)
+assert (_ROPE.size, _ROWS.size, _ATTENTION.size) == (_SIZEOF_ROPE, _SIZEOF_ROWS, _SIZEOF_ATTENTION)
+
+
+class _ServingCalls:
+    def __init__(self, lib):
+        def bind(name: str, args: int):
+            fn = lib["oct_b200_" + name]  # a function object of its own
+            fn.restype, fn.argtypes = C.c_int, [C.c_void_p] * args + [_i32p]
+            return fn
+
+        self.rope, self.store, self.load = bind("qk_norm_rope_device", 3), bind("kv4_store_device", 5), bind(
+            "kv4_load_device", 5)
+        self.attention = bind("kv4_attention_device", 5)
+
+
+_NO_ROWS, _NO_PAIRS = (0, 0, 0), (0, 0, 0, 0)
 _TORCH_TYPES: dict = {}  # the torch dtypes of the serving calls, once such a call has been made
 
 
@@ -1435,6 +1462,7 @@ class Kv4Cache:
         self.default_scale = float(np.float32(1.0) / np.sqrt(np.float32(head_dim)))
         self.desc = OctB200Kv4Cache(C.sizeof(OctB200Kv4Cache), page_size, kv_heads, head_dim, self.pages, 0,
                                     data.data_ptr())
+        self.address = C.addressof(self.desc)
 
 
 class Kv4Batch:
@@ -1463,6 +1491,7 @@ class Kv4Batch:
         self.desc = OctB200Kv4Batch(C.sizeof(OctB200Kv4Batch), batch, page_table.data_ptr(), page_table.stride(0),
                                     page_table.shape[1], max_tokens, max_kv_len, 0, kv_lens.data_ptr(),
                                     cu_tokens.data_ptr() if cu_tokens is not None else None)
+        self.address = C.addressof(self.desc)
 
 
 class Block:

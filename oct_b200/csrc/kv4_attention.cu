@@ -35,6 +35,7 @@
 // Blocks take equal runs of the call's tiles, whatever the sequences' lengths:
 // each adds up the lengths on the device and finds its own run.  An item that
 // a run's end cuts leaves partial results, which a second kernel joins in order.
+#include <atomic>
 #include <type_traits>
 
 #include "kernels.h"
@@ -1029,8 +1030,17 @@ cudaError_t launch(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream
   constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
   constexpr size_t kSmem = static_cast<size_t>(kWarps) * G::kStages * G::kBytes;
   const auto kernel = kv4_attention_kernel<T, D, NT, QP, PP>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
+  // the attribute stays with the device's function: set once on each
+  static std::atomic<uint64_t> set{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device > 63 || (set.load(std::memory_order_acquire) & bit) == 0) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
+    if (e != cudaSuccess) return e;
+    set.fetch_or(bit, std::memory_order_release);
+  }
   kernel<<<plan.blocks, kThreads, kSmem, stream>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess || plan.workspace == 0) return e;

@@ -86,25 +86,6 @@ __device__ __forceinline__ int correction(float x, float z, float s, float d, fl
   return other ? (above ? 1 : -1) : 0;
 }
 
-// Two fp32 values in one register pair: sm_100 adds and multiplies both with one instruction.
-typedef unsigned long long Pair;
-__device__ __forceinline__ Pair pair_of(float a, float b) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void split(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
-__device__ __forceinline__ Pair add(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // Eight codes, the first in the lowest bits: each the integer nearest to (x - z) / s, exactly.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float z, float s) {
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, in the low bits

@@ -13,10 +13,12 @@
 //
 // Bound: HBM, each element read and written once.  A row is spread over dim/16
 // lanes, each with the two 8-element vectors that hold both halves of its eight
-// pairs, so a rotation needs no exchange between lanes.  A thread keeps its row
-// (head) and channels while it goes through a block's tokens: the weight stays in
-// registers, the loads of the next tokens are on their way, and the tokens'
-// cosines and sines, computed once per block into shared memory, serve all heads.
+// pairs, so a rotation needs no exchange between lanes; first and second elements
+// of two neighbouring pairs share a register pair, and every step works on both
+// at once.  A thread keeps its row (head) and channels while it goes through a
+// block's tokens: the weight stays in registers, the loads of the next tokens are
+// on their way, and the tokens' cosines and sines, computed once per block into
+// shared memory, serve all heads.
 //
 // Angles: position * frequency is reduced to a fraction of a turn in binary64
 // before the fp32 sine and cosine, because a far position loses every digit of
@@ -27,7 +29,9 @@ namespace oct {
 namespace {
 
 constexpr uint32_t kMaxThreads = 256;
-constexpr int kInFlight = 4;              // tokens whose loads are issued together
+// Tokens whose loads are on their way at a time: 128 bytes a lane (16-bit types 45 us with two tokens, 41
+// with four, for 2 x 4096 x 48 rows of 128; fp32 14.4 with two, 16.5 with four, for 4096 x 9 rows of 256).
+template <typename T> constexpr int kTokensInFlight = sizeof(T) == 4 ? 2 : 4;
 constexpr uint32_t kMaxBlockTokens = 16;
 
 template <typename T> struct Raw { uint4 v[sizeof(T)]; };  // two vectors of eight elements
@@ -42,14 +46,46 @@ __device__ __forceinline__ Raw<T> load_raw(const T* a, const T* b) {
   }
   return r;
 }
+// The two vectors' sixteen elements as first and second elements of eight pairs: half-split, element i
+// of either vector; interleaved, elements 2 i and 2 i + 1 of both in a row.
+template <typename E>
+__device__ __forceinline__ void to_pairs(const E (&e)[16], bool interleaved, E (&x)[8], E (&y)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = interleaved ? e[2 * i] : e[i];
+    y[i] = interleaved ? e[2 * i + 1] : e[8 + i];
+  }
+}
+__device__ __forceinline__ void as_pairs(const float (&x)[8], Pair (&p)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = pair_of(x[2 * i], x[2 * i + 1]);
+}
 
 // Grid x: runs of block_tokens tokens; y: runs of the rows (query heads, then key heads) of a token.
-template <typename T, int LANES>
+template <typename T, int LANES, bool kInterleaved>
 __global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_kernel(const QkNormRopeArgs a, uint32_t block_tokens) {
-  extern __shared__ float2 turns[];  // [block_tokens][8][rotary / 16] (cos, sin) of pair 8 lane + i at [i][lane]
-  const uint32_t pairs = a.rotary / 2, strip = pairs / 8;
+  constexpr int kInFlight = kTokensInFlight<T>;
+  extern __shared__ float2 turns[];  // [block_tokens][cos, sin][4][rotary / 16]: pairs 2 i and 2 i + 1 of a lane
+  const uint32_t pairs = a.rotary / 2, strip = a.rotary / 16;
   const uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * block_tokens;
   const uint32_t nt = static_cast<uint32_t>(min(static_cast<uint64_t>(block_tokens), a.tokens - t0));
+
+  const uint32_t lane = threadIdx.x % LANES, r = blockIdx.y * (blockDim.x / LANES) + threadIdx.x / LANES;
+  const uint32_t which = r < a.heads[0] ? 0 : 1, h = which == 0 ? r : r - a.heads[0];
+  const bool live = lane < a.dim / 16 && r < a.heads[0] + a.heads[1];
+  const bool rotates = lane < strip;
+  const uint32_t ca = kInterleaved || !rotates ? 16 * lane : 8 * lane;
+  const uint32_t cb = kInterleaved || !rotates ? 16 * lane + 8 : a.rotary / 2 + 8 * lane;
+  const uint64_t in_step = a.in_token[which], out_step = a.out_token[which];
+  const T* in = live ? static_cast<const T*>(a.in[which]) + t0 * in_step + h * a.in_head[which] : nullptr;
+  T* out = live ? static_cast<T*>(a.out[which]) + t0 * out_step + h * a.out_head[which] : nullptr;
+  Raw<T> raw[kInFlight];
+#pragma unroll
+  for (int i = 0; i < kInFlight; ++i) {
+    raw[i] = live && i < static_cast<int>(nt) ? load_raw(in + ca, in + cb) : Raw<T>{};
+    in += in_step;
+  }
+  // the table, while the first rows are on their way
   for (uint32_t e = threadIdx.x; e < nt * pairs; e += blockDim.x) {
     const uint32_t t = e / pairs, j = e - t * pairs;
     uint32_t axis = 0, end = a.axis_pairs[0];
@@ -59,82 +95,91 @@ __global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_kernel(const QkNormR
     const float f = static_cast<float>(turn - rint(turn));
     float s, c;
     sincospif(2.0f * f, &s, &c);
-    turns[t * pairs + (j % 8) * strip + j / 8] = make_float2(c, s);
+    float* to = reinterpret_cast<float*>(turns + t * pairs + j % 8 / 2 * strip + j / 8) + j % 2;
+    to[0] = c;
+    to[2 * 4 * strip] = s;
   }
-
-  const uint32_t lane = threadIdx.x % LANES, r = blockIdx.y * (blockDim.x / LANES) + threadIdx.x / LANES;
-  const uint32_t which = r < a.heads[0] ? 0 : 1, h = which == 0 ? r : r - a.heads[0];
-  const bool live = lane < a.dim / 16 && r < a.heads[0] + a.heads[1];
-  // this lane's two vectors of eight channels
-  const bool rotates = lane < a.rotary / 16;
-  const uint32_t ca = a.interleaved || !rotates ? 16 * lane : 8 * lane;
-  const uint32_t cb = a.interleaved || !rotates ? 16 * lane + 8 : a.rotary / 2 + 8 * lane;
-  const T* in = live ? static_cast<const T*>(a.in[which]) + t0 * a.in_token[which] + h * a.in_head[which] : nullptr;
-  T* out = live ? static_cast<T*>(a.out[which]) + t0 * a.out_token[which] + h * a.out_head[which] : nullptr;
-  float wa[8], wb[8];
-  if (live && a.weight[which] != nullptr) {
-    load8(a.weight[which] + ca, wa);
-    load8(a.weight[which] + cb, wb);
-  } else {
+  Pair wx[4], wy[4];
+  {
+    float e[16], x[8], y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) wa[i] = wb[i] = 1.f;
+    for (int i = 0; i < 16; ++i) e[i] = 1.f;
+    if (live && a.weight[which] != nullptr) {
+      float va[8], vb[8];
+      load8(a.weight[which] + ca, va);
+      load8(a.weight[which] + cb, vb);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = va[i], e[8 + i] = vb[i];
+    }
+    to_pairs(e, kInterleaved, x, y);
+    as_pairs(x, wx);
+    as_pairs(y, wy);
   }
+  const float mean = 1.0f / static_cast<float>(a.dim);
   __syncthreads();
 #pragma unroll 1
   for (uint32_t b0 = 0; b0 < nt; b0 += kInFlight) {
-    Raw<T> raw[kInFlight];
-#pragma unroll
-    for (int i = 0; i < kInFlight; ++i) {
-      const T* p = in + (b0 + i) * a.in_token[which];
-      raw[i] = live && b0 + i < nt ? load_raw(p + ca, p + cb) : Raw<T>{};
-    }
 #pragma unroll
     for (int n = 0; n < kInFlight; ++n) {
       const uint32_t t = b0 + n;
       if (t >= nt) break;
-      float x[8], y[8];
-      load8(reinterpret_cast<const T*>(raw[n].v), x);
-      load8(reinterpret_cast<const T*>(raw[n].v + sizeof(T) / 2), y);
-      if (a.normalize) {
-        float ss = 0.f;
+      Pair x[4], y[4];
+      {
+        float va[8], vb[8], e[16], u[8], v[8];
+        load8(reinterpret_cast<const T*>(raw[n].v), va);
+        load8(reinterpret_cast<const T*>(raw[n].v + sizeof(T) / 2), vb);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
+        for (int i = 0; i < 8; ++i) e[i] = va[i], e[8 + i] = vb[i];
+        to_pairs(e, kInterleaved, u, v);
+        as_pairs(u, x);
+        as_pairs(v, y);
+      }
+      if (live && t + kInFlight < nt) raw[n] = load_raw(in + ca, in + cb);
+      in += in_step;
+      if (a.normalize) {
+        Pair sum = 0ull;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = fma(x[i], x[i], fma(y[i], y[i], sum));
+        float ss, other;
+        split(sum, ss, other);
+        ss += other;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.dim) + a.eps);
+        const float inv = rsqrtf(fmaf(ss, mean, a.eps));
+        const Pair inv2 = pair_of(inv, inv);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = x[i] * inv * wa[i];
-          y[i] = y[i] * inv * wb[i];
+        for (int i = 0; i < 4; ++i) {
+          x[i] = mul(mul(x[i], inv2), wx[i]);
+          y[i] = mul(mul(y[i], inv2), wy[i]);
         }
       }
       if (!live) continue;
       if (rotates) {
         const float2* cs = turns + t * pairs + lane;
-        if (a.interleaved) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 u = cs[i * strip], v = cs[(4 + i) * strip];
-            const float p = x[2 * i], q = x[2 * i + 1];
-            x[2 * i] = p * u.x - q * u.y;
-            x[2 * i + 1] = q * u.x + p * u.y;
-            const float m = y[2 * i], n2 = y[2 * i + 1];
-            y[2 * i] = m * v.x - n2 * v.y;
-            y[2 * i + 1] = n2 * v.x + m * v.y;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 u = cs[i * strip];
-            const float p = x[i], q = y[i];
-            x[i] = p * u.x - q * u.y;
-            y[i] = q * u.x + p * u.y;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float2 c = cs[i * strip], s = cs[(4 + i) * strip];
+          const Pair c2 = pair_of(c.x, c.y), s2 = pair_of(s.x, s.y), n2 = pair_of(-s.x, -s.y);
+          const Pair u = fma(x[i], c2, mul(y[i], n2));
+          y[i] = fma(y[i], c2, mul(x[i], s2));
+          x[i] = u;
         }
       }
-      T* o = out + t * a.out_token[which];
-      store8(o + ca, x);
-      store8(o + cb, y);
+      float va[8], vb[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x0, x1, y0, y1;
+        split(x[i], x0, x1);
+        split(y[i], y0, y1);
+        if constexpr (kInterleaved) {
+          float(&to)[8] = i < 2 ? va : vb;
+          to[4 * (i % 2)] = x0, to[4 * (i % 2) + 1] = y0, to[4 * (i % 2) + 2] = x1, to[4 * (i % 2) + 3] = y1;
+        } else {
+          va[2 * i] = x0, va[2 * i + 1] = x1, vb[2 * i] = y0, vb[2 * i + 1] = y1;
+        }
+      }
+      store8(out + t * out_step + ca, va);
+      store8(out + t * out_step + cb, vb);
     }
   }
 }
@@ -151,7 +196,11 @@ cudaError_t launch(const QkNormRopeArgs& a, cudaStream_t stream) {
   const uint32_t bt = static_cast<uint32_t>(share < 1 ? 1 : (share > kMaxBlockTokens ? kMaxBlockTokens : share));
   const uint64_t blocks = (a.tokens + bt - 1) / bt;
   const size_t smem = static_cast<size_t>(bt) * (a.rotary / 2) * sizeof(float2);
-  qk_norm_rope_kernel<T, LANES><<<dim3(static_cast<uint32_t>(blocks), row_runs), threads, smem, stream>>>(a, bt);
+  const dim3 grid(static_cast<uint32_t>(blocks), row_runs);
+  if (a.interleaved)
+    qk_norm_rope_kernel<T, LANES, true><<<grid, threads, smem, stream>>>(a, bt);
+  else
+    qk_norm_rope_kernel<T, LANES, false><<<grid, threads, smem, stream>>>(a, bt);
   return cudaGetLastError();
 }
 

@@ -66,6 +66,30 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v.x, v.y, T()), pack2(v.z, v.w, T()));
 }
 
+// Two fp32 values in one register pair: sm_100 adds and multiplies both with one instruction.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ Pair add(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Pair mul(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // What sequence `b` of a call brings and holds.  False, with *bad set, when the
 // arrays on the device do not fit the bounds that the host was given: such a
 // sequence is skipped and nothing of it is read or written.

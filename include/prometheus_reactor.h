@@ -1627,7 +1627,7 @@ typedef struct OctB200Kv4Rows {
   void *k, *v; /* read by the store, written by the load */
   uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
 } OctB200Kv4Rows;
-/* Quantises the rows into the cache / reads the same positions back. */
+/* Quantises the rows into the cache / reads the same positions back (k and v apart). */
 PROM_REACTOR_API int oct_b200_kv4_store_device(void* handle, const OctB200Kv4Cache* cache,
                                                const OctB200Kv4Batch* batch, const OctB200Kv4Rows* rows,
                                                void* stream, int* out_detail_code);
@@ -1640,7 +1640,8 @@ PROM_REACTOR_API int oct_b200_kv4_load_device(void* handle, const OctB200Kv4Cach
    h / (q_heads / kv_heads).  With causal, the query at position p sees keys <= p
    and, with a window, keys > p - window; without, every key of its sequence.  A
    query that sees nothing gets zeros and lse = -inf.  lse (may be NULL) is the
-   natural logarithm of the softmax's sum, [tokens][q_heads].  The workspace
+   natural logarithm of the softmax's sum, [tokens][q_heads].  out may be q itself
+   (same strides) and overlap no other part of it.  The workspace
    (oct_b200_kv4_attention_workspace_bytes of the same sizes; NULL when that is
    0) is used between this call's kernels only: calls that may run at the same
    time, graphs too, need one each.  Meant for the few tokens of a decode or

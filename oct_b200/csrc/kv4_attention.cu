@@ -78,7 +78,7 @@ template <int D> constexpr int kMaxRowGroups = D == 64 ? 4 : (D == 128 ? 2 : 1);
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -94,7 +94,7 @@ __device__ __forceinline__ uint32_t centred(uint32_t codes, uint32_t middle) {
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 // 8 x 8 matrices of 16-bit elements from shared memory, transposed: lanes 8 m .. 8 m + 7 name the rows of matrix m.
@@ -271,7 +271,8 @@ __device__ __forceinline__ bool find_share(const KernelArgs& a, uint32_t rows_pe
   total *= a.view.kv_heads;
   all_items *= a.view.kv_heads;
   const bool few = total <= 4 * gridDim.x && all_items <= gridDim.x / 2;
-  out->cost = few ? 0 : kItemCost;
+  // without a workspace every item is one unit and stays whole: no cost may be cut off it
+  out->cost = few || a.part_o == nullptr ? 0 : kItemCost;
   const uint32_t run = total + out->cost * all_items, blocks = few ? gridDim.x - all_items : gridDim.x;
   out->per = max(1u, (run + blocks - 1) / blocks);
   out->pad = few ? out->per : 1;
@@ -884,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     const uint32_t first_row = rows.first, count = rows.count;
     const bool whole = item.take == item.size;
     const uint32_t slot = blockIdx.x * 2 + (item.offset == 0 ? 1u : 0u);
-    if (!whole && item.offset == 0 && threadIdx.x == 0) {
+    if (!whole && item.offset == 0 && threadIdx.x == 0 && a.part_o != nullptr) {
       const uint32_t last = (unit + item.size - 1) / share.per;
       a.part_of[blockIdx.x] = PartOf{min(last, gridDim.x - 1) + 1, head, first_row, count, row0};
     }
@@ -925,7 +926,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
                make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
         if (c4 == 0 && a.lse != nullptr)
           a.lse[token * a.heads + qh] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
-      } else {
+      } else if (a.part_o != nullptr) {
         const uint64_t at = static_cast<uint64_t>(slot) * kRows + col;
         *reinterpret_cast<float4*>(a.part_o + at * D + 4 * c4) = sum;
         if (c4 == 0) a.part_ml[at] = make_float2(top, total);

@@ -139,6 +139,7 @@ int run_rows(void* handle, const OctB200Kv4Cache* cache, const OctB200Kv4Batch* 
         bad = check_rows(rows->v, rows->tokens, cache->kv_heads, cache->head_dim, rows->v_token_stride,
                          rows->v_head_stride, vec, !store);
     }
+    if (any && bad == 0 && !store && rows->k == rows->v) bad = OCT_B200_DETAIL_INVALID_ARGUMENT;
     if (bad != 0) return fail(out_detail_code, bad);
     if (!rt->available) return fail(out_detail_code, PROM_DETAIL_CAPABILITY_MISMATCH);
     if (!any) return PROM_OK;
@@ -235,6 +236,7 @@ int oct_b200_qk_norm_rope_device(void* handle, const OctB200QkNormRopeRequest* r
         if (bad == 0 && a.in[i] == a.out[i] &&
             ((r->tokens > 1 && a.in_token[i] != a.out_token[i]) || (a.heads[i] > 1 && a.in_head[i] != a.out_head[i])))
           bad = OCT_B200_DETAIL_INVALID_ARGUMENT;
+        if (bad == 0 && a.heads[0] > 0 && a.heads[1] > 0 && a.out[0] == a.out[1]) bad = OCT_B200_DETAIL_INVALID_ARGUMENT;
         if (bad != 0) return fail(out_detail_code, bad);
       }
     }

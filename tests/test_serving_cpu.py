@@ -51,7 +51,7 @@ def _rope(**kw):
     r = R.OctB200QkNormRopeRequest()
     base = dict(struct_size=C.sizeof(r), dtype=R.DTYPE_BF16, tokens=3, q_heads=4, k_heads=2, head_dim=128, rotary_dim=96,
                 interleaved=0, normalize=1, eps=1e-6, axes=2, axis_pairs=(C.c_uint32 * 4)(16, 32), q=P, k=P, q_out=P,
-                k_out=P, q_token_stride=512, q_head_stride=128, k_token_stride=256, k_head_stride=128,
+                k_out=3 * P, q_token_stride=512, q_head_stride=128, k_token_stride=256, k_head_stride=128,
                 q_out_token_stride=512, q_out_head_stride=128, k_out_token_stride=256, k_out_head_stride=128,
                 positions=P, position_stride=2, frequencies=P)
     for name, value in (base | kw).items():
@@ -69,7 +69,7 @@ def _rope(**kw):
     (dict(q_token_stride=516), UNALIGNED), (dict(q_out=2 * P, q_out_token_stride=504), INVALID),
     (dict(q_out=2 * P, q_out_head_stride=64), INVALID), (dict(q_out_token_stride=128, q_out_head_stride=384), INVALID),
     (dict(q_out=2 * P, q_out_token_stride=128, q_out_head_stride=384), NO_DEVICE), (dict(q_weight=P + 4), UNALIGNED),
-    (dict(tokens=1 << 31), SHAPE), (dict(tokens=0), NO_DEVICE),
+    (dict(k_out=P), INVALID), (dict(tokens=1 << 31), SHAPE), (dict(tokens=0), NO_DEVICE),
     (dict(rotary_dim=0, axis_pairs=(C.c_uint32 * 4)(0, 0)), SHAPE),
 ])
 def test_qk_norm_rope_refusals(lib, handle, change, code):
@@ -105,7 +105,7 @@ def _batch(**kw):
 
 
 def _rows(**kw):
-    return _fill(R.OctB200Kv4Rows, dict(struct_size=C.sizeof(R.OctB200Kv4Rows), dtype=R.DTYPE_F32, tokens=7, k=P, v=P,
+    return _fill(R.OctB200Kv4Rows, dict(struct_size=C.sizeof(R.OctB200Kv4Rows), dtype=R.DTYPE_F32, tokens=7, k=P, v=2 * P,
                                         k_token_stride=256, k_head_stride=128, v_token_stride=256,
                                         v_head_stride=128), kw)
 
@@ -157,6 +157,15 @@ def test_row_refusals(lib, handle, change, code):
     detail = C.c_int()
     for fn in (lib.oct_b200_kv4_store_device, lib.oct_b200_kv4_load_device):
         assert (fn(handle, _cache(), _batch(), _rows(**change), None, detail), detail.value) == (R.PROM_ERROR, code)
+
+
+def test_keys_and_values_are_not_read_back_into_one_tensor(lib, handle):
+    detail = C.c_int()
+    one = _rows(v=P)
+    assert lib.oct_b200_kv4_load_device(handle, _cache(), _batch(), one, None, detail) == R.PROM_ERROR
+    assert detail.value == INVALID
+    assert lib.oct_b200_kv4_store_device(handle, _cache(), _batch(), one, None, detail) == R.PROM_ERROR
+    assert detail.value == NO_DEVICE
 
 
 def test_rows_that_share_elements_may_be_read_and_not_written(lib, handle):

@@ -586,6 +586,171 @@ def test_attention_refuses_a_missing_workspace_and_foreign_types(runtime):
     assert (out == 7.0).all() and runtime.sync_status().ok
 
 
+def test_attention_may_write_over_its_queries_and_take_any_scale(runtime):
+    import torch
+    rng = np.random.default_rng(16)
+    host = Host(rng, 128, 2, 16, [1, 3], [900, 70])
+    host.fill(rng)
+    q = _torch(rng.standard_normal((4, 8, 128)), "bf16")
+    dev, batch = host.device(), host.batch()
+    ws = torch.empty(runtime.kv4_attention_workspace_bytes(dev, batch, q), dtype=torch.uint8, device="cuda")
+    for scale in (0.07, -0.05, 0.0):
+        out, lse, _ = _attend(runtime, host, q, 8, scale=scale, dev=dev, batch=batch)
+        own = q.clone()
+        runtime.kv4_attention_device(dev, batch, own, own, scale=scale, workspace=ws)
+        _ok(runtime)
+        assert torch.equal(own, out)
+        _check_attention(host, "bf16", q, out, lse, scale=scale)
+
+
+def test_many_short_sequences(runtime):
+    """More sequences than thread blocks' threads, most of a few tokens, some of none."""
+    rng = np.random.default_rng(17)
+    held = [int(x) for x in rng.integers(0, 6, 700)]
+    held[3], held[500] = 90, 40
+    host = Host(rng, 64, 1, 16, [1] * 700, held)
+    host.fill(rng)
+    q = _torch(rng.standard_normal((700, 2, 64)), "f16")
+    out, lse, _ = _attend(runtime, host, q, 2)
+    _ok(runtime)
+    _check_attention(host, "f16", q, out, lse)
+
+
+def test_pages_of_the_largest_size_and_far_positions(runtime):
+    import torch
+    rng = np.random.default_rng(18)
+    host = Host(rng, 64, 1, 65536, [3], [65536 + 40])
+    dev, batch = host.device(), host.batch()
+    k, v = (_torch(rng.standard_normal((3, 1, 64)), "f32") for _ in range(2))
+    runtime.kv4_store_device(dev, batch, k, v)
+    for i, p in enumerate(range(host.held[0] - 3, host.held[0])):
+        host.cache.write(host.table[0, p // 65536], p % 65536, 0, 0, _np(k[i, 0]))
+        host.cache.write(host.table[0, p // 65536], p % 65536, 0, 1, _np(v[i, 0]))
+    q = _torch(rng.standard_normal((1, 3, 64)), "f32")
+    one = R.Kv4Batch(_int(host.table), _int(host.held), max_kv_len=2 * 65536)
+    out, lse, _ = _attend(runtime, host, q, 3, dev=dev, batch=one, window=3)
+    _ok(runtime)
+    got = dev.data.cpu().numpy()
+    assert np.array_equal(got, host.cache.data)
+    row = np.array([host.table[0, 1]])
+    small = O.Cache(host.cache.pages, 65536, 1, 64)
+    small.data = host.cache.data
+    kk = np.stack([O.values(*small.parts(int(row[0]), p, 0, 0)) for p in range(37, 40)])
+    vv = np.stack([O.values(*small.parts(int(row[0]), p, 0, 1)) for p in range(37, 40)])
+    x = _np(q[0]) @ kk.T * float(np.float32(0.125))
+    e = np.exp(x - x.max(-1, keepdims=True))
+    want = e @ vv / e.sum(-1, keepdims=True)
+    _near(_np(out[0]), want, 2.0 ** -15)  # |v| < 4: weights to 2^-18
+    _near(_np(lse[0]), x.max(-1) + np.log(e.sum(-1)), 2.0 ** -17)
+
+
+def test_cache_offsets_beyond_32_bits(runtime):
+    """A cache of 6 GB; the sequence's pages lie at its end."""
+    import torch
+    dim, page, kv = 256, 256, 8
+    pages = (6 << 30) // (kv * (page // 16) * R.kv4_tile_bytes(dim))
+    data = torch.zeros((pages, kv * (page // 16) * R.kv4_tile_bytes(dim)), dtype=torch.uint8, device="cuda")
+    dev = R.Kv4Cache(data, page_size=page, kv_heads=kv, head_dim=dim)
+    n = 300
+    g = torch.Generator("cuda").manual_seed(1)
+    k, v, q = (torch.randn((n, h, dim), device="cuda", generator=g) for h in (kv, kv, kv))
+    small = R.Kv4Cache(torch.zeros((2, data.shape[1]), dtype=torch.uint8, device="cuda"), page_size=page, kv_heads=kv,
+                       head_dim=dim)
+    results = []
+    for cache, table in ((dev, [[pages - 1, pages - 2]]), (small, [[1, 0]])):
+        batch = R.Kv4Batch(_int(table), _int([n]), _int([0, n]), max_tokens=n, page_size=page)
+        runtime.kv4_store_device(cache, batch, k, v)
+        back = torch.empty_like(k), torch.empty_like(v)
+        runtime.kv4_load_device(cache, batch, *back)
+        one = R.Kv4Batch(_int(table), _int([n]), page_size=page)
+        out = torch.empty_like(q[:1])
+        ws = torch.empty(runtime.kv4_attention_workspace_bytes(cache, one, q[:1]), dtype=torch.uint8, device="cuda")
+        runtime.kv4_attention_device(cache, one, q[:1], out, workspace=ws)
+        _ok(runtime)
+        results.append((*back, out))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert not data[: pages - 2].any()
+    assert torch.equal(data[pages - 2:], small.data)
+    assert (results[0][0] - k).abs().max() <= 0.5  # steps of at most (max - min) / 15 < 10 / 15 and a bit
+
+
+def test_a_decode_step_captured_on_its_first_call(lib):
+    """A new process's first calls are under capture: nothing is loaded, set up or allocated before."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from oct_b200 import reactor as R
+rt = R.Runtime()
+g = torch.Generator('cuda').manual_seed(3)
+data = torch.zeros((8, 2 * R.kv4_tile_bytes(64)), dtype=torch.uint8, device='cuda')
+cache = R.Kv4Cache(data, page_size=32, kv_heads=1, head_dim=64)
+lens = torch.zeros(2, dtype=torch.int32, device='cuda')
+table = torch.arange(8, dtype=torch.int32, device='cuda').view(2, 4)
+batch = R.Kv4Batch(table, lens, page_size=32)
+x = torch.zeros((2, 6, 64), dtype=torch.float16, device='cuda')
+out = torch.zeros((2, 4, 64), dtype=torch.float16, device='cuda')
+pos = torch.zeros((2, 1), dtype=torch.int32, device='cuda')
+freq = torch.logspace(0, -4, 32, dtype=torch.float64, device='cuda')
+ws = torch.empty(rt.kv4_attention_workspace_bytes(cache, batch, x[:, :4]), dtype=torch.uint8, device='cuda')
+s = torch.cuda.Stream()
+
+def step(stream):
+    rt.qk_norm_rope_device(x[:, :4], x[:, 4:5], x[:, :4], x[:, 4:5], pos, freq, stream=stream)
+    rt.kv4_store_device(cache, batch, x[:, 4:5], x[:, 5:], stream=stream)
+    rt.kv4_attention_device(cache, batch, x[:, :4], out, workspace=ws, stream=stream)
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=s):
+    step(s)
+inputs = [torch.randn(x.shape, device='cuda', generator=g).half() for _ in range(100)]
+outs = []
+for run in (lambda: graph.replay(), lambda: step(None)):
+    data.zero_()
+    got = []
+    for i, y in enumerate(inputs):
+        x.copy_(y); pos.fill_(i); lens.fill_(i + 1)
+        torch.cuda.synchronize()
+        run()
+        torch.cuda.synchronize()
+        got.append(out.clone())
+    outs.append(torch.stack(got))
+    assert rt.sync_status().ok
+assert torch.equal(outs[0], outs[1])
+assert outs[0].isfinite().all() and outs[0].abs().amax() > 0.1
+del graph
+rt.close()
+print('captured')
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+def test_calls_at_once_on_two_streams(runtime):
+    """Two sequences' decode steps on streams of their own, each with its workspace and its cache pages."""
+    import torch
+    rng = np.random.default_rng(19)
+    hosts = [Host(rng, 128, 1, 16, [1], [1200]) for _ in range(2)]
+    streams, parts = [torch.cuda.Stream() for _ in range(2)], []
+    for h in hosts:
+        h.fill(rng)
+        q = _torch(rng.standard_normal((1, 8, 128)), "bf16")
+        dev, batch = h.device(), h.batch()
+        ws = torch.empty(runtime.kv4_attention_workspace_bytes(dev, batch, q), dtype=torch.uint8, device="cuda")
+        parts.append((dev, batch, q, torch.full_like(q, 7.0), torch.empty((1, 8), device="cuda"), ws))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (dev, batch, q, out, lse, ws), s in zip(parts, streams):
+            runtime.kv4_attention_device(dev, batch, q, out, lse=lse, workspace=ws, stream=s)
+    _ok(runtime)
+    for h, (_, _, q, out, lse, _) in zip(hosts, parts):
+        _check_attention(h, "bf16", q, out, lse)
+
+
 # ------------------------------------------------------------------ together
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_a_prompt_and_decode_steps_as_they_are_used(runtime, kind):

@@ -129,14 +129,12 @@ __device__ __forceinline__ float max_half(uint32_t a) {
   const __half2 h = *reinterpret_cast<const __half2*>(&a);
   return __half2float(__hmax(__low2half(h), __high2half(h)));
 }
-// both halves of a times the low half of b
-__device__ __forceinline__ uint32_t times_low(uint32_t a, uint32_t b) {
-  const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), __low2half2(*reinterpret_cast<const __half2*>(&b)));
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
+  const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// a times the low half of b, plus c
-__device__ __forceinline__ uint32_t fma_low(uint32_t a, uint32_t b, uint32_t c) {
-  const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), __low2half2(*reinterpret_cast<const __half2*>(&b)),
+__device__ __forceinline__ uint32_t times_plus(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
                             *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
@@ -352,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   const int32_t tok_v[2] = {static_cast<int32_t>(i4), 4 + static_cast<int32_t>(i4 ^ 1u)};  // rows 2 i4, 2 i4 + 1
 
   const int32_t tok_ld = static_cast<int32_t>((lane & 1) ? 4 + (((lane % 8) >> 1) ^ 1u) : (lane % 8) >> 1) + 8 * static_cast<int32_t>((lane >> 3) & 1);
-  const bool looks = kCentred || (g % 2 == 0 && g < 2 * NG);  // whether its row of the zeros' operand holds scales
+  const bool looks = g % 2 == 0 && g < 2 * NG;  // whether its row of the zeros' operand holds scales
 
   // The item at `unit`, if it is this block's.
   struct Item {
@@ -678,48 +676,43 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
             raw[h][nt][e] = exp2_approx(raw[h][nt][e] - m[nt][e & 1]);
             l[nt][e & 1] += raw[h][nt][e];
           }
-      // ---- values.  The zeros' operand (16-bit results): rows 2 j and 2 j + 1 are the scales and zeros
-      // of group j (of group 4 + j from row 8 on), columns a tile's tokens.
-      [[maybe_unused]] uint32_t pa[H][4];
+      // ---- values.  Scales and zeros as a matrix: rows 2 j and 2 j + 1 are those of group j (of group
+      // 4 + j from row 8 on), columns a tile's tokens.  It is the zeros' operand (16-bit results), and its
+      // scale rows, dealt to all lanes, lie as the transposed weights do.
+      uint32_t pa[H][4];
+      [[maybe_unused]] uint32_t strange[H][4];  // kMasked: where a zero is no number
       float smax = 0.f;  // the largest scale that this lane looks at
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         const uint8_t* st = stage + h * G::kBytes;
-        if constexpr (!kCentred) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) pa[h][r] = 0u;
-          if constexpr (NG == 8) {
-            load_transposed(pa[h][0], pa[h][2], pa[h][1], pa[h][3],
-                            st + G::kValueParams + tok_ld * 4 * NG + 16 * (lane / 16));
-          } else if constexpr (NG == 4) {
-            load_transposed(pa[h][0], pa[h][2], st + G::kValueParams + tok_ld * 4 * NG);
-          } else if (g < 4) {
-            uint32_t x[4];
+        for (int r = 0; r < 4; ++r) pa[h][r] = 0u;
+        if constexpr (NG == 8) {
+          load_transposed(pa[h][0], pa[h][2], pa[h][1], pa[h][3],
+                          st + G::kValueParams + tok_ld * 4 * NG + 16 * (lane / 16));
+        } else if constexpr (NG == 4) {
+          load_transposed(pa[h][0], pa[h][2], st + G::kValueParams + tok_ld * 4 * NG);
+        } else if (g < 4) {
+          uint32_t x[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              x[r] = *reinterpret_cast<const uint16_t*>(st + G::kValueParams + (tok_v[r & 1] + 8 * (r >> 1)) * 4 * NG + 2 * g);
-            pa[h][0] = x[0] | (x[1] << 16), pa[h][2] = x[2] | (x[3] << 16);
-          }
-          if constexpr (kMasked) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              // rows 2 i4 and 2 i4 + 1 (r < 2) of the order above, or 8 further on.  A zero that is no
-              // number reaches, through its codes' weights, the rows that see it
-              const int32_t x = at[h] + 8 * (r >> 1) + tok_v[0], y = at[h] + 8 * (r >> 1) + tok_v[1];
-              const uint32_t lo = x >= rows.lo_min && x <= rows.hi_max ? finite_half(pa[h][r] & 0xffffu) : 0u;
-              const uint32_t up = y >= rows.lo_min && y <= rows.hi_max ? finite_half(pa[h][r] >> 16) : 0u;
-              pa[h][r] = lo | (up << 16);
-            }
-          }
-          smax = fmaxf(smax, max_half(max_half2(max_half2(pa[h][0], pa[h][2]), max_half2(pa[h][1], pa[h][3]))));
-        } else {
-          uint32_t p0[NG], p1[NG];
-          lds(p0, st + G::kValueParams + tok_g * 4 * NG);
-          lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
-#pragma unroll
-          for (int j = 0; j < NG; ++j)
-            smax = max3(smax, keep[h][0] ? unpack_half2(p0[j]).x : 0.f, keep[h][1] ? unpack_half2(p1[j]).x : 0.f);
+          for (int r = 0; r < 4; ++r)
+            x[r] = *reinterpret_cast<const uint16_t*>(st + G::kValueParams + (tok_v[r & 1] + 8 * (r >> 1)) * 4 * NG + 2 * g);
+          pa[h][0] = x[0] | (x[1] << 16), pa[h][2] = x[2] | (x[3] << 16);
         }
+        if constexpr (kMasked) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            // rows 2 i4 and 2 i4 + 1 (r < 2) of the order above, or 8 further on: zero where no row looks.
+            // A zero that is no number reaches, through its codes' weights, the rows that see it
+            const int32_t x = at[h] + 8 * (r >> 1) + tok_v[0], y = at[h] + 8 * (r >> 1) + tok_v[1];
+            const uint32_t kept = (x >= rows.lo_min && x <= rows.hi_max ? 0xffffu : 0u) |
+                                  (y >= rows.lo_min && y <= rows.hi_max ? 0xffff0000u : 0u);
+            const uint32_t all = pa[h][r] & kept;
+            pa[h][r] = finite_half(all & 0xffffu) | (finite_half(all >> 16) << 16);
+            strange[h][r] = ((all & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((all & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+          }
+        }
+        smax = fmaxf(smax, max_half(max_half2(max_half2(pa[h][0], pa[h][2]), max_half2(pa[h][1], pa[h][3]))));
       }
       if (__any_sync(0xffffffffu, smax > (looks ? pm_limit : INFINITY))) {
         if (!looks) smax = 0.f;
@@ -745,48 +738,48 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         const uint8_t* st = stage + h * G::kBytes;
-        uint32_t vw[4][NG / 2], p0[NG], p1[NG];
+        uint32_t vw[4][NG / 2];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           lds(vw[r], st + G::kValues + (tok_v[r & 1] + 8 * (r >> 1)) * G::kRowBytes + g * 2 * NG);
-        lds(p0, st + G::kValueParams + tok_g * 4 * NG);
-        lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
-        if constexpr (kMasked) {
+        if constexpr (kCentred) {  // zeros + 8 s, summed beside the weights and rounded to nearest
+          uint32_t p0[NG], p1[NG];
+          lds(p0, st + G::kValueParams + tok_g * 4 * NG);
+          lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
 #pragma unroll
           for (int j = 0; j < NG; ++j) {
-            if (!keep[h][0]) p0[j] = 0u;
-            if (!keep[h][1]) p1[j] = 0u;
-          }
-        }
-        [[maybe_unused]] uint32_t wh[NT][2], wl[NT][2];  // w * pm in float16, and what that leaves
-        float(&w)[NT][4] = raw[h];
+            const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
+            const float z0 = fmaf(8.f, f0.x, f0.y), z1 = fmaf(8.f, f1.x, f1.y);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if constexpr (kCentred) {  // zeros + 8 s, summed beside the weights and rounded to nearest
-#pragma unroll
-            for (int j = 0; j < NG; ++j) {
-              const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
-              const float z0 = fmaf(8.f, f0.x, f0.y), z1 = fmaf(8.f, f1.x, f1.y);
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                zsum[nt][j][c] = vis[h][nt][c] ? fmaf(w[nt][c], z0, zsum[nt][j][c]) : zsum[nt][j][c];
-                zsum[nt][j][c] = vis[h][nt][2 + c] ? fmaf(w[nt][2 + c], z1, zsum[nt][j][c]) : zsum[nt][j][c];
+                const float* w = raw[h][nt];
+                if (vis[h][nt][c]) zsum[nt][j][c] = fmaf(w[c], z0, zsum[nt][j][c]);
+                if (vis[h][nt][2 + c]) zsum[nt][j][c] = fmaf(w[2 + c], z1, zsum[nt][j][c]);
               }
-            }
           }
+        }
+        // w * pm in float16 and what that leaves, transposed: tokens 2 i4, 2 i4 + 1 (and 8 on) of column g
+        uint32_t wh[NT][2];
+        [[maybe_unused]] uint32_t wl[NT][2], seen[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const float u = w[nt][2 * r] * pm, v = w[nt][2 * r + 1] * pm;
-            wh[nt][r] = pack_half2(u, v);
+            const float u = raw[h][nt][2 * r] * pm, v = raw[h][nt][2 * r + 1] * pm;
+            const uint32_t x = pack_half2(u, v);
             if constexpr (PP == 2) {
-              const float2 f = unpack_half2(wh[nt][r]);
-              wl[nt][r] = pack_half2(u - f.x, v - f.y);
+              const float2 f = unpack_half2(x);
+              wl[nt][r] = transpose8x8(pack_half2(u - f.x, v - f.y));
             }
+            wh[nt][r] = transpose8x8(x);
+            if constexpr (kMasked)
+              seen[nt][r] = transpose8x8((vis[h][nt][2 * r] ? 0xffffu : 0u) | (vis[h][nt][2 * r + 1] ? 0xffff0000u : 0u));
           }
           if constexpr (!kCentred) {
-            mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], transpose8x8(wh[nt][0]), transpose8x8(wh[nt][1]));
-            if constexpr (PP == 2)
-              mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], transpose8x8(wl[nt][0]), transpose8x8(wl[nt][1]));
+            mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], wh[nt][0], wh[nt][1]);
+            if constexpr (PP == 2) mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], wl[nt][0], wl[nt][1]);
           }
         }
 #pragma unroll
@@ -796,24 +789,26 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
           uint32_t x23 = __byte_perm(vw[2][j / 2], vw[3][j / 2], sel);
           uint32_t bf[NT][2][PP];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t scales = __shfl_sync(0xffffffffu, pa[h][j < 4 ? 2 * r : 2 * r + 1], 8 * (j % 4) + i4);
+            [[maybe_unused]] uint32_t odd = 0u;
+            if constexpr (kMasked && !kCentred)
+              odd = __shfl_sync(0xffffffffu, strange[h][j < 4 ? 2 * r : 2 * r + 1], 8 * (j % 4) + 4 + i4);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const uint32_t sz = r == 0 ? p0[j] : p1[j];
+            for (int nt = 0; nt < NT; ++nt) {
               // weight * scale: the product rounded to float16, and in two parts what the rounding left,
               // exactly, plus the weight's own second part
-              uint32_t x = times_low(wh[nt][r], sz), rest = 0u;
-              if constexpr (PP == 2) rest = fma_low(wl[nt][r], sz, fma_low(wh[nt][r], sz, x ^ 0x80008000u));
+              uint32_t x = times(wh[nt][r], scales);
+              [[maybe_unused]] uint32_t rest = 0u;
+              if constexpr (PP == 2) rest = times_plus(wl[nt][r], scales, times_plus(wh[nt][r], scales, x ^ 0x80008000u));
               if constexpr (kMasked) {
-                const bool number = kCentred || ((sz >> 16) & 0x7c00u) != 0x7c00u;
-                if (!number) rest = 0u, x = 0x7fff7fffu;
-                const uint32_t seen = (vis[h][nt][2 * r] ? 0xffffu : 0u) | (vis[h][nt][2 * r + 1] ? 0xffff0000u : 0u);
-                x &= seen;
-                rest &= seen;
+                x = ((x & ~odd) | (0x7fff7fffu & odd)) & seen[nt][r];
+                rest &= ~odd & seen[nt][r];
               }
-              bf[nt][r][0] = transpose8x8(x);
-              if constexpr (PP == 2) bf[nt][r][1] = transpose8x8(rest);
+              bf[nt][r][0] = x;
+              if constexpr (PP == 2) bf[nt][r][1] = rest;
             }
+          }
 #pragma unroll
           for (int m2 = 0; m2 < 2; ++m2) {
             uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;

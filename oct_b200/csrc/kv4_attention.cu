@@ -83,10 +83,15 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Value codes less 8, for fp32 results: code - 8 from the low nibble, 16 times that from
-// the high one.  The tensor cores truncate as they accumulate; unsigned codes let that grow with the
-// sum of the weights while the zeros cancel most of the sum itself (1.6e-5 of the result over 512 keys).
+// Codes less 8 as normal numbers: code - 8 from the low nibble, 16 times that from the high one.  The
+// subnormal codes are exact, but the tensor cores align their products as if they were 2^-14, so that the
+// sums keep about 18 bits, and truncate as they add, which unsigned codes let grow with the sum of the
+// weights while the zeros cancel most of it.  Scores are 5e-8 off with centred keys against up to 1.4e-6
+// (16-bit results differ by that in their lse alone, so bf16 takes the cheaper form: 125 us against 145
+// for 64 sequences), fp32 results over 512 keys 2e-7 with centred values against 1.6e-5 (there less 7.5, 16 times over, so that
+// the codes' mean is near zero and a bias of the sums has nothing to act on).
 constexpr uint32_t kMiddleLow = 0x64086408u, kMiddleHigh = 0x64806480u;  // 1024 + 8, 1024 + 128
+constexpr uint32_t kMiddleHalf = 0x64786478u;                             // 1024 + 120
 __device__ __forceinline__ uint32_t centred(uint32_t codes, uint32_t middle) {
   const uint32_t x = codes | 0x64006400u;  // 1024 + code
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&middle));
@@ -331,7 +336,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   constexpr int kZeroWords = NG == 8 ? 2 : 1;
   constexpr int H = tiles_per_step(D, NT), kUnit = kWarps * H;
   constexpr int kStages = G::kStages / H, kStageBytes = H * G::kBytes;
-  constexpr bool kCentred = std::is_same<T, float>::value;
+  constexpr bool kCentred = std::is_same<T, float>::value;  // value codes less 7.5
+  constexpr bool kCentredKeys = PP == 2;                    // key codes less 8
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t loaded[kWarps][kStages];
   __shared__ float2 warp_ml[kWarps][kRows];
@@ -474,21 +480,22 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const float nq = pow2_toward(amax, 10), nz = pow2_toward(smax, 10);
-      // The zeros' operand: slot 2 j of 16 meets the scale of group j and is zero, slot 2 j + 1 its zero.
-      // Four groups (or two) fill eight slots: the sums' high part there, the low part in the next
-      // eight; eight groups fill all sixteen, and the low part is a second operand.
-      float mine[kZeroWords];
+      // The zeros' operand: slot 2 j of 16 meets the scale of group j, of which centred codes lack 8,
+      // slot 2 j + 1 its zero.  Four groups (or two) fill eight slots: the sums' high part there, the low
+      // part in the next eight; eight groups fill all sixteen, and the low part is a second operand.
 #pragma unroll
       for (int x = 0; x < kZeroWords; ++x) {
-        mine[x] = 0.f;
+        float mine = 0.f;
 #pragma unroll
         for (int j = 0; j < 4 && j < NG; ++j)
-          if (static_cast<int>(i4) == j) mine[x] = sums[4 * x + j] * nz;
-        const uint32_t h = pack_half2(0.f, mine[x]);
+          if (static_cast<int>(i4) == j) mine = sums[4 * x + j] * nz;
+        const float lack = kCentredKeys ? 8.f * mine : 0.f;
+        const uint32_t h = pack_half2(lack, mine);
+        const float2 f = unpack_half2(h);
         qz[nt][0][x] = h;
-        qz[nt][1][x] = pack_half2(0.f, mine[x] - unpack_half2(h).y);
+        qz[nt][1][x] = pack_half2(lack - f.x, mine - f.y);
       }
-      const float kfac = kCodeLow / nq * a.scale_log2, zfac = a.scale_log2 / nz;
+      const float kfac = (kCentredKeys ? 1.f : kCodeLow) / nq * a.scale_log2, zfac = a.scale_log2 / nz;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int from = (2 * i4 + c) * 4;
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
 
     float o[NT][NG][2][4];  // out^T: channels 32 j + 4 g + 2 m2 (+ 1, 16 times as large), columns 2 i4, 2 i4 + 1
     float oz[NT][4];        // the zeros' share, in the rows of their operand below (16-bit results)
-    float zsum[NT][NG][2];  // the same of the zeros + 8 s, of this lane's tokens (fp32 results)
+    float zsum[NT][NG][2];  // the same of the zeros + 7.5 s, of this lane's tokens (fp32 results)
     float l[NT][2], m[NT][2], trigger[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -593,8 +600,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
             for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
 #pragma unroll
           for (int m2 = 0; m2 < 2; ++m2) {
-            const uint32_t a0 = x0 & 0x000f000fu, a2 = x0 & 0x00f000f0u;
-            const uint32_t a1 = x1 & 0x000f000fu, a3 = x1 & 0x00f000f0u;
+            uint32_t a0 = x0 & 0x000f000fu, a2 = x0 & 0x00f000f0u;
+            uint32_t a1 = x1 & 0x000f000fu, a3 = x1 & 0x00f000f0u;
+            if constexpr (kCentredKeys) {
+              a0 = centred(a0, kMiddleLow), a2 = centred(a2, kMiddleHigh);
+              a1 = centred(a1, kMiddleLow), a3 = centred(a3, kMiddleHigh);
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -742,14 +753,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           lds(vw[r], st + G::kValues + (tok_v[r & 1] + 8 * (r >> 1)) * G::kRowBytes + g * 2 * NG);
-        if constexpr (kCentred) {  // zeros + 8 s, summed beside the weights and rounded to nearest
+        if constexpr (kCentred) {  // zeros + 7.5 s, summed beside the weights and rounded to nearest
           uint32_t p0[NG], p1[NG];
           lds(p0, st + G::kValueParams + tok_g * 4 * NG);
           lds(p1, st + G::kValueParams + (tok_g + 8) * 4 * NG);
 #pragma unroll
           for (int j = 0; j < NG; ++j) {
             const float2 f0 = unpack_half2(p0[j]), f1 = unpack_half2(p1[j]);
-            const float z0 = fmaf(8.f, f0.x, f0.y), z1 = fmaf(8.f, f1.x, f1.y);
+            const float z0 = fmaf(7.5f, f0.x, f0.y), z1 = fmaf(7.5f, f1.x, f1.y);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -814,8 +825,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
             uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
             uint32_t a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
             if constexpr (kCentred) {
-              a0 = centred(a0, kMiddleLow), a1 = centred(a1, kMiddleHigh);
-              a2 = centred(a2, kMiddleLow), a3 = centred(a3, kMiddleHigh);
+              a0 = centred((x01 << 4) & 0x00f000f0u, kMiddleHalf), a1 = centred(a1, kMiddleHalf);
+              a2 = centred((x23 << 4) & 0x00f000f0u, kMiddleHalf), a3 = centred(a3, kMiddleHalf);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -847,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
 
     // ---- this warp's result, then the block's
     const float unit_f = pm_limit < 0.f ? 0.f : 1.f / pm;
-    const float low = kCentred ? unit_f : unit_f * kCodeLow, high = kCentred ? unit_f * 0.0625f : unit_f * kCodeHigh;
+    const float low = unit_f * (kCentred ? 0.0625f : kCodeLow), high = unit_f * (kCentred ? 0.0625f : kCodeHigh);
     __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)

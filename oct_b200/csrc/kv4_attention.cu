@@ -338,6 +338,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   constexpr int kStages = G::kStages / H, kStageBytes = H * G::kBytes;
   constexpr bool kCentred = std::is_same<T, float>::value;  // value codes less 7.5
   constexpr bool kCentredKeys = PP == 2;                    // key codes less 8
+  // fp32: every tile's part of the result is added rounded to nearest, since the tensor cores' truncation adds
+  // up over the keys (2 x 64 rows over 77541 keys: 8e-6 of the result off, so 1e-7; the 512-key window 20.7 us,
+  // so 22.5; 16-bit results do not show it).
+  constexpr bool kNearest = kCentred;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t loaded[kWarps][kStages];
   __shared__ float2 warp_ml[kWarps][kRows];
@@ -789,8 +793,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
               seen[nt][r] = transpose8x8((vis[h][nt][2 * r] ? 0xffffu : 0u) | (vis[h][nt][2 * r + 1] ? 0xffff0000u : 0u));
           }
           if constexpr (!kCentred) {
-            mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], wh[nt][0], wh[nt][1]);
-            if constexpr (PP == 2) mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], wl[nt][0], wl[nt][1]);
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            float(&to)[4] = kNearest ? part : oz[nt];
+            if constexpr (PP == 2) mma_f16(to, pa[h][0], pa[h][1], pa[h][2], pa[h][3], wl[nt][0], wl[nt][1]);
+            mma_f16(to, pa[h][0], pa[h][1], pa[h][2], pa[h][3], wh[nt][0], wh[nt][1]);
+            if constexpr (kNearest) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) oz[nt][e] += part[e];
+            }
           }
         }
 #pragma unroll
@@ -830,8 +840,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
+            {
+              if constexpr (kNearest) {
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int pp = 0; pp < PP; ++pp) mma_f16(o[nt][j][m2], a0, a1, a2, a3, bf[nt][0][pp], bf[nt][1][pp]);
+                for (int pp = PP - 1; pp >= 0; --pp) mma_f16(part, a0, a1, a2, a3, bf[nt][0][pp], bf[nt][1][pp]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[nt][j][m2][e] += part[e];
+              } else {
+#pragma unroll
+                for (int pp = 0; pp < PP; ++pp) mma_f16(o[nt][j][m2], a0, a1, a2, a3, bf[nt][0][pp], bf[nt][1][pp]);
+              }
+            }
             x01 >>= 8;
             x23 >>= 8;
           }

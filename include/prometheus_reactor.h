@@ -1536,8 +1536,8 @@ PROM_REACTOR_API int oct_b200_attention_device(void* handle, const float* d_q, c
    allocates nothing, keeps nothing between calls and may be captured into a
    CUDA graph.  Pointers are device pointers of the handle's GPU unless stated
    otherwise, 16-byte aligned where they point at elements; strides count
-   elements and make every row start on 16 bytes; the channels of a row are
-   adjacent.  Errors: OCT_B200_DETAIL_INVALID_ARGUMENT, _UNALIGNED,
+   elements and make every row start on 16 bytes (that of a dimension of one is
+   not used); the channels of a row are adjacent.  Errors: OCT_B200_DETAIL_INVALID_ARGUMENT, _UNALIGNED,
    _UNSUPPORTED_SHAPE, _KV4_WORKSPACE, and PROM_DETAIL_CAPABILITY_MISMATCH on a
    handle without a device.  Nothing is enqueued by a call that fails. */
 enum { OCT_B200_F32 = 0u, OCT_B200_BF16 = 1u, OCT_B200_F16 = 2u };
@@ -1639,7 +1639,8 @@ PROM_REACTOR_API int oct_b200_kv4_load_device(void* handle, const OctB200Kv4Cach
    sequence: out = softmax(scale q k^T) v, query head h with key head
    h / (q_heads / kv_heads).  With causal, the query at position p sees keys <= p
    and, with a window, keys > p - window; without, every key of its sequence.  A
-   query that sees nothing gets zeros and lse = -inf.  lse (may be NULL) is the
+   query that sees nothing gets zeros and lse = -inf.  Scores and sums are fp32,
+   for queries below 2^113.  lse (may be NULL) is the
    natural logarithm of the softmax's sum, [tokens][q_heads].  out may be q itself
    (same strides) and overlap no other part of it.  The workspace
    (oct_b200_kv4_attention_workspace_bytes of the same sizes; NULL when that is

@@ -25,10 +25,15 @@ uint32_t vector_elements(uint32_t dtype) {
   return dtype == OCT_B200_F32 ? 4u : (dtype == OCT_B200_BF16 || dtype == OCT_B200_F16 ? 8u : 0u);
 }
 
+// The stride of a dimension of one is not used.
+uint64_t used(uint64_t stride, uint64_t extent) { return extent > 1 ? stride : 0; }
+
 // A [tokens][heads][dim] tensor.  Rows of an output must not share elements.
 int check_rows(const void* p, uint64_t tokens, uint32_t heads, uint32_t dim, uint64_t token_stride,
                uint64_t head_stride, uint32_t vec, bool output) {
   if (p == nullptr) return OCT_B200_DETAIL_INVALID_ARGUMENT;
+  token_stride = used(token_stride, tokens);
+  head_stride = used(head_stride, heads);
   if (!aligned16(p) || token_stride % vec != 0 || head_stride % vec != 0) return OCT_B200_DETAIL_UNALIGNED;
   if (token_stride > kMaxStride || head_stride > kMaxStride) return OCT_B200_DETAIL_INVALID_ARGUMENT;
   // one of an output's two strides steps over all that the other covers
@@ -154,10 +159,10 @@ int run_rows(void* handle, const OctB200Kv4Cache* cache, const OctB200Kv4Batch* 
     a.type = static_cast<oct::ElementType>(rows->dtype);
     a.rows[0] = rows->k;
     a.rows[1] = rows->v;
-    a.token_stride[0] = rows->k_token_stride;
-    a.token_stride[1] = rows->v_token_stride;
-    a.head_stride[0] = rows->k_head_stride;
-    a.head_stride[1] = rows->v_head_stride;
+    a.token_stride[0] = used(rows->k_token_stride, rows->tokens);
+    a.token_stride[1] = used(rows->v_token_stride, rows->tokens);
+    a.head_stride[0] = used(rows->k_head_stride, cache->kv_heads);
+    a.head_stride[1] = used(rows->v_head_stride, cache->kv_heads);
     cudaStream_t s = static_cast<cudaStream_t>(stream);  // NULL is the CUDA default stream
     if ((store ? oct::kv4_store(a, s) : oct::kv4_load(a, s)) != cudaSuccess)
       return fail(out_detail_code, OCT_B200_DETAIL_CUDA_ERROR);
@@ -222,10 +227,10 @@ int oct_b200_qk_norm_rope_device(void* handle, const OctB200QkNormRopeRequest* r
       a.heads[0] = r->q_heads, a.heads[1] = r->k_heads;
       a.in[0] = r->q, a.in[1] = r->k;
       a.out[0] = r->q_out, a.out[1] = r->k_out;
-      a.in_token[0] = r->q_token_stride, a.in_token[1] = r->k_token_stride;
-      a.in_head[0] = r->q_head_stride, a.in_head[1] = r->k_head_stride;
-      a.out_token[0] = r->q_out_token_stride, a.out_token[1] = r->k_out_token_stride;
-      a.out_head[0] = r->q_out_head_stride, a.out_head[1] = r->k_out_head_stride;
+      a.in_token[0] = used(r->q_token_stride, r->tokens), a.in_token[1] = used(r->k_token_stride, r->tokens);
+      a.in_head[0] = used(r->q_head_stride, r->q_heads), a.in_head[1] = used(r->k_head_stride, r->k_heads);
+      a.out_token[0] = used(r->q_out_token_stride, r->tokens), a.out_token[1] = used(r->k_out_token_stride, r->tokens);
+      a.out_head[0] = used(r->q_out_head_stride, r->q_heads), a.out_head[1] = used(r->k_out_head_stride, r->k_heads);
       a.weight[0] = r->q_weight, a.weight[1] = r->k_weight;
       for (int i = 0; i < 2; ++i) {
         if (a.heads[i] == 0) continue;
@@ -233,8 +238,7 @@ int oct_b200_qk_norm_rope_device(void* handle, const OctB200QkNormRopeRequest* r
         if (bad == 0)
           bad = check_rows(a.out[i], r->tokens, a.heads[i], r->head_dim, a.out_token[i], a.out_head[i], vec, true);
         // in place means row for row
-        if (bad == 0 && a.in[i] == a.out[i] &&
-            ((r->tokens > 1 && a.in_token[i] != a.out_token[i]) || (a.heads[i] > 1 && a.in_head[i] != a.out_head[i])))
+        if (bad == 0 && a.in[i] == a.out[i] && (a.in_token[i] != a.out_token[i] || a.in_head[i] != a.out_head[i]))
           bad = OCT_B200_DETAIL_INVALID_ARGUMENT;
         if (bad == 0 && a.heads[0] > 0 && a.heads[1] > 0 && a.out[0] == a.out[1]) bad = OCT_B200_DETAIL_INVALID_ARGUMENT;
         if (bad != 0) return fail(out_detail_code, bad);
@@ -342,10 +346,10 @@ int oct_b200_kv4_attention_device(void* handle, const OctB200Kv4Cache* cache, co
     a.heads = r->q_heads;
     a.q = r->q;
     a.out = r->out;
-    a.q_token = r->q_token_stride;
-    a.q_head = r->q_head_stride;
-    a.out_token = r->out_token_stride;
-    a.out_head = r->out_head_stride;
+    a.q_token = used(r->q_token_stride, r->tokens);
+    a.q_head = used(r->q_head_stride, r->q_heads);
+    a.out_token = used(r->out_token_stride, r->tokens);
+    a.out_head = used(r->out_head_stride, r->q_heads);
     a.lse = r->lse;
     a.scale = r->scale;
     a.causal = r->causal != 0;

@@ -177,6 +177,21 @@ def test_rows_that_share_elements_may_be_read_and_not_written(lib, handle):
     assert detail.value == INVALID
 
 
+def test_the_stride_of_a_dimension_of_one_is_not_used(lib, handle):
+    detail, odd = C.c_int(), (1 << 50) + 1
+    one_token = dict(tokens=1, q_token_stride=odd, q_out_token_stride=odd + 1, k_token_stride=odd, k_out_token_stride=odd)
+    one_head = dict(q_heads=1, q_head_stride=odd, q_out_head_stride=odd + 2, k_heads=1, k_head_stride=3, k_out_head_stride=0)
+    for change in (one_token, one_head):
+        assert lib.oct_b200_qk_norm_rope_device(handle, _rope(**change), None, detail) == R.PROM_ERROR
+        assert detail.value == NO_DEVICE
+    rows = _rows(tokens=1, k_token_stride=odd, v_token_stride=7)
+    for fn in (lib.oct_b200_kv4_store_device, lib.oct_b200_kv4_load_device):
+        assert (fn(handle, _cache(), _batch(), rows, None, detail), detail.value) == (R.PROM_ERROR, NO_DEVICE)
+    rows = _attention(q_heads=1, q_head_stride=odd, out_head_stride=odd)
+    got = lib.oct_b200_kv4_attention_device(handle, _cache(kv_heads=1), _batch(), rows, None, detail)
+    assert (got, detail.value) == (R.PROM_ERROR, NO_DEVICE)
+
+
 @pytest.mark.parametrize("change, code", [
     (dict(), NO_DEVICE), (dict(struct_size=8), INVALID), (dict(dtype=4), INVALID), (dict(q_heads=0), INVALID),
     (dict(q_heads=7), INVALID), (dict(scale=float("inf")), INVALID), (dict(window=5, causal=0), INVALID),

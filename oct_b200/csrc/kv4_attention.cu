@@ -6,35 +6,44 @@
 // the window when there is one):
 //   score_p = scale * sum_j (s_pj (q . code)_pj + z_pj sum(q)_j),   j over groups of 32 channels
 //   out     = sum_p w_p (z_pj + s_pj code_p) / sum_p w_p,           w_p = exp(score_p - max)
-// so the codes enter the matrix products as integers and the scales, zeros and
-// softmax stay in fp32.
+// The codes enter the matrix products as integers; scales meet fp32 sums (keys)
+// or the weights (values), the zeros are a small product of their own, maxima,
+// sums and results stay in fp32.
 //
 // Codes as operands.  A code masked out of its word into the low bits of a
-// float16 IS the number code * 2^-24 (a subnormal, exact in the tensor cores),
-// and one nibble further up code * 2^-20.  So four ANDs and one shift turn
-// eight codes into matrix operands, with no conversion and no unpacking; the
-// powers of two are undone on the other operand (q / 16 for the upper nibbles)
-// and at the end.  q is scaled per row by a power of two that puts its largest
-// value near 2^10, so that as float16 (one part for 16-bit inputs, two for fp32)
-// it keeps its digits.
+// float16 is the number code * 2^-24, and one nibble further up code * 2^-20.  So
+// four ANDs and one shift turn eight codes into matrix operands, with no
+// conversion; the powers of two are undone on the other operand (q / 16 for the
+// upper nibbles) and at the end.  fp16 and fp32 scores and fp32 results take
+// normal numbers instead (`centred`, below).  q is scaled per row by a power of
+// two that puts its largest value near 2^10, so that as float16 (one part for
+// 16-bit inputs, two for fp32) it keeps its digits; the weights likewise, in one
+// part for bf16 (2^-12 of each, an eighth of the result's rounding) and two else.
 //
 // Tokens are the rows of both products (m16n8k16: 16 tokens, 8 query rows), so
 // one warp works through 16 keys at a time for 8 query rows -- the query heads
 // that share a key head -- and the scores' fragment becomes the second
 // product's operand with one 8 x 8 transposition per 8 tokens.
 //
-// Bound: HBM at a decode batch, reading each cached key once; the tensor pipe
-// has nothing to do beside it, which is why this runs on warp-level matrix
-// instructions whose operands come from registers instead of through tcgen05
-// and tensor memory.  Each warp streams its own tiles (16 tokens, keys and
-// values side by side) through a private ring in shared memory, by 16-byte
-// asynchronous copies: no barrier between warps until an item's end, and none
-// of the per-copy cost that bulk copies have at these sizes (a bulk copy a tile
-// streamed at 4.6 TB/s with no arithmetic at all).
+// Bound: HBM at a decode batch, reading each cached key once: 268 instructions
+// per tile of 16 keys (bf16, 128 channels), 2560 bytes, stream at 6.1 TB/s once
+// the blocks run (0.93 of the measured copy rate), which leaves the tensor pipe
+// at 15-30 % and is why this runs on warp-level matrix instructions whose
+// operands come from registers instead of through tcgen05 and tensor memory.
+// fp16 (about 350 instructions) and fp32 are bound by their warps' latencies:
+// with 168 registers a thread 12 warps share an SM and issue in every second
+// cycle.  Each warp streams its own tiles (keys and values side by side) through
+// a private ring in shared memory, by 16-byte asynchronous copies: no barrier
+// between warps until an item's end, and none of the per-copy cost that bulk
+// copies have at these sizes (a bulk copy a tile streamed at 4.6 TB/s with no
+// arithmetic at all).
 //
 // Blocks take equal runs of the call's tiles, whatever the sequences' lengths:
-// each adds up the lengths on the device and finds its own run.  An item that
-// a run's end cuts leaves partial results, which a second kernel joins in order.
+// each adds up the lengths on the device and finds its own run (2 us).  An item
+// that a run's end cuts leaves partial results, which a second kernel joins in
+// order (4-5 us).  Measured, whole calls: 64 sequences of up to 16384 keys, 32 / 8
+// heads of 128, bf16 126-135 us (587 MB, floor 89); one of 131071 keys, fp16 59 us
+// (168 MB, floor 26); one of 1000 keys, 8 / 1 heads of 256, bf16 14 us (latency).
 #include <atomic>
 #include <type_traits>
 
@@ -87,8 +96,8 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 // subnormal codes are exact, but the tensor cores align their products as if they were 2^-14, so that the
 // sums keep about 18 bits, and truncate as they add, which unsigned codes let grow with the sum of the
 // weights while the zeros cancel most of it.  Scores are 5e-8 off with centred keys against up to 1.4e-6
-// (16-bit results differ by that in their lse alone, so bf16 takes the cheaper form: 125 us against 145
-// for 64 sequences), fp32 results over 512 keys 2e-7 with centred values against 1.6e-5 (there less 7.5, 16 times over, so that
+// (16-bit results differ by that in their lse alone; bf16 takes the cheaper form, 125 us against 145 for
+// 64 sequences, fp16 does not, 60 us against 55 for 131071 keys), fp32 results over 512 keys 2e-7 with centred values against 1.6e-5 (there less 7.5, 16 times over, so that
 // the codes' mean is near zero and a bias of the sums has nothing to act on).
 constexpr uint32_t kMiddleLow = 0x64086408u, kMiddleHigh = 0x64806480u;  // 1024 + 8, 1024 + 128
 constexpr uint32_t kMiddleHalf = 0x64786478u;                             // 1024 + 120
@@ -793,14 +802,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
               seen[nt][r] = transpose8x8((vis[h][nt][2 * r] ? 0xffffu : 0u) | (vis[h][nt][2 * r + 1] ? 0xffff0000u : 0u));
           }
           if constexpr (!kCentred) {
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
-            float(&to)[4] = kNearest ? part : oz[nt];
-            if constexpr (PP == 2) mma_f16(to, pa[h][0], pa[h][1], pa[h][2], pa[h][3], wl[nt][0], wl[nt][1]);
-            mma_f16(to, pa[h][0], pa[h][1], pa[h][2], pa[h][3], wh[nt][0], wh[nt][1]);
-            if constexpr (kNearest) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) oz[nt][e] += part[e];
-            }
+            if constexpr (PP == 2) mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], wl[nt][0], wl[nt][1]);
+            mma_f16(oz[nt], pa[h][0], pa[h][1], pa[h][2], pa[h][3], wh[nt][0], wh[nt][1]);
           }
         }
 #pragma unroll
@@ -839,8 +842,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
               a2 = centred((x23 << 4) & 0x00f000f0u, kMiddleHalf), a3 = centred(a3, kMiddleHalf);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-            {
+            for (int nt = 0; nt < NT; ++nt) {
               if constexpr (kNearest) {
                 float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

@@ -42,7 +42,7 @@
 // each adds up the lengths on the device and finds its own run (2 us).  An item
 // that a run's end cuts leaves partial results, which a second kernel joins in
 // order (4-5 us).  Measured, whole calls: 64 sequences of up to 16384 keys, 32 / 8
-// heads of 128, bf16 126-135 us (587 MB, floor 89); one of 131071 keys, fp16 59 us
+// heads of 128, bf16 126-137 us (587 MB, floor 89); one of 131071 keys, fp16 60 us
 // (168 MB, floor 26); one of 1000 keys, 8 / 1 heads of 256, bf16 14 us (latency).
 #include <atomic>
 #include <type_traits>
@@ -77,12 +77,12 @@ struct Geometry {
   static constexpr int kStages = D == 64 ? 8 : (D == 128 ? 6 : 4);
 };
 
-// Query rows of one block in groups of 8, by what the accumulators leave of the registers.
 // Tiles that a warp works through at a time: with two, one vote on the maximum and one on the scales
 // serve 32 keys and their operands' latencies overlap.
 constexpr int tiles_per_step(int dim, int row_groups) { return dim * row_groups <= 128 ? 2 : 1; }
 // Blocks per SM that the compiler leaves registers for, and that a launch fills.
 constexpr int blocks_per_sm(int dim, int row_groups, int query_parts) { return dim * row_groups <= 128 ? 3 : 2; }
+// Query rows of one block in groups of 8, by what the accumulators leave of the registers.
 template <int D> constexpr int kMaxRowGroups = D == 64 ? 4 : (D == 128 ? 2 : 1);
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -95,10 +95,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 // Codes less 8 as normal numbers: code - 8 from the low nibble, 16 times that from the high one.  The
 // subnormal codes are exact, but the tensor cores align their products as if they were 2^-14, so that the
 // sums keep about 18 bits, and truncate as they add, which unsigned codes let grow with the sum of the
-// weights while the zeros cancel most of it.  Scores are 5e-8 off with centred keys against up to 1.4e-6
-// (16-bit results differ by that in their lse alone; bf16 takes the cheaper form, 125 us against 145 for
-// 64 sequences, fp16 does not, 60 us against 55 for 131071 keys), fp32 results over 512 keys 2e-7 with centred values against 1.6e-5 (there less 7.5, 16 times over, so that
-// the codes' mean is near zero and a bias of the sums has nothing to act on).
+// weights while the zeros cancel most of it.  Scores are 5e-8 off with centred keys against up to 1.4e-6:
+// 16-bit results differ by that in their lse alone, so bf16 takes the cheaper form (125 us against 145 for
+// 64 sequences) and fp16, whose lse is asked for more digits, does not (60 us against 55 for 131071 keys).
+// fp32 results over 512 keys are 2e-7 off with centred values against 1.6e-5 (there less 7.5, 16 times
+// over, so that the codes' mean is near zero and a bias of the sums has nothing to act on).
 constexpr uint32_t kMiddleLow = 0x64086408u, kMiddleHigh = 0x64806480u;  // 1024 + 8, 1024 + 128
 constexpr uint32_t kMiddleHalf = 0x64786478u;                             // 1024 + 120
 __device__ __forceinline__ uint32_t centred(uint32_t codes, uint32_t middle) {

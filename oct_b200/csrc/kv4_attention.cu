@@ -38,12 +38,16 @@
 // copies have at these sizes (a bulk copy a tile streamed at 4.6 TB/s with no
 // arithmetic at all).
 //
-// Blocks take equal runs of the call's tiles, whatever the sequences' lengths:
-// each adds up the lengths on the device and finds its own run (2 us).  An item
-// that a run's end cuts leaves partial results, which a second kernel joins in
-// order (4-5 us).  Measured, whole calls: 64 sequences of up to 16384 keys, 32 / 8
-// heads of 128, bf16 126-137 us (587 MB, floor 89); one of 131071 keys, fp16 60 us
-// (168 MB, floor 26); one of 1000 keys, 8 / 1 heads of 256, bf16 14 us (latency).
+// Short items (one or few sequences, short keys, windows) get a cluster of blocks
+// each, which join their parts through distributed shared memory.  Else blocks
+// take equal runs of the call's tiles, whatever the sequences' lengths: each adds
+// up the lengths on the device and finds its own run (2 us), and an item that a
+// run's end cuts leaves partial results, which a second kernel joins in order
+// (4-5 us).  Measured, whole calls: 64 sequences of up to 16384 keys, 32 / 8
+// heads of 128, bf16 124-135 us (587 MB, floor 89); one of 131071 keys, fp16 57 us
+// (168 MB, floor 26); one of 1000 keys, 8 / 1 heads of 256, bf16 9.8 us (latency;
+// 14.4 spread over the GPU and joined by a second kernel).
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -80,6 +84,14 @@ struct Geometry {
 // Tiles that a warp works through at a time: with two, one vote on the maximum and one on the scales
 // serve 32 keys and their operands' latencies overlap.
 constexpr int tiles_per_step(int dim, int row_groups) { return dim * row_groups <= 128 ? 2 : 1; }
+// Blocks of a cluster that share one item, at most: more than the portable 8 (one token over 1000 keys of
+// 256 channels: 10.8 us with up to 16, 12.3 with up to 8).
+constexpr uint32_t kMaxCluster = 16;
+// Units that each block of a cluster may get; longer items are spread over the whole GPU, which balances
+// sequences of unequal lengths.  Clusters against equal runs, sequences of one length: 8 of 2048 keys, 32 / 8
+// heads of 128, bf16, 12.2 us against 15.5 (4 units a block), of 4096 16.4 against 20.9 (8), 16 of 8192 45.5
+// against 43.9 (32); fp32, 8 / 1 heads of 256, one of 4096 15.6 against 16.4 (4), of 8192 22.0 against 20.3 (8).
+constexpr uint32_t cluster_units(ElementType type) { return type == kF32 ? 4 : 8; }
 // Blocks per SM that the compiler leaves registers for, and that a launch fills.
 constexpr int blocks_per_sm(int dim, int row_groups, int query_parts) { return dim * row_groups <= 128 ? 3 : 2; }
 // Query rows of one block in groups of 8, by what the accumulators leave of the registers.
@@ -122,6 +134,20 @@ __device__ __forceinline__ void load_transposed(uint32_t& m0, uint32_t& m1, uint
                : "r"(smem_addr(row))
                : "memory");
 }
+// Loads from the shared memory of another block of the cluster.
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -151,6 +177,11 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t times_plus(uint32_t a, uint32_t b, uint32_t c) {
   const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
                             *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t times_minus(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                            __hneg2(*reinterpret_cast<const __half2*>(&c)));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t w) {
@@ -209,6 +240,7 @@ struct KernelArgs {
   float* part_o;    // [blocks][2][rows of a tile][D]
   float2* part_ml;  // [blocks][2][rows of a tile]
   PartOf* part_of;  // [blocks]
+  uint32_t cluster;  // blocks that share one item and join it among themselves; 0: equal runs of all items
 };
 
 // The keys that the rows of one row tile see: row r of a sequence is query
@@ -335,6 +367,24 @@ __device__ __forceinline__ bool find_share(const KernelArgs& a, uint32_t rows_pe
   return true;
 }
 
+// A block's share where every cluster has one item: an equal run of its units.
+__device__ __forceinline__ void cluster_share(const KernelArgs& a, uint32_t rows_per_tile, int32_t unit_tiles,
+                                              Share* out, PartOf* item) {
+  const uint32_t at = blockIdx.x / a.cluster, rank = blockIdx.x - at * a.cluster;
+  out->pair = at / a.view.kv_heads;
+  out->head = at - out->pair * a.view.kv_heads;
+  Kv4Seq s;
+  Rows r;
+  uint32_t units = 0, count = 0;
+  if (item_rows(a, out->pair, rows_per_tile, &s, &r)) units = item_units(r, unit_tiles), count = r.count;
+  out->per = (units + a.cluster - 1) / a.cluster;
+  out->begin = out->offset = min(units, rank * out->per);
+  out->end = min(units, out->begin + out->per);
+  out->cost = 0;
+  out->pad = 1;
+  if (threadIdx.x == 0) *item = PartOf{0, out->head, count > 0 ? r.first : 0, count, count > 0 ? s.row0 : 0, 0};
+}
+
 // float16 bits, zero for infinities and NaN
 __device__ __forceinline__ uint32_t finite_half(uint32_t bits) { return (bits & 0x7c00u) == 0x7c00u ? 0u : bits; }
 
@@ -356,11 +406,20 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
   __shared__ uint32_t loaded[kWarps][kStages];
   __shared__ float2 warp_ml[kWarps][kRows];
 
-  griddep_launch_dependents();
+  __shared__ PartOf cluster_item;
+  __shared__ float2 block_ml[kRows];
+
+  griddep_wait();
   Share share;
-  const bool any = find_share(a, kRows, kUnit, &share);
-  if (threadIdx.x == 0 && a.part_of != nullptr) a.part_of[blockIdx.x] = PartOf{};
-  if (!any) return;
+  if (a.cluster != 0) {
+    cluster_share(a, kRows, kUnit, &share, &cluster_item);
+    if (share.begin >= share.end && threadIdx.x < kRows) block_ml[threadIdx.x] = make_float2(-INFINITY, 0.f);
+  } else {
+    griddep_launch_dependents();
+    const bool any = find_share(a, kRows, kUnit, &share);
+    if (threadIdx.x == 0 && a.part_of != nullptr) a.part_of[blockIdx.x] = PartOf{};
+    if (!any) return;
+  }
 
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, i4 = lane % 4;
   uint8_t* ring = smem + warp * (G::kStages * G::kBytes);
@@ -825,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
               // exactly, plus the weight's own second part
               uint32_t x = times(wh[nt][r], scales);
               [[maybe_unused]] uint32_t rest = 0u;
-              if constexpr (PP == 2) rest = times_plus(wl[nt][r], scales, times_plus(wh[nt][r], scales, x ^ 0x80008000u));
+              if constexpr (PP == 2) rest = times_plus(wl[nt][r], scales, times_minus(wh[nt][r], scales, x));
               if constexpr (kMasked) {
                 x = ((x & ~odd) | (0x7fff7fffu & odd)) & seen[nt][r];
                 rest &= ~odd & seen[nt][r];
@@ -836,11 +895,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
           }
 #pragma unroll
           for (int m2 = 0; m2 < 2; ++m2) {
-            uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u;
-            uint32_t a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
+            uint32_t a0, a1, a2, a3;
             if constexpr (kCentred) {
-              a0 = centred((x01 << 4) & 0x00f000f0u, kMiddleHalf), a1 = centred(a1, kMiddleHalf);
-              a2 = centred((x23 << 4) & 0x00f000f0u, kMiddleHalf), a3 = centred(a3, kMiddleHalf);
+              a0 = centred((x01 << 4) & 0x00f000f0u, kMiddleHalf), a1 = centred(x01 & 0x00f000f0u, kMiddleHalf);
+              a2 = centred((x23 << 4) & 0x00f000f0u, kMiddleHalf), a3 = centred(x23 & 0x00f000f0u, kMiddleHalf);
+              x01 >>= 8;
+              x23 >>= 8;
+            } else {  // the low nibble's code, and both as one byte, from which the end takes the low one
+              a1 = __byte_perm(x01, 0u, m2 == 0 ? 0x4240u : 0x4341u), a0 = a1 & 0x000f000fu;
+              a3 = __byte_perm(x23, 0u, m2 == 0 ? 0x4240u : 0x4341u), a2 = a3 & 0x000f000fu;
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -855,8 +918,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
                 for (int pp = 0; pp < PP; ++pp) mma_f16(o[nt][j][m2], a0, a1, a2, a3, bf[nt][0][pp], bf[nt][1][pp]);
               }
             }
-            x01 >>= 8;
-            x23 >>= 8;
           }
         }
       }
@@ -907,7 +968,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
           float2* to = reinterpret_cast<float2*>(mine + col * D + 32 * j + 4 * g);
 #pragma unroll
           for (int m2 = 0; m2 < 2; ++m2)
-            to[m2] = make_float2(fmaf(o[nt][j][m2][c], low, z), fmaf(o[nt][j][m2][2 + c], high, z));
+            {
+            const float lower = o[nt][j][m2][c], upper = o[nt][j][m2][2 + c] - (kCentred ? 0.f : lower);
+            to[m2] = make_float2(fmaf(lower, low, z), fmaf(upper, high, z));
+          }
         }
       }
     const uint64_t row0 = seq.row0;
@@ -924,7 +988,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     if (more)
       for (int32_t k = 0; k < kAhead; ++k) issue(item, k);
     __syncthreads();
-    const float* all = reinterpret_cast<const float*>(smem + (kStages - kResultStages) * kStageBytes);
+    float* all = reinterpret_cast<float*>(smem + (kStages - kResultStages) * kStageBytes);
     constexpr int kWarpFloats = G::kStages * G::kBytes / 4;
     for (uint32_t e = threadIdx.x; e < count * (D / 4); e += kThreads) {
       const uint32_t col = e / (D / 4), c4 = e % (D / 4);
@@ -946,7 +1010,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
         sum.z = fmaf(f, x.z, sum.z);
         sum.w = fmaf(f, x.w, sum.w);
       }
-      if (whole) {
+      if (a.cluster != 0) {  // over the first warp's part, which no other thread reads here
+        *reinterpret_cast<float4*>(all + col * D + 4 * c4) = sum;
+        if (c4 == 0) block_ml[col] = make_float2(top, total);
+      } else if (whole) {
         const uint32_t row = first_row + col;
         const uint64_t token = row0 + row / a.share;
         const uint32_t qh = head * a.share + row % a.share;
@@ -963,6 +1030,48 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     }
     __syncthreads();  // the next item's copies overwrite what was written and read here
   }
+  if (a.cluster == 0) return;
+  // The cluster's blocks have their parts in shared memory; each joins its share of the item's results.
+  cluster_sync();
+  const uint32_t count = cluster_item.count;
+  const float* const parts = reinterpret_cast<const float*>(smem + (kStages - kResultStages) * kStageBytes);
+  for (uint32_t e = cluster_cta_rank() * kThreads + threadIdx.x; e < count * (D / 4); e += a.cluster * kThreads) {
+    const uint32_t col = e / (D / 4), c4 = e % (D / 4);
+    float2 ml[kMaxCluster];
+    float4 x[kMaxCluster];
+    float top = -INFINITY;
+#pragma unroll
+    for (uint32_t r = 0; r < kMaxCluster; ++r) {
+      ml[r] = make_float2(-INFINITY, 0.f);
+      if (r >= a.cluster) continue;
+      ml[r] = ld_cluster_v2(cluster_smem_addr(block_ml + col, r));
+      x[r] = ld_cluster_v4(cluster_smem_addr(parts + col * D + 4 * c4, r));
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < kMaxCluster; ++r) top = fmaxf(top, ml[r].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float total = 0.f;
+#pragma unroll
+    for (uint32_t r = 0; r < kMaxCluster; ++r) {
+      if (ml[r].x == -INFINITY) continue;  // what such a block holds is no part
+      const float f = exp2_approx(ml[r].x - base);
+      total = fmaf(f, ml[r].y, total);
+      sum.x = fmaf(f, x[r].x, sum.x);
+      sum.y = fmaf(f, x[r].y, sum.y);
+      sum.z = fmaf(f, x[r].z, sum.z);
+      sum.w = fmaf(f, x[r].w, sum.w);
+    }
+    const uint32_t row = cluster_item.first + col;
+    const uint64_t token = cluster_item.row0 + row / a.share;
+    const uint32_t qh = cluster_item.head * a.share + row % a.share;
+    const float inv = top == -INFINITY ? 0.f : 1.0f / total;
+    store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c4,
+           make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+    if (c4 == 0 && a.lse != nullptr) a.lse[token * a.heads + qh] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
+  }
+  __syncwarp();
+  cluster_sync();  // no block's shared memory goes before the others have read it
 }
 
 // Joins the parts of every item that was split: block x looks at what block x of the first kernel
@@ -1040,16 +1149,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const KernelArgs
 
 template <typename T, int D, int kJoinColumns>
 cudaError_t launch_join(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(plan.blocks, D / 4 / kJoinColumns);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D, kJoinColumns>, a, plan.row_tile);
+  return launch_dependent(kv4_join_kernel<T, D, kJoinColumns>, dim3(plan.blocks, D / 4 / kJoinColumns), kJoinThreads, 0,
+                          stream, 0, a, plan.row_tile);
 }
 
 template <typename T> constexpr int kQueryParts = sizeof(T) == 4 ? 2 : 1;
@@ -1069,10 +1170,11 @@ cudaError_t launch(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream
   if (device > 63 || (set.load(std::memory_order_acquire) & bit) == 0) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
     if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
     set.fetch_or(bit, std::memory_order_release);
   }
-  kernel<<<plan.blocks, kThreads, kSmem, stream>>>(a);
-  e = cudaGetLastError();
+  e = launch_dependent(kernel, dim3(plan.blocks), kThreads, kSmem, stream, a.cluster, a);
   if (e != cudaSuccess || plan.workspace == 0) return e;
   // Few items have many parts each: narrower blocks give a row's parts to more threads (8 items of 54
   // parts: 55 us against 58 of the whole call).  Many items have a few: fewer blocks start faster (439
@@ -1110,22 +1212,41 @@ cudaError_t dispatch_dim(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t 
 bool kv4_attention_supported(uint32_t dim) { return dim == 64 || dim == 128 || dim == 256; }
 
 Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint32_t batch, uint32_t max_tokens,
-                           uint32_t max_kv_len, ElementType type) {
+                           uint32_t max_kv_len, uint32_t window, ElementType type) {
   Kv4Plan p;
-  const uint64_t rows = static_cast<uint64_t>(max_tokens) * (heads / kv_heads);
+  const uint64_t share = heads / kv_heads, rows = static_cast<uint64_t>(max_tokens) * share;
   const uint32_t most = dim == 64 ? 8 * kMaxRowGroups<64> : 8 * (dim == 128 ? kMaxRowGroups<128> : kMaxRowGroups<256>);
   p.row_tile = 8;
   while (p.row_tile < most && p.row_tile < rows) p.row_tile *= 2;
   p.row_tiles = (rows + p.row_tile - 1) / p.row_tile;
-  // One wave: as many blocks as the SMs hold, each with an equal share of the units, or a block per
-  // unit where there are fewer (of the longest sequences the call allows).
-  const uint64_t resident = 148ull * blocks_per_sm(static_cast<int>(dim), static_cast<int>(p.row_tile / 8), type == kF32 ? 2 : 1);
-  const uint64_t tiles = (static_cast<uint64_t>(max_kv_len) + kKv4Tile - 1) / kKv4Tile;
+  // Most tiles that an item's rows see: those of the longest sequence the call allows, or of the window
+  // and the tokens whose rows share the item, wherever that begins in a tile.
+  uint64_t tiles = (static_cast<uint64_t>(max_kv_len) + kKv4Tile - 1) / kKv4Tile;
+  if (window > 0) {
+    const uint64_t tokens = std::min<uint64_t>(max_tokens, (p.row_tile + share - 2) / share + 1);
+    tiles = std::min(tiles, (window + tokens - 2) / kKv4Tile + 2);
+  }
   const uint64_t unit = kWarps * tiles_per_step(static_cast<int>(dim), static_cast<int>(p.row_tile / 8));
   const uint64_t item = tiles <= unit ? 1 : (tiles + unit - 1) / unit;
   const uint64_t items = static_cast<uint64_t>(batch) * kv_heads * p.row_tiles;
-  p.blocks = static_cast<uint32_t>(items >= resident || items * (item + 1) >= resident ? resident : items * (item + 1));
+  const uint64_t resident = 148ull * blocks_per_sm(static_cast<int>(dim), static_cast<int>(p.row_tile / 8), type == kF32 ? 2 : 1);
   p.run = items * (item + kItemCost);
+  // Few items of a few units: a cluster of blocks for each, which joins it in shared memory, needs no
+  // workspace and looks at no other sequence's length.
+  if (item > 1 && 2 * items <= resident) {
+    uint64_t cluster = 2;
+    // a cluster's blocks share a GPC, of whose places clusters of 8 and 16 may leave some empty
+    auto room = [&](uint64_t c) { return c > 4 ? resident / 4 * 3 : resident; };
+    while (cluster < kMaxCluster && cluster < item && 2 * cluster * items <= room(2 * cluster)) cluster *= 2;
+    if (item <= cluster * cluster_units(type)) {
+      p.cluster = static_cast<uint32_t>(cluster);
+      p.blocks = static_cast<uint32_t>(items * cluster);
+      return p;
+    }
+  }
+  // Else one wave: as many blocks as the SMs hold, each with an equal share of the units, or a block per
+  // unit where there are fewer.
+  p.blocks = static_cast<uint32_t>(items >= resident || items * (item + 1) >= resident ? resident : items * (item + 1));
   // an item of one unit is never split
   if (item > 1)
     p.workspace = static_cast<uint64_t>(p.blocks) * (2 * p.row_tile * (static_cast<uint64_t>(dim) * 4 + 8) + sizeof(PartOf));
@@ -1149,6 +1270,7 @@ cudaError_t kv4_attention(const Kv4AttnArgs& in, const Kv4Plan& plan, cudaStream
   a.causal = in.causal ? 1 : 0;
   a.window = in.window;
   a.row_tiles = static_cast<uint32_t>(plan.row_tiles);
+  a.cluster = plan.cluster;
   if (plan.workspace > 0) {
     const uint64_t parts = 2ull * plan.blocks * plan.row_tile;
     a.part_o = static_cast<float*>(in.workspace);

@@ -15,7 +15,7 @@
 // fragments both read their operands from that one order without unpacking a
 // code twice.
 //
-// Bound: HBM for the load (119 us for 701 MB: 5.9 TB/s, 0.90 of the measured copy
+// Bound: HBM for the load (116 us for 701 MB: 6.0 TB/s, 0.92 of the measured copy
 // rate), the issue slots for the store (170 us for 493 MB: 180 instructions for a
 // warp's 256 channels, the schedulers issue in 73 % of the cycles).  A warp takes rows of one
 // tile's keys or values of one head: one page lookup serves them all, and the loads
@@ -217,6 +217,7 @@ struct Runs {
 template <typename T, int D, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 8) kv4_store_kernel(const Kv4RowArgs a) {
   using G = Geometry<D>;
+  griddep_wait();
   Kv4Seq s;
   if (!kv4_seq(a.view, blockIdx.y, &s)) return;
   const int lane = threadIdx.x % G::kLanes, sub = threadIdx.x % 32 / G::kLanes;
@@ -278,6 +279,7 @@ __global__ void __launch_bounds__(kThreads, 8) kv4_store_kernel(const Kv4RowArgs
 template <typename T, int D, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 12) kv4_load_kernel(const Kv4RowArgs a) {
   using G = Geometry<D>;
+  griddep_wait();
   Kv4Seq s;
   if (!kv4_seq(a.view, blockIdx.y, &s)) return;
   const int lane = threadIdx.x % G::kLanes, sub = threadIdx.x % 32 / G::kLanes;
@@ -344,15 +346,9 @@ cudaError_t launch(const Kv4RowArgs& a, bool store, cudaStream_t stream) {
   const bool fills = whole * a.view.batch >= 148ull * 32;
   const uint64_t blocks = ((fills ? whole : whole * 2 * Geometry<D>::kStrips) + kWarps - 1) / kWarps;
   const dim3 grid(static_cast<uint32_t>(blocks < 65536 ? blocks : 65536), a.view.batch);
-  if (store && fills)
-    kv4_store_kernel<T, D, true><<<grid, kThreads, 0, stream>>>(a);
-  else if (store)
-    kv4_store_kernel<T, D, false><<<grid, kThreads, 0, stream>>>(a);
-  else if (fills)
-    kv4_load_kernel<T, D, true><<<grid, kThreads, 0, stream>>>(a);
-  else
-    kv4_load_kernel<T, D, false><<<grid, kThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  const auto kernel = store ? (fills ? kv4_store_kernel<T, D, true> : kv4_store_kernel<T, D, false>)
+                            : (fills ? kv4_load_kernel<T, D, true> : kv4_load_kernel<T, D, false>);
+  return launch_dependent(kernel, grid, kThreads, 0, stream, 0, a);
 }
 
 template <typename T>

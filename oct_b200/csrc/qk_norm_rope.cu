@@ -18,9 +18,9 @@
 // at once.  A thread keeps its row (head) and channels while it goes through a
 // block's tokens: the weight stays in registers, the loads of the next tokens are
 // on their way, and the tokens' cosines and sines, computed once per block into
-// shared memory, serve all heads.  2 x 4096 tokens x 48 heads of 128 (bf16): 41 us,
-// 4.9 TB/s (0.75 of the measured copy rate); 4096 tokens x 9 heads of 256 (fp32):
-// 14.4-18 us, 4.1-5.2 TB/s; one token: 4 us of kernel.
+// shared memory, serve all heads.  2 x 4096 tokens x 48 heads of 128 (bf16): 39 us,
+// 5.1 TB/s (0.78 of the measured copy rate); 4096 tokens x 9 heads of 256 (fp32):
+// 13-16 us, 4.7-5.8 TB/s; one token: 1.8 us from call to call in a graph.
 //
 // Angles: position * frequency is reduced to a fraction of a turn in binary64
 // before the fp32 sine and cosine, because a far position loses every digit of
@@ -67,6 +67,7 @@ __device__ __forceinline__ void as_pairs(const float (&x)[8], Pair (&p)[4]) {
 template <typename T, int LANES, bool kInterleaved>
 __global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_kernel(const QkNormRopeArgs a, uint32_t block_tokens) {
   constexpr int kInFlight = kTokensInFlight<T>;
+  griddep_wait();
   extern __shared__ float2 turns[];  // [block_tokens][cos, sin][4][rotary / 16]: pairs 2 i and 2 i + 1 of a lane
   const uint32_t pairs = a.rotary / 2, strip = a.rotary / 16;
   const uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * block_tokens;
@@ -199,11 +200,8 @@ cudaError_t launch(const QkNormRopeArgs& a, cudaStream_t stream) {
   const uint64_t blocks = (a.tokens + bt - 1) / bt;
   const size_t smem = static_cast<size_t>(bt) * (a.rotary / 2) * sizeof(float2);
   const dim3 grid(static_cast<uint32_t>(blocks), row_runs);
-  if (a.interleaved)
-    qk_norm_rope_kernel<T, LANES, true><<<grid, threads, smem, stream>>>(a, bt);
-  else
-    qk_norm_rope_kernel<T, LANES, false><<<grid, threads, smem, stream>>>(a, bt);
-  return cudaGetLastError();
+  return launch_dependent(a.interleaved ? qk_norm_rope_kernel<T, LANES, true> : qk_norm_rope_kernel<T, LANES, false>,
+                          grid, threads, smem, stream, 0, a, bt);
 }
 
 template <typename T>

@@ -5,9 +5,32 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "ptx.cuh"
 #include "serving.h"
 
 namespace oct {
+
+// Launches a kernel whose threads all begin with griddep_wait(): its blocks may be placed while the
+// stream's previous kernel ends, and touch no memory before that one's is all written.  Cluster: blocks
+// per cluster along x, or 0.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, uint32_t threads, size_t smem, cudaStream_t stream,
+                             uint32_t cluster, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 template <ElementType T> struct Element;
 template <> struct Element<kF32> { using type = float; };

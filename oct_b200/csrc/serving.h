@@ -70,11 +70,12 @@ struct Kv4Plan {
   uint32_t row_tile = 0;   // query rows (token, head of a key head's share) of one item
   uint64_t row_tiles = 0;  // items per (sequence, key head)
   uint32_t blocks = 0;
+  uint32_t cluster = 0;    // blocks per cluster where each cluster has one item; 0: equal runs of all items
   uint64_t run = 0;        // bound of the call's work in the kernel's units
   uint64_t workspace = 0;  // bytes; 0 when no item can be split
 };
 Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint32_t batch, uint32_t max_tokens,
-                           uint32_t max_kv_len, ElementType type);
+                           uint32_t max_kv_len, uint32_t window, ElementType type);
 struct Kv4AttnArgs {
   Kv4View view;
   ElementType type = kF32;

@@ -189,7 +189,7 @@ int check_attention(const OctB200Kv4Cache* c, const OctB200Kv4Batch* b, const Oc
   }
   if (r->q_heads > 65535u || static_cast<uint64_t>(b->max_tokens) * r->q_heads > 0x7fffffffull)
     return OCT_B200_DETAIL_UNSUPPORTED_SHAPE;
-  *plan = oct::kv4_attention_plan(c->head_dim, c->kv_heads, r->q_heads, b->batch, b->max_tokens, b->max_kv_len,
+  *plan = oct::kv4_attention_plan(c->head_dim, c->kv_heads, r->q_heads, b->batch, b->max_tokens, b->max_kv_len, r->window,
                                   static_cast<oct::ElementType>(r->dtype));
   // work is counted in 32 bits, in units of 64 or 128 keys of an item
   return plan->row_tiles * b->batch > 0x3fffffffull || plan->run > 0x3fffffffull ? OCT_B200_DETAIL_UNSUPPORTED_SHAPE : 0;

@@ -219,8 +219,10 @@ def test_workspace_is_a_function_of_sizes(lib):
     rc, long = ask(_batch(**wide), _attention())
     assert rc == R.PROM_OK and 0 < long < 1 << 25  # two parts per thread block, however many the keys
     assert ask(_batch(**(wide | dict(max_kv_len=1 << 16))), _attention()) == (R.PROM_OK, long)
-    rc, short = ask(_batch(), _attention())
-    assert rc == R.PROM_OK and 0 < short < long
+    assert ask(_batch(), _attention()) == (R.PROM_OK, 0)  # a cluster's blocks join in shared memory
+    rc, few = ask(_batch(**(wide | dict(max_kv_len=1 << 14))), _attention())
+    assert rc == R.PROM_OK and 0 < few <= long
+    assert ask(_batch(**wide), _attention(window=512)) == (R.PROM_OK, 0)  # the window bounds an item's keys
     assert ask(_batch(batch=0), _attention()) == (R.PROM_OK, 0)
     assert ask(_batch(), _attention(q_heads=3))[0] == R.PROM_ERROR
 

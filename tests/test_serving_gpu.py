@@ -514,6 +514,13 @@ def test_attention_of_strided_rows(runtime):
     _check_attention(host, "bf16", q, out, lse)
 
 
+def _wide(host):
+    """The same sequences in a table of many more pages (no pages of the cache): their keys are spread over the GPU."""
+    table = np.full((len(host.held), (1 << 18) // host.page), -1, np.int32)
+    table[:, : host.table.shape[1]] = host.table
+    return R.Kv4Batch(_int(table), _int(host.held), _int(host.starts), max_tokens=max(1, max(host.new)), page_size=host.page)
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_split_keys_join_to_the_same_result(runtime, kind):
     """A long table makes the host plan many splits; short and empty sequences use few of them."""
@@ -521,10 +528,47 @@ def test_split_keys_join_to_the_same_result(runtime, kind):
     host = Host(rng, 64, 1, 16, [1, 1, 1, 3], [3000, 0, 5, 260])
     host.fill(rng)
     q = _torch(rng.standard_normal((8, 4, 64)), kind)
-    dev, batch = host.device(), host.batch(max_kv_len=3008)
+    dev, batch = host.device(), _wide(host)
     assert runtime.kv4_attention_workspace_bytes(dev, batch, q) > 0
     out, lse, _ = _attend(runtime, host, q, 4, dev=dev, batch=batch)
     again, lse2, _ = _attend(runtime, host, q, 4, dev=dev, batch=batch)
+    _ok(runtime)
+    import torch
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    _check_attention(host, kind, q, out, lse)
+
+
+@pytest.mark.parametrize("case", [c for c in ATTENTIONS if c[7] == 0],
+                         ids=lambda c: f"{c[0]}-{c[1]}-{c[2]}x{c[3]}-q{max(c[5])}-{c[8]}")
+def test_spread_keys_match_oracle(runtime, case):
+    kind, dim, kv, share, page, new, held, _, causal = case
+    rng = np.random.default_rng(dim + share)
+    host = Host(rng, dim, kv, page, new, held)
+    host.fill(rng)
+    q = _torch(rng.standard_normal((sum(new) + 2, kv * share, dim)), kind)
+    batch = _wide(host)
+    assert runtime.kv4_attention_workspace_bytes(host.device(), batch, q, causal=causal) > 0
+    out, lse, _ = _attend(runtime, host, q, kv * share, causal=causal, batch=batch)
+    _ok(runtime)
+    _check_attention(host, kind, q, out, lse, causal=causal)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim, sequences, longest, heads", [
+    (64, 1, 400, 2), (64, 120, 400, 3), (64, 1, 2300, 8), (64, 40, 1100, 20), (128, 1, 1500, 8), (128, 30, 700, 9),
+    (256, 1, 1000, 5), (256, 20, 520, 8), (256, 70, 300, 12),
+])
+def test_clusters_of_every_size_join_their_parts(runtime, kind, dim, sequences, longest, heads):
+    """One long sequence beside short and empty ones: blocks of a cluster without a part, and none with one.
+    (40 sequences of 1100 keys are spread over the GPU in fp32, whose blocks take fewer units.)"""
+    rng = np.random.default_rng(dim + sequences + longest)
+    held = [longest] + [int(x) for x in rng.integers(0, 20, sequences - 1)]
+    host = Host(rng, dim, 1, 16, [1] * sequences, held)
+    host.fill(rng)
+    q = _torch(rng.standard_normal((sequences, heads, dim)), kind)
+    dev, batch = host.device(), host.batch()
+    out, lse, _ = _attend(runtime, host, q, heads, dev=dev, batch=batch)
+    again, lse2, _ = _attend(runtime, host, q, heads, dev=dev, batch=batch)
     _ok(runtime)
     import torch
     assert torch.equal(out, again) and torch.equal(lse, lse2)
@@ -566,7 +610,7 @@ def test_captured_step_follows_lengths_and_pages_on_the_device(runtime):
 def test_attention_refuses_a_missing_workspace_and_foreign_types(runtime):
     import torch
     rng = np.random.default_rng(14)
-    host = Host(rng, 64, 1, 16, [1], [2000])
+    host = Host(rng, 64, 1, 16, [1], [20000])  # more keys than one cluster of blocks takes
     dev, batch = host.device(), host.batch()
     q = torch.zeros((1, 4, 64), device="cuda")
     out = torch.full_like(q, 7.0)

@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     cluster_share(a, kRows, kUnit, &share, &cluster_item);
     if (share.begin >= share.end && threadIdx.x < kRows) block_ml[threadIdx.x] = make_float2(-INFINITY, 0.f);
   } else {
-    griddep_launch_dependents();
+    if (a.part_o != nullptr) griddep_launch_dependents();  // the join
     const bool any = find_share(a, kRows, kUnit, &share);
     if (threadIdx.x == 0 && a.part_of != nullptr) a.part_of[blockIdx.x] = PartOf{};
     if (!any) return;

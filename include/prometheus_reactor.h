@@ -1683,7 +1683,9 @@ PROM_REACTOR_API int oct_b200_selftest_wait_timeout(void* handle, uint64_t budge
    clears the device status words the kernels write: returns PROM_ERROR with
    OCT_B200_DETAIL_DEVICE_TIMEOUT if a bounded in-kernel wait gave up,
    OCT_B200_DETAIL_KV4_BAD_INDEX if a cache call skipped what its indices named,
-   or PROM_REDUCTION_DETAIL_NONFINITE_INPUT if a reduction saw NaN/Inf. */
+   or PROM_REDUCTION_DETAIL_NONFINITE_INPUT if a reduction saw NaN/Inf: the first
+   of these that there is.  A skipped index behind a timeout, and a non-finite
+   input behind a skipped index, are the next call's report. */
 PROM_REACTOR_API int oct_b200_sync_status(void* handle, void* stream, int* out_detail_code);
 
 /* No counterpart in the reference.  C = A * B on device pointers (row-major,

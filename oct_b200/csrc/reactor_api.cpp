@@ -1834,8 +1834,10 @@ int oct_b200_sync_status(void* handle, void* stream, int* out_detail_code) {
       if (out_detail_code) *out_detail_code = OCT_B200_DETAIL_CUDA_ERROR;
       return PROM_ERROR;
     }
-    if (reset_words(rt) != cudaSuccess || cudaMemsetAsync(rt->cache_index_word(), 0, 4, rt->stream) != cudaSuccess ||
-        cudaStreamSynchronize(rt->stream) != cudaSuccess) {
+    // one report per call; what it does not tell stays for the next
+    const bool tells_index = w.err == 0 && bad_index != 0;
+    const cudaError_t e = tells_index ? cudaMemsetAsync(rt->cache_index_word(), 0, 4, rt->stream) : reset_words(rt);
+    if (e != cudaSuccess || cudaStreamSynchronize(rt->stream) != cudaSuccess) {
       if (out_detail_code) *out_detail_code = OCT_B200_DETAIL_CUDA_ERROR;
       return PROM_ERROR;
     }
@@ -1843,7 +1845,7 @@ int oct_b200_sync_status(void* handle, void* stream, int* out_detail_code) {
       if (out_detail_code) *out_detail_code = OCT_B200_DETAIL_DEVICE_TIMEOUT;
       return PROM_ERROR;
     }
-    if (bad_index != 0) {
+    if (tells_index) {
       if (out_detail_code) *out_detail_code = OCT_B200_DETAIL_KV4_BAD_INDEX;
       return PROM_ERROR;
     }

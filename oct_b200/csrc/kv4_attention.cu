@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
       if (page < a.view.pages)
         source[h] = (page * a.view.kv_heads + it.head) * a.view.page_tiles + (t + h) - in_table * a.view.page_tiles;
       else
-        atomicOr(a.view.bad, 1u);
+        atomicAdd(a.view.skipped, 1ull);
     }
   };
   // The tiles of step k into its stage; one commit group per call, empty behind the last step.

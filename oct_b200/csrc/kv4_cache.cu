@@ -187,7 +187,7 @@ __device__ __forceinline__ bool find_strip(const Kv4View& v, const Kv4Seq& s, ui
   const uint32_t in_table = tile / v.page_tiles;
   const uint32_t page = static_cast<uint32_t>(v.table[b * v.table_stride + in_table]);
   if (page >= v.pages) {
-    if (threadIdx.x % 32 == 0) atomicOr(v.bad, 1u);
+    if (threadIdx.x % 32 == 0) atomicAdd(v.skipped, 1ull);
     return false;
   }
   p->tile = kv4_tile(v, page, p->head, tile - in_table * v.page_tiles, G::kBytes);
@@ -197,7 +197,7 @@ __device__ __forceinline__ bool find_strip(const Kv4View& v, const Kv4Seq& s, ui
 // Strips of a sequence; reports rows before position 0, which none covers.
 template <int D, bool kWhole>
 __device__ __forceinline__ uint32_t strips_of(const Kv4View& v, const Kv4Seq& s) {
-  if (s.n > s.len && threadIdx.x == 0 && blockIdx.x == 0) atomicOr(v.bad, 1u);
+  if (s.n > s.len && threadIdx.x == 0 && blockIdx.x == 0) atomicAdd(v.skipped, 1ull);
   if (s.n == 0 || s.len == 0) return 0;
   const uint32_t tile0 = (s.n > s.len ? 0u : s.len - s.n) / kKv4Tile;
   return ((s.len + kKv4Tile - 1) / kKv4Tile - tile0) * v.kv_heads * (kWhole ? 1 : 2 * Geometry<D>::kStrips);

@@ -196,7 +196,7 @@ Runtime* create_runtime(const PrometheusReactorConfig* cfg, int* status) {
   if (cudaStreamCreateWithFlags(&rt->stream, cudaStreamNonBlocking) != cudaSuccess ||
       cudaEventCreate(&rt->ev0) != cudaSuccess || cudaEventCreate(&rt->ev1) != cudaSuccess ||
       rt->words.ensure(32, rt->stream) != cudaSuccess || reset_words(rt) != cudaSuccess ||
-      cudaMemsetAsync(rt->cache_index_word(), 0, 4, rt->stream) != cudaSuccess ||
+      cudaMemsetAsync(rt->skipped_word(), 0, 8, rt->stream) != cudaSuccess ||
       cudaStreamSynchronize(rt->stream) != cudaSuccess) {
     rt->reason = PROM_REASON_VULKAN_UNAVAILABLE;
     *status = PROM_OK;
@@ -1828,25 +1828,22 @@ int oct_b200_sync_status(void* handle, void* stream, int* out_detail_code) {
       return PROM_ERROR;
     }
     Words w;
-    unsigned int bad_index = 0;
-    if (cudaMemcpyAsync(&bad_index, rt->cache_index_word(), 4, cudaMemcpyDeviceToHost, rt->stream) != cudaSuccess ||
-        read_words(rt, &w) != cudaSuccess) {
+    if (read_words(rt, &w) != cudaSuccess) {
       if (out_detail_code) *out_detail_code = OCT_B200_DETAIL_CUDA_ERROR;
       return PROM_ERROR;
     }
     // one report per call; what it does not tell stays for the next
-    const bool tells_index = w.err == 0 && bad_index != 0;
-    const cudaError_t e = tells_index ? cudaMemsetAsync(rt->cache_index_word(), 0, 4, rt->stream) : reset_words(rt);
-    if (e != cudaSuccess || cudaStreamSynchronize(rt->stream) != cudaSuccess) {
+    if (w.err == 0 && w.skipped != rt->skipped_told) {
+      rt->skipped_told = w.skipped;
+      if (out_detail_code) *out_detail_code = OCT_B200_DETAIL_KV4_BAD_INDEX;
+      return PROM_ERROR;
+    }
+    if (reset_words(rt) != cudaSuccess || cudaStreamSynchronize(rt->stream) != cudaSuccess) {
       if (out_detail_code) *out_detail_code = OCT_B200_DETAIL_CUDA_ERROR;
       return PROM_ERROR;
     }
     if (w.err != 0) {
       if (out_detail_code) *out_detail_code = OCT_B200_DETAIL_DEVICE_TIMEOUT;
-      return PROM_ERROR;
-    }
-    if (tells_index) {
-      if (out_detail_code) *out_detail_code = OCT_B200_DETAIL_KV4_BAD_INDEX;
       return PROM_ERROR;
     }
     if (w.nonfinite != ~0ull) {

@@ -113,7 +113,7 @@ struct Runtime {
   DevBuf scratch;               // split-TF32 operand buffers
   DevBuf da, db, dc;            // staging for host-pointer SGEMM
   DevBuf rin, rout, rw, rinv;   // staging for reductions / RMSNorm
-  DevBuf words;                 // [0] kernel error bits (u32), [8] first non-finite index (u64), [16] cache index (u32)
+  DevBuf words;                 // [0] kernel error bits (u32), [8] first non-finite index (u64), [16] indices skipped (u64)
   AsyncTask tasks[kAsyncSlots];
   int next_task_id = 1;
   AsyncStats async_stats;
@@ -159,11 +159,12 @@ struct Runtime {
   unsigned long long* nonfinite_word() {
     return reinterpret_cast<unsigned long long*>(static_cast<char*>(words.aligned()) + 8);
   }
-  // Set by the cache kernels when an index on the device is out of range.  A word of
-  // its own: the host entries read and clear the one above around their own kernels.
-  unsigned int* cache_index_word() {
-    return reinterpret_cast<unsigned int*>(static_cast<char*>(words.aligned()) + 16);
+  // Counted up by the cache kernels where an index on the device is out of range, and never cleared: a
+  // kernel may count at any time, on any stream, and `skipped_told` is what the last report had seen.
+  unsigned long long* skipped_word() {
+    return reinterpret_cast<unsigned long long*>(static_cast<char*>(words.aligned()) + 16);
   }
+  unsigned long long skipped_told = 0;
 };
 
 
@@ -186,16 +187,17 @@ inline cudaError_t reset_words(Runtime* rt) {
 
 struct Words {
   unsigned int err = 0;
-  unsigned long long nonfinite = ~0ull;
+  unsigned long long nonfinite = ~0ull, skipped = 0;
 };
 
 inline cudaError_t read_words(Runtime* rt, Words* w) {
-  unsigned char host[16];
-  cudaError_t e = cudaMemcpyAsync(host, rt->words.aligned(), 16, cudaMemcpyDeviceToHost, rt->stream);
+  unsigned char host[24];
+  cudaError_t e = cudaMemcpyAsync(host, rt->words.aligned(), 24, cudaMemcpyDeviceToHost, rt->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(rt->stream);
   if (e != cudaSuccess) return e;
   std::memcpy(&w->err, host, 4);
   std::memcpy(&w->nonfinite, host + 8, 8);
+  std::memcpy(&w->skipped, host + 16, 8);
   return cudaSuccess;
 }
 

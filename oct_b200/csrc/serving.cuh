@@ -113,7 +113,7 @@ __device__ __forceinline__ Pair mul(Pair a, Pair b) {
   return r;
 }
 
-// What sequence `b` of a call brings and holds.  False, with *bad set, when the
+// What sequence `b` of a call brings and holds.  False, and counted, when the
 // arrays on the device do not fit the bounds that the host was given: such a
 // sequence is skipped and nothing of it is read or written.
 struct Kv4Seq {
@@ -131,7 +131,7 @@ __device__ __forceinline__ bool kv4_seq(const Kv4View& v, uint32_t b, Kv4Seq* s)
   const bool ok = len >= 0 && static_cast<uint32_t>(len) <= v.max_kv_len && r0 >= 0 && r1 >= r0 &&
                   static_cast<uint64_t>(r1) <= v.tokens && static_cast<uint32_t>(r1 - r0) <= v.max_tokens;
   if (!ok) {
-    atomicOr(v.bad, 1u);
+    atomicAdd(v.skipped, 1ull);
     return false;
   }
   s->row0 = static_cast<uint64_t>(r0);

@@ -51,7 +51,7 @@ struct Kv4View {
   const int32_t* cu_tokens = nullptr;  // null: one token per sequence
   uint32_t max_tokens = 0, max_kv_len = 0;
   uint64_t tokens = 0;  // rows of the call's own tensors
-  unsigned int* bad = nullptr;  // set to 1 when a device-side index is out of range
+  unsigned long long* skipped = nullptr;  // counts the device-side indices that are out of range
 };
 
 struct Kv4RowArgs {

@@ -106,7 +106,7 @@ int check_batch(const OctB200Kv4Cache* c, const OctB200Kv4Batch* b, uint64_t tok
   return 0;
 }
 
-oct::Kv4View view_of(const OctB200Kv4Cache* c, const OctB200Kv4Batch* b, uint64_t tokens, unsigned int* bad) {
+oct::Kv4View view_of(const OctB200Kv4Cache* c, const OctB200Kv4Batch* b, uint64_t tokens, unsigned long long* skipped) {
   oct::Kv4View v;
   v.data = static_cast<uint8_t*>(c->data);
   v.pages = c->pages;
@@ -121,7 +121,7 @@ oct::Kv4View view_of(const OctB200Kv4Cache* c, const OctB200Kv4Batch* b, uint64_
   v.max_tokens = b->max_tokens;
   v.max_kv_len = b->max_kv_len;
   v.tokens = tokens;
-  v.bad = bad;
+  v.skipped = skipped;
   return v;
 }
 
@@ -155,7 +155,7 @@ int run_rows(void* handle, const OctB200Kv4Cache* cache, const OctB200Kv4Batch* 
                           static_cast<const void*>(rows->k), static_cast<const void*>(rows->v)})
       if (!on.holds(p)) return fail(out_detail_code, OCT_B200_DETAIL_INVALID_ARGUMENT);
     oct::Kv4RowArgs a;
-    a.view = view_of(cache, batch, rows->tokens, rt->cache_index_word());
+    a.view = view_of(cache, batch, rows->tokens, rt->skipped_word());
     a.type = static_cast<oct::ElementType>(rows->dtype);
     a.rows[0] = rows->k;
     a.rows[1] = rows->v;
@@ -341,7 +341,7 @@ int oct_b200_kv4_attention_device(void* handle, const OctB200Kv4Cache* cache, co
                           static_cast<const void*>(plan.workspace > 0 ? r->workspace : nullptr)})
       if (!on.holds(p)) return fail(out_detail_code, OCT_B200_DETAIL_INVALID_ARGUMENT);
     oct::Kv4AttnArgs a;
-    a.view = view_of(cache, batch, r->tokens, rt->cache_index_word());
+    a.view = view_of(cache, batch, r->tokens, rt->skipped_word());
     a.type = static_cast<oct::ElementType>(r->dtype);
     a.heads = r->q_heads;
     a.q = r->q;

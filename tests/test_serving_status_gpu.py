@@ -35,3 +35,24 @@ def test_a_bad_index_does_not_hide_a_non_finite_input(runtime):
     assert {runtime.sync_status().detail, runtime.sync_status().detail} == {
         R.DETAIL_KV4_BAD_INDEX, NONFINITE}
     assert runtime.sync_status().ok
+
+
+def test_a_bad_index_reported_while_another_stream_is_asked(runtime):
+    """The kernel that skips may end at any time of a status call that waits for another stream: its report is
+    given by that call or by the next one, once."""
+    import torch
+    store = _bad_store(runtime)
+    busy, asked = torch.cuda.Stream(), torch.cuda.Stream()
+    store()
+    assert runtime.sync_status().detail == R.DETAIL_KV4_BAD_INDEX
+    lost = twice = 0
+    for i in range(600):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(busy):
+            torch.cuda._sleep(200 * i)  # 0 to about 60 us
+        store(busy)
+        first = runtime.sync_status(asked).detail
+        torch.cuda.synchronize()
+        reports = [first, runtime.sync_status().detail].count(R.DETAIL_KV4_BAD_INDEX)
+        lost, twice = lost + (reports == 0), twice + (reports == 2)
+    assert (lost, twice) == (0, 0)

@@ -322,6 +322,11 @@ int oct_b200_kv4_attention_device(void* handle, const OctB200Kv4Cache* cache, co
       if (bad == 0)
         bad = check_rows(r->out, r->tokens, r->q_heads, cache->head_dim, r->out_token_stride, r->out_head_stride, vec,
                          true);
+      // over the queries means row for row
+      if (bad == 0 && r->q == r->out &&
+          (used(r->q_token_stride, r->tokens) != used(r->out_token_stride, r->tokens) ||
+           used(r->q_head_stride, r->q_heads) != used(r->out_head_stride, r->q_heads)))
+        bad = OCT_B200_DETAIL_INVALID_ARGUMENT;
       if (bad == 0 && r->lse != nullptr && reinterpret_cast<uintptr_t>(r->lse) % 4 != 0) bad = OCT_B200_DETAIL_UNALIGNED;
       if (bad == 0 && plan.workspace > 0) {
         if (r->workspace == nullptr || r->workspace_bytes < plan.workspace)

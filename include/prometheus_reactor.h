@@ -1580,8 +1580,8 @@ PROM_REACTOR_API int oct_b200_qk_norm_rope_device(void* handle, const OctB200QkN
    quantised in groups of 32 channels to codes 0..15 with a scale and a zero:
      x clamped to +-65504;  z = greatest float16 <= min x;  s = least float16 with z + 15 s >= max x;
      code = (x - z) / s rounded to nearest, ties to even (0 when s = 0);  value = z + s * code.
-   A NaN makes the 32 values of its group NaN; float16 outputs are clamped to +-65504.  Layout of `data`
-   ([pages][kv_heads][page_size / 16] tiles of oct_b200_kv4_tile_bytes(head_dim) bytes):
+   A NaN makes the 32 values of its group NaN; float16 outputs, of the attention too, are clamped to +-65504.
+   Layout of `data` ([pages][kv_heads][page_size / 16] tiles of oct_b200_kv4_tile_bytes(head_dim) bytes):
      key codes [16][head_dim / 2] | key (s, z) float16 pairs [16][head_dim / 32] | the same of the values;
    in a row of codes, channels 32 j + 4 g + 0..3 are halfword g * (head_dim / 32) + j, channel + 0 lowest. */
 typedef struct OctB200Kv4Cache {

@@ -221,6 +221,12 @@ __device__ __forceinline__ void lds(uint32_t (&w)[N], const uint8_t* p) {
   }
 }
 
+// A row's four channels from their sums and one over the sum of the weights.
+template <typename T>
+__device__ __forceinline__ float4 result(float4 sum, float inv) {
+  return make_float4(within<T>(sum.x * inv), within<T>(sum.y * inv), within<T>(sum.z * inv), within<T>(sum.w * inv));
+}
+
 // What a block began and did not finish, for the join.
 struct PartOf {
   uint32_t last1 = 0;  // the last block with a part of it, plus 1; 0: nothing was left unfinished
@@ -1018,8 +1024,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
         const uint64_t token = row0 + row / a.share;
         const uint32_t qh = head * a.share + row % a.share;
         const float inv = top == -INFINITY ? 0.f : 1.0f / total;
-        store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c4,
-               make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+        store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c4, result<T>(sum, inv));
         if (c4 == 0 && a.lse != nullptr)
           a.lse[token * a.heads + qh] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
       } else if (a.part_o != nullptr) {
@@ -1066,8 +1071,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     const uint64_t token = cluster_item.row0 + row / a.share;
     const uint32_t qh = cluster_item.head * a.share + row % a.share;
     const float inv = top == -INFINITY ? 0.f : 1.0f / total;
-    store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c4,
-           make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+    store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + 4 * c4, result<T>(sum, inv));
     if (c4 == 0 && a.lse != nullptr) a.lse[token * a.heads + qh] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * kLn2;
   }
   __syncwarp();
@@ -1138,8 +1142,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const KernelArgs
       const uint64_t token = of.row0 + row / a.share;
       const uint32_t qh = of.head * a.share + row % a.share;
       const float inv = ml.x == -INFINITY ? 0.f : 1.0f / ml.y;
-      store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + channel,
-             make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+      store4(static_cast<T*>(a.out) + token * a.out_token + qh * a.out_head + channel, result<T>(sum, inv));
       if (channel == 0 && a.lse != nullptr)
         a.lse[token * a.heads + qh] = ml.x == -INFINITY ? -INFINITY : (ml.x + log2f(ml.y)) * kLn2;
     }

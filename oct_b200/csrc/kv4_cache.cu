@@ -33,24 +33,13 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kPasses = 4;  // row passes whose loads are issued together
-constexpr float kF16Max = 65504.f;
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float min_nan(float a, float b, float c) {
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
   float r;
   asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b, float c) {
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
@@ -135,8 +124,8 @@ __device__ __forceinline__ Raw<T> load_raw(const T* p) {
 
 // Smallest and largest of a lane's eight elements, NaN where one is NaN.
 __device__ __forceinline__ void bounds(const Raw<float>&, const float (&x)[8], float& lo, float& hi) {
-  lo = min_nan(min_nan(x[0], x[1], x[2]), min_nan(x[3], x[4], x[5]), min_nan(x[6], x[7]));
-  hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7]));
+  lo = min3_nan(min3_nan(x[0], x[1], x[2]), min3_nan(x[3], x[4], x[5]), min_nan(x[6], x[7]));
+  hi = max3_nan(max3_nan(x[0], x[1], x[2]), max3_nan(x[3], x[4], x[5]), max_nan(x[6], x[7]));
 }
 template <typename T>
 __device__ __forceinline__ void bounds(const Raw<T>& raw, const float (&)[8], float& lo, float& hi) {
@@ -324,11 +313,8 @@ __global__ void __launch_bounds__(kThreads, 12) kv4_load_kernel(const Kv4RowArgs
                              pair_of(-8388608.f, -8388608.f));
           split(fma(c, pair_of(sz.x, sz.x), pair_of(sz.y, sz.y)), x[2 * i], x[2 * i + 1]);
         }
-        if constexpr (std::is_same<T, __half>::value) {
-          // z + 15 s may lie a step behind a clamped row's 65504: no finite row reads back as infinite
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = min_nan(max_nan(x[i], -kF16Max), kF16Max);
-        }
+        for (int i = 0; i < 8; ++i) x[i] = within<T>(x[i]);
         store8(out + p * G::kRowsPerPass * stride, x);
       }
     }

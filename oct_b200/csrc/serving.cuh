@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "ptx.cuh"
 #include "serving.h"
 
@@ -81,6 +83,23 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   w.z = pack2(v[4], v[5], T());
   w.w = pack2(v[6], v[7], T());
   *reinterpret_cast<uint4*>(p) = w;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// What reads back from the cache may lie a step (half of s) behind a clamped row's 65504: as float16 it is
+// clamped there, so that no finite row becomes infinite; NaN stays NaN.
+constexpr float kF16Max = 65504.f;
+template <typename T>
+__device__ __forceinline__ float within(float x) {
+  return std::is_same<T, __half>::value ? min_nan(max_nan(x, -kF16Max), kF16Max) : x;
 }
 // Four consecutive elements.
 __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }

@@ -1164,20 +1164,28 @@ cudaError_t launch(const KernelArgs& a, const Kv4Plan& plan, cudaStream_t stream
   constexpr int PP = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
   constexpr size_t kSmem = static_cast<size_t>(kWarps) * G::kStages * G::kBytes;
   const auto kernel = kv4_attention_kernel<T, D, NT, QP, PP>;
-  // the attribute stays with the device's function: set once on each
-  static std::atomic<uint64_t> set{0};
+  // the attributes stay with the device's function, and so does the largest cluster that it has room for (a
+  // part of a GPU may have less than all of one): set and asked once on each
+  static std::atomic<uint32_t> most[64];
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
-  const uint64_t bit = 1ull << (device & 63);
-  if (device > 63 || (set.load(std::memory_order_acquire) & bit) == 0) {
+  uint32_t fits = device < 64 ? most[device].load(std::memory_order_acquire) : 0;
+  if (fits == 0) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    set.fetch_or(bit, std::memory_order_release);
+    fits = kv4_cluster_to_launch(kMaxCluster, [&](uint32_t n) { return has_room(kernel, kThreads, kSmem, n); });
+    if (device < 64) most[device].store(fits, std::memory_order_release);
   }
-  e = launch_dependent(kernel, dim3(plan.blocks), kThreads, kSmem, stream, a.cluster, a);
+  uint32_t blocks = plan.blocks;
+  KernelArgs args = a;
+  if (plan.cluster > fits) {
+    args.cluster = fits;
+    blocks = plan.blocks / plan.cluster * fits;
+  }
+  e = launch_dependent(kernel, dim3(blocks), kThreads, kSmem, stream, args.cluster, args);
   if (e != cudaSuccess || plan.workspace == 0) return e;
   // Few items have many parts each: narrower blocks give a row's parts to more threads (8 items of 54
   // parts: 55 us against 58 of the whole call).  Many items have a few: fewer blocks start faster (439

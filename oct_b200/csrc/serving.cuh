@@ -33,6 +33,26 @@ cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, uint32_t threads, 
   cfg.numAttrs = cluster > 0 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
+// Whether the current device has room for a cluster of that many blocks.
+template <typename... P>
+bool has_room(void (*kernel)(P...), uint32_t threads, size_t smem, uint32_t cluster) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  return clusters > 0;
+}
 
 template <ElementType T> struct Element;
 template <> struct Element<kF32> { using type = float; };

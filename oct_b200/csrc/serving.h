@@ -76,6 +76,14 @@ struct Kv4Plan {
 };
 Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint32_t batch, uint32_t max_tokens,
                            uint32_t max_kv_len, uint32_t window, ElementType type);
+// The blocks of a cluster to launch where `wanted` (a power of two) are planned: halved until `places`, asked once
+// per size, says that the device has room for one such cluster.  Every size gives the same parts of the work to
+// some block, so what a smaller one costs is time.
+template <typename Places>
+uint32_t kv4_cluster_to_launch(uint32_t wanted, Places places) {
+  while (wanted > 1 && !places(wanted)) wanted /= 2;
+  return wanted;
+}
 struct Kv4AttnArgs {
   Kv4View view;
   ElementType type = kF32;

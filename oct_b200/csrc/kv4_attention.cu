@@ -93,7 +93,7 @@ constexpr uint32_t kMaxCluster = 16;
 // against 43.9 (32); fp32, 8 / 1 heads of 256, one of 4096 15.6 against 16.4 (4), of 8192 22.0 against 20.3 (8).
 constexpr uint32_t cluster_units(ElementType type) { return type == kF32 ? 4 : 8; }
 // Blocks per SM that the compiler leaves registers for, and that a launch fills.
-constexpr int blocks_per_sm(int dim, int row_groups, int query_parts) { return dim * row_groups <= 128 ? 3 : 2; }
+constexpr int blocks_per_sm(int dim, int row_groups) { return dim * row_groups <= 128 ? 3 : 2; }
 // Query rows of one block in groups of 8, by what the accumulators leave of the registers.
 template <int D> constexpr int kMaxRowGroups = D == 64 ? 4 : (D == 128 ? 2 : 1);
 
@@ -395,7 +395,7 @@ __device__ __forceinline__ void cluster_share(const KernelArgs& a, uint32_t rows
 __device__ __forceinline__ uint32_t finite_half(uint32_t bits) { return (bits & 0x7c00u) == 0x7c00u ? 0u : bits; }
 
 template <typename T, int D, int NT, int QP, int PP>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attention_kernel(const KernelArgs a) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) kv4_attention_kernel(const KernelArgs a) {
   using G = Geometry<D>;
   constexpr int NG = G::kGroups;
   constexpr int kRows = 8 * NT;
@@ -627,15 +627,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT, QP)) kv4_attent
     auto step = [&](const uint8_t* stage, int32_t key0, uint32_t there, auto masked_tag) {
       constexpr bool kMasked = decltype(masked_tag)::value;
       int32_t at[H];            // position of a tile's first token; behind every key when it is not there
-      bool keep[H][2];          // tokens that some row sees: what lies outside may be any bits
       bool vis[H][NT][4];
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        at[h] = kMasked && !((there >> h) & 1u) ? kNowhere : key0 + 16 * h;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          keep[h][r] = !kMasked || (at[h] + tok_g + 8 * r >= rows.lo_min && at[h] + tok_g + 8 * r <= rows.hi_max);
-      }
+      for (int h = 0; h < H; ++h) at[h] = kMasked && !((there >> h) & 1u) ? kNowhere : key0 + 16 * h;
       // ---- scores
       float raw[H][NT][4];
 #pragma unroll
@@ -1240,7 +1234,7 @@ Kv4Plan kv4_attention_plan(uint32_t dim, uint32_t kv_heads, uint32_t heads, uint
   const uint64_t unit = kWarps * tiles_per_step(static_cast<int>(dim), static_cast<int>(p.row_tile / 8));
   const uint64_t item = tiles <= unit ? 1 : (tiles + unit - 1) / unit;
   const uint64_t items = static_cast<uint64_t>(batch) * kv_heads * p.row_tiles;
-  const uint64_t resident = 148ull * blocks_per_sm(static_cast<int>(dim), static_cast<int>(p.row_tile / 8), type == kF32 ? 2 : 1);
+  const uint64_t resident = 148ull * blocks_per_sm(static_cast<int>(dim), static_cast<int>(p.row_tile / 8));
   p.run = items * (item + kItemCost);
   // Few items of a few units: a cluster of blocks for each, which joins it in shared memory, needs no
   // workspace and looks at no other sequence's length.

@@ -45,7 +45,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
-// What rounding d = x - z lost: x - z = d + the result, exactly.
+// What rounding d = x - z lost: x - z = d + the result, exactly (Knuth's two-sum, of x and -z).
 __device__ __forceinline__ float difference_error(float x, float z, float d) {
   const float bb = d - x;
   return (x - (d - bb)) + (-z - bb);

@@ -1639,15 +1639,25 @@ PROM_REACTOR_API int oct_b200_kv4_load_device(void* handle, const OctB200Kv4Cach
    sequence: out = softmax(scale q k^T) v, query head h with key head
    h / (q_heads / kv_heads).  With causal, the query at position p sees keys <= p
    and, with a window, keys > p - window; without, every key of its sequence.  A
-   query that sees nothing gets zeros and lse = -inf.  Scores and sums are fp32,
-   for queries below 2^113.  lse (may be NULL) is the
-   natural logarithm of the softmax's sum, [tokens][q_heads].  out may be q itself
-   (same strides) and overlap no other part of it.  The workspace
-   (oct_b200_kv4_attention_workspace_bytes of the same sizes; NULL when that is
-   0) is used between this call's kernels only: calls that may run at the same
-   time, graphs too, need one each.  Meant for the few tokens of a decode or
-   verification step; more work the same, 8 to 32 rows of (token, query head) per
-   pass over the keys. */
+   query that sees nothing gets zeros and lse = -inf.  lse (may be NULL) is the
+   natural logarithm of the softmax's sum, [tokens][q_heads], in fp32.
+   out may be q itself (same strides, or the call is refused) and overlap no other
+   part of it.
+   Scores, the softmax's maxima and sums, and results are kept in fp32, for queries
+   below 2^113; what enters the matrix products has fewer bits.  Scores, and lse
+   with them, are off by at most 2^-20 of the largest scale * sum |q| (|z| + 15 s)
+   of a key that the row sees, beside fp32's own rounding.  Measured, lse is 3e-6
+   off for bf16 rows over up to 16384 keys (their products of keys keep about 18
+   bits) and 1e-6 for fp16 rows over 131071.  A weight has 12 bits in a bf16 call
+   and 22 in the others, and so has its product with a value's s.  Rows handled
+   together (up to 32 of one key head) share a unit, set by the largest s among the
+   values that any of them sees: of that s, a row's weights are exact to 2^-34 (2^-36
+   where s < 1/4) and what a key adds to a result to 2^-30.
+   The workspace (oct_b200_kv4_attention_workspace_bytes of the same sizes; NULL
+   when that is 0) is used between this call's kernels only: calls that may run at
+   the same time, graphs too, need one each.  Meant for the few tokens of a decode
+   or verification step; more work the same, 8 to 32 rows of (token, query head)
+   per pass over the keys. */
 typedef struct OctB200Kv4AttentionRequest {
   uint32_t struct_size;
   uint32_t dtype;    /* of q and out */

@@ -1244,7 +1244,8 @@ class Runtime:
         adjacent channels; an output may be its input; k and k_out may be None.  positions: int32
         [tokens][axes] (or [tokens]); frequencies: fp64 [rotary_dim / 2], radians per position, whose
         pairs go to the axes in order, axis_pairs[i] each (default: one axis).  Weights: fp32 [head_dim]
-        or None."""
+        or None.  stream: a torch or CUDA stream; None is the CUDA default stream, whatever torch's current
+        one is (in the calls below too)."""
         dtype, shape, pairs = _element_type(q), q.shape, frequencies.numel()
         if axis_pairs is None:
             axis_pairs = (pairs,)

@@ -370,3 +370,87 @@ def test_spread_calls_at_once_on_two_streams(runtime):
     _ok(runtime)
     for pool, table, held, _, q, out, lse, _ in parts:
         _check(pool, "f16", table, held, [1] * 4, q, out, lse)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim, ratio", [(64, 30), (64, 1000), (128, 100), (256, 30), (256, 1000)])
+def test_queries_with_channels_that_stand_out(runtime, kind, dim, ratio):
+    """One channel of every group of 32 is far larger than the others (of either sign, or all positive), so that the
+    products of the others are small beside those they are added to."""
+    rng = np.random.default_rng(8 + dim + ratio)
+    held, new = [1500, 40000], [4, 1]
+    pool = Pool(rng, dim, 1, 16, 200)
+    table = pool.random_table(rng, held)
+    batch = pool.batch(table, held, new)
+    for positive in (False, True):
+        x = rng.standard_normal((5, 8, dim))
+        x = np.abs(x) if positive else x
+        x[:, :, 5::32] *= ratio
+        q = _torch(x, kind)
+        scale = 8.0 / (2.0 * (ratio * dim / 32 + dim))
+        out, lse, _ = _run(runtime, pool, batch, q, scale=scale)
+        _ok(runtime)
+        _check(pool, kind, table, held, new, q, out, lse, scale=scale)
+
+
+def test_a_step_on_torchs_current_stream(runtime):
+    """Norm and rotation, store, attention and status with the stream that torch's own operations of the step are
+    on, then the same captured: what an inference loop under torch.cuda.stream or torch.cuda.graph does."""
+    import torch
+    heads, kv, dim, page, sequences = 8, 2, 64, 16, 3
+    data = torch.zeros((3 * 20 * kv, R.kv4_tile_bytes(dim)), dtype=torch.uint8, device="cuda")
+    cache = R.Kv4Cache(data, page_size=page, kv_heads=kv, head_dim=dim)
+    table = torch.arange(60, dtype=torch.int32, device="cuda").view(sequences, 20)
+    lens = torch.zeros(sequences, dtype=torch.int32, device="cuda")
+    batch = R.Kv4Batch(table, lens, page_size=page)
+    freq = torch.logspace(0, -4, dim // 2, dtype=torch.float64, device="cuda")
+    w = torch.randn(dim, (heads + 2 * kv) * dim, generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    first = torch.randn(sequences, dim, generator=torch.Generator("cuda").manual_seed(2), device="cuda")
+    state = first.clone()
+    ws = torch.empty(runtime.kv4_attention_workspace_bytes(cache, batch, torch.empty(sequences, heads, dim)),
+                     dtype=torch.uint8, device="cuda")
+
+    def step():
+        s = torch.cuda.current_stream()
+        x = (state @ w).view(sequences, heads + 2 * kv, dim)
+        q, k, v = x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+        pos = lens.clone()
+        lens.add_(1)
+        runtime.qk_norm_rope_device(q, k, q, k, pos, freq, stream=s)
+        runtime.kv4_store_device(cache, batch, k, v, stream=s)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        runtime.kv4_attention_device(cache, batch, q, out, workspace=ws, stream=s)
+        state.copy_(torch.tanh(out.mean(1)) + first)
+
+    def run(once):
+        data.zero_()
+        lens.zero_()
+        state.copy_(first)
+        torch.cuda.synchronize()
+        for _ in range(100):
+            once()
+        torch.cuda.synchronize()
+        return state.clone()
+
+    side = torch.cuda.Stream()
+
+    def waiting():
+        step()
+        torch.cuda.synchronize()
+
+    def beside():
+        with torch.cuda.stream(side):
+            step()
+
+    want = run(waiting)
+    assert runtime.sync_status().ok
+    assert torch.equal(run(beside), want)
+    with torch.cuda.stream(side):
+        step()  # torch's own matrix product sets itself up before the capture
+    assert runtime.sync_status(side).ok
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    assert torch.equal(run(graph.replay), want)
+    assert runtime.sync_status().ok and (lens == 100).all()
+    del graph

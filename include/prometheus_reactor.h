@@ -1648,11 +1648,12 @@ PROM_REACTOR_API int oct_b200_kv4_load_device(void* handle, const OctB200Kv4Cach
    with them, are off by at most 2^-20 of the largest scale * sum |q| (|z| + 15 s)
    of a key that the row sees, beside fp32's own rounding.  Measured, lse is 3e-6
    off for bf16 rows over up to 16384 keys (their products of keys keep about 18
-   bits) and 1e-6 for fp16 rows over 131071.  A weight has 12 bits in a bf16 call
-   and 22 in the others, and so has its product with a value's s.  Rows handled
-   together (up to 32 of one key head) share a unit, set by the largest s among the
-   values that any of them sees: of that s, a row's weights are exact to 2^-34 (2^-36
-   where s < 1/4) and what a key adds to a result to 2^-30.
+   bits) and 1e-6 for fp16 rows over 131071.  A weight is rounded by at most 2^-12
+   of it in a bf16 call and 2^-22 in the others, and so is its product with a
+   value's s.  Rows handled together (up to 32 of one key head) share a unit, set
+   by the largest s among the values that any of them sees: with a row's largest
+   weight as 1, weights are exact to 2^-34 of that s (2^-36 where s < 1/4) and what
+   a key adds to a result to 2^-30 of it.
    The workspace (oct_b200_kv4_attention_workspace_bytes of the same sizes; NULL
    when that is 0) is used between this call's kernels only: calls that may run at
    the same time, graphs too, need one each.  Meant for the few tokens of a decode

@@ -1033,6 +1033,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, NT)) kv4_attention_
   }
   if (a.cluster == 0) return;
   // The cluster's blocks have their parts in shared memory; each joins its share of the item's results.
+  __syncwarp();  // the barrier takes whole warps, and a block without a part comes here from a branch of its first threads
   cluster_sync();
   const uint32_t count = cluster_item.count;
   const float* const parts = reinterpret_cast<const float*>(smem + (kStages - kResultStages) * kStageBytes);

@@ -1643,8 +1643,8 @@ PROM_REACTOR_API int oct_b200_kv4_load_device(void* handle, const OctB200Kv4Cach
    natural logarithm of the softmax's sum, [tokens][q_heads], in fp32.
    out may be q itself (same strides, or the call is refused) and overlap no other
    part of it.
-   Scores, the softmax's maxima and sums, and results are kept in fp32, for queries
-   below 2^113; what enters the matrix products has fewer bits.  Scores, and lse
+   Scores, the softmax's maxima and sums, and results are kept in fp32, for queries,
+   and scale times them, below 2^113; what enters the matrix products has fewer bits.  Scores, and lse
    with them, are off by at most 2^-20 of the largest scale * sum |q| (|z| + 15 s)
    of a key that the row sees, beside fp32's own rounding.  Measured, lse is 3e-6
    off for bf16 rows over up to 16384 keys (their products of keys keep about 18
@@ -1665,7 +1665,7 @@ typedef struct OctB200Kv4AttentionRequest {
   uint32_t q_heads;  /* a multiple of kv_heads */
   uint32_t causal;
   uint32_t window;   /* 0: none; needs causal */
-  float scale;       /* finite */
+  float scale;       /* magnitude below 2^100 */
   uint64_t tokens;
   const void* q;     /* [tokens][q_heads][head_dim] by its strides */
   void* out;

@@ -18,6 +18,9 @@ int fail(int* detail, int code) {
 
 constexpr uint64_t kMaxStride = 1ull << 32;  // elements; times 2^31 rows it stays below 2^64
 
+// Of the attention's scale: times 2^24 and log2(e), which the kernel makes of it, it stays finite.
+constexpr float kMaxScale = 0x1p100f;
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Elements of `dtype` in 16 bytes; 0 for an unknown type.
@@ -178,7 +181,7 @@ int check_attention(const OctB200Kv4Cache* c, const OctB200Kv4Batch* b, const Oc
   int bad = check_cache(c);
   if (bad != 0) return bad;
   if (r == nullptr || r->struct_size < sizeof(OctB200Kv4AttentionRequest) || vector_elements(r->dtype) == 0 ||
-      r->q_heads == 0 || r->q_heads % c->kv_heads != 0 || !std::isfinite(r->scale) ||
+      r->q_heads == 0 || r->q_heads % c->kv_heads != 0 || !(std::fabs(r->scale) < kMaxScale) ||
       (r->window != 0 && r->causal == 0))
     return OCT_B200_DETAIL_INVALID_ARGUMENT;
   bad = check_batch(c, b, r->tokens);

@@ -4,7 +4,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from tests.test_serving_gpu import Host, _attend, _np, _ok, _torch, _wide
+from tests.test_serving_gpu import Host, _attend, _check_attention, _np, _ok, _torch, _wide
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,20 @@ def test_float16_results_stay_finite_where_rows_were(runtime, dim, spread):
     assert (got[0, :, 1::2] == 65504.0).all() and (got[1, :, 33::2] == -65504.0).all()
     assert (np.abs(got[0, :, 0::2] + 100.0) <= 100.0 * 2.0 ** -11 + 65536 * 2.0 ** -20).all()
     assert torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("exponent", [-120, -98, 60, 110])
+def test_queries_at_the_ends_of_their_range(runtime, kind, exponent):
+    """Tiny and huge queries whose scale brings the scores back to the ordinary; a row of zeros weighs all keys alike."""
+    rng = np.random.default_rng(abs(exponent))
+    host = Host(rng, 128, 1, 16, [2, 1], [600, 40])
+    host.fill(rng)
+    x = np.clip(rng.standard_normal((3, 8, 128)), -3.9, 3.9)
+    x[0, 5] = 0.0
+    q = _torch(x * 2.0 ** exponent, kind)
+    scale = float(np.float32(min(0.1 * 2.0 ** -exponent, 2.0 ** 99)))
+    out, lse, _ = _attend(runtime, host, q, 8, scale=scale)
+    _ok(runtime)
+    assert np.isfinite(_np(out)).all()
+    _check_attention(host, kind, q, out, lse, scale=scale)

@@ -31,3 +31,17 @@ def test_attention_over_its_queries_keeps_their_strides(lib, handle, change, cod
     detail = C.c_int()
     rc = lib.oct_b200_kv4_attention_device(handle, _cache(), _batch(), _attention(**change), None, detail)
     assert (rc, detail.value) == (R.PROM_ERROR, code)
+
+
+@pytest.mark.parametrize("scale, code", [
+    (2.0 ** 99, NO_DEVICE), (-2.0 ** 99, NO_DEVICE), (2.0 ** 100, INVALID), (-2.0 ** 127, INVALID), (3e38, INVALID),
+    (float("nan"), INVALID), (0.0, NO_DEVICE), (1e-45, NO_DEVICE),
+])
+def test_a_scale_whose_factors_would_not_be_finite_is_refused(lib, handle, scale, code):
+    """The kernel multiplies a scale by powers of two up to 2^24 and by log2(e) on its way to a score: a row of zero
+    queries must not meet an infinite factor."""
+    detail, size = C.c_int(), C.c_uint64()
+    rc = lib.oct_b200_kv4_attention_device(handle, _cache(), _batch(), _attention(scale=scale), None, detail)
+    assert (rc, detail.value) == (R.PROM_ERROR, code)
+    rc = lib.oct_b200_kv4_attention_workspace_bytes(_cache(), _batch(), _attention(scale=scale), size, detail)
+    assert (rc, detail.value) == ((R.PROM_OK, 0) if code == NO_DEVICE else (R.PROM_ERROR, INVALID))
